@@ -42,12 +42,15 @@ enum b2_status_code {
 };
 
 enum b2_dtype { B2_F32 = 0, B2_BF16 = 1 };
+/* Element types of the 8-bit KV cache (the *_q8 entry points' cache_dtype). */
+enum b2_cache_dtype { B2_I8 = 2, B2_E4M3 = 3 };
 
 /* Device-side error bits ORed into *status by kernels. */
 enum b2_device_error {
   B2_DEV_RANGE = 1,        /* position >= max_seq_len, block index past the table, bad block id, bad token id */
   B2_DEV_PIPE_TIMEOUT = 2, /* an in-kernel pipeline wait (mbarrier) ran out of its bound */
-  B2_DEV_PEER_TIMEOUT = 4  /* a peer flag was not raised before the all-reduce timeout */
+  B2_DEV_PEER_TIMEOUT = 4, /* a peer flag was not raised before the all-reduce timeout */
+  B2_DEV_NO_BLOCKS = 8     /* the free ring holds fewer KV blocks than a call needs */
 };
 
 /* ---------------------------------------------------------------- library */
@@ -222,6 +225,106 @@ int b2_prefill_attention_tc(const void* q, int64_t ld_q, int n_rows, int nq, int
                             const int32_t* block_tables, int table_stride, const int32_t* seq_start,
                             const int32_t* seq_ctx0, int n_seqs, float scale, void* out, int64_t ld_out, int dtype,
                             int32_t* status, b2_stream_t stream);
+
+/* ---------------------------------------------------------------- block tables and slot maps
+ * The per-step bookkeeping of engine/model/kv_cache.py:172-227 (blocks taken from and given
+ * back to a FIFO free list) and of attention.py:166-184 (a slot per token) on the device.
+ * Sequence s (0 <= s < n_seqs <= 16384) is row s of block_tables [n_seqs, table_stride] int32
+ * and holds ceil(lens[s] / block_size) blocks.  free_ring [num_blocks] int32 holds the free
+ * block ids; free_state int32 [4] = {head, count, 0, 0}.  Calls on one state must be stream
+ * ordered.
+ *
+ * extend: every sequence takes the blocks its new_lens[s] >= 0 tokens need, in sequence order
+ * from the ring's head, and lens[s] += new_lens[s].  For the new tokens, numbered sequence by
+ * sequence, i = 0 .. total-1:
+ *   seq_start [n_seqs + 1]: the first token of each sequence, and the total
+ *   positions[i] (int64) in its sequence, table_index[i] = its sequence, slots[i] (int64) =
+ *   block * block_size + offset, ctx_lens[i] = positions[i] + 1
+ *   last_rows [n_seqs] (int64): the sequence's last new token, -1 where it has none.
+ * The maps hold max_tokens entries; those behind the total are left as they were.  With
+ * free_ring and free_state NULL nothing is taken and lens stays as it is: the maps of tokens
+ * whose blocks block_tables already names (an entry outside [0, num_blocks) gives slot -1 and
+ * B2_DEV_RANGE).
+ *
+ * truncate: sequences longer than keep_lens[s] >= 0 give the blocks behind their first
+ * keep_lens[s] tokens back to the ring's tail, in sequence and then table order; the entries
+ * become -1 and lens[s] = min(lens[s], keep_lens[s]).
+ *
+ * A call that cannot be served whole (a negative length, a sequence past its table row, more
+ * than max_tokens tokens, a ring that would overflow: B2_DEV_RANGE; too few free blocks:
+ * B2_DEV_NO_BLOCKS) raises its bit in *status and changes nothing, maps included. */
+int b2_block_tables_extend(int32_t* block_tables, int n_seqs, int table_stride, int32_t* lens,
+                           const int32_t* new_lens, int block_size, int32_t* free_ring, int num_blocks,
+                           int32_t* free_state, int max_tokens, int32_t* seq_start, int64_t* positions,
+                           int32_t* table_index, int64_t* slots, int32_t* ctx_lens, int64_t* last_rows,
+                           int32_t* status, b2_stream_t stream);
+int b2_block_tables_truncate(int32_t* block_tables, int n_seqs, int table_stride, int32_t* lens,
+                             const int32_t* keep_lens, int block_size, int32_t* free_ring, int num_blocks,
+                             int32_t* free_state, int32_t* status, b2_stream_t stream);
+
+/* ---------------------------------------------------------------- q/k norms + RoPE + paged KV write
+ * b2_rope_kv_write with an RMS norm of every q and k head before the rotation:
+ * y = x * rsqrt(mean(x^2) + eps) * weight over head_dim, weight float32 [head_dim] (NULL: no
+ * norm).  Everything is computed in float32 and rounded once, when it is stored; with both
+ * weights NULL the outputs are those of b2_rope_kv_write, bit for bit.  head_dim 32, 64 or 128.
+ * block_tables has table_rows rows; a token whose table_index or position lies outside is
+ * skipped and raises B2_DEV_RANGE.
+ *
+ * The _q8 form writes the 8-bit cache: k_cache/v_cache [L, num_blocks, nkv, 16, head_dim] of
+ * cache_dtype (B2_I8 or B2_E4M3), k_scale/v_scale float32 [L, num_blocks, nkv]; a stored value
+ * is code * scale.  block_size 16.  The tokens of one sequence must be consecutive and in
+ * order of position; those that fall into one block form a run.  Per (run, kv head):
+ *   scale = max|x| / 127 (B2_I8) or / 448 (B2_E4M3), 0 where that is below 2^-126;
+ *   a run that begins inside a block keeps the block's scale if it is larger, else the codes
+ *   in the slots before the run are rounded again: code * old_scale / scale;
+ *   code = x / scale to nearest even, saturating.
+ * A value that is not finite makes the tile's scale NaN until the block is begun anew.  Slots
+ * behind the run keep their codes.  Two runs of one call must not meet in one block. */
+int b2_qk_norm_rope_kv_write(const void* qkv, int64_t ld_qkv, int n_tokens, int nq, int nkv, int head_dim,
+                             const float* q_weight, const float* k_weight, float eps, const int64_t* rope_pos,
+                             const int64_t* store_pos, const int32_t* table_index, const int32_t* block_tables,
+                             int table_rows, int table_stride, int num_blocks, int block_size, const float* cos,
+                             const float* sin, int max_seq_len, void* q_out, void* k_cache, void* v_cache, int layer,
+                             int dtype, int32_t* status, b2_stream_t stream);
+int b2_qk_norm_rope_kv_write_q8(const void* qkv, int64_t ld_qkv, int n_tokens, int nq, int nkv, int head_dim,
+                                const float* q_weight, const float* k_weight, float eps, const int64_t* rope_pos,
+                                const int64_t* store_pos, const int32_t* table_index, const int32_t* block_tables,
+                                int table_rows, int table_stride, int num_blocks, int block_size, const float* cos,
+                                const float* sin, int max_seq_len, void* q_out, void* k_cache, void* v_cache,
+                                float* k_scale, float* v_scale, int cache_dtype, int layer, int dtype,
+                                int32_t* status, b2_stream_t stream);
+
+/* The values of blocks block_ids[0 .. n_blocks) of one layer of the 8-bit cache: k_out, v_out
+ * [n_blocks, 16, nkv, head_dim] of out_dtype = code * scale (kv_cache.py:121-147 for this
+ * cache).  An id outside the pool gives zeros and raises B2_DEV_RANGE. */
+int b2_kv_read_q8(const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
+                  int cache_dtype, int layer, int num_blocks, int block_size, int nkv, int head_dim,
+                  const int32_t* block_ids, int n_blocks, void* k_out, void* v_out, int out_dtype, int32_t* status,
+                  b2_stream_t stream);
+
+/* ---------------------------------------------------------------- attention over the 8-bit cache
+ * b2_paged_attention and b2_prefill_attention over the cache that b2_qk_norm_rope_kv_write_q8
+ * writes; q and out are of dtype (B2_BF16 or B2_F32).  block_size 16, head_dim 32, 64 or 128,
+ * nq/nkv 1..16; other shapes return B2_ENOTSUP.  q, out and their row strides and the caches
+ * must be 16-byte aligned.  The split of the work over the context is made on the device from
+ * ctx_lens (seq_start, seq_ctx0), so there is no split count.  workspace: at least
+ * *_workspace_bytes() bytes, in any state; calls that may overlap on the GPU need one each.
+ * A row that sees no key gives zeros; rows behind the last sequence of a prefill are left as
+ * they were.  Keys behind a row's context are never used, whatever their codes and scales. */
+size_t b2_paged_attention_q8_workspace_bytes(int n_rows, int nq, int nkv, int head_dim);
+int b2_paged_attention_q8(const void* q, int64_t ld_q, int n_rows, int nq, int nkv, int head_dim, const void* k_cache,
+                          const void* v_cache, const float* k_scale, const float* v_scale, int cache_dtype, int layer,
+                          int num_blocks, int block_size, const int32_t* block_tables, int table_rows,
+                          int table_stride, const int32_t* table_index, const int32_t* ctx_lens, int compat_pad,
+                          float scale, void* out, int64_t ld_out, int dtype, void* workspace, size_t workspace_bytes,
+                          int32_t* status, b2_stream_t stream);
+size_t b2_prefill_attention_q8_workspace_bytes(int n_rows, int nq, int nkv, int head_dim, int n_seqs);
+int b2_prefill_attention_q8(const void* q, int64_t ld_q, int n_rows, int nq, int nkv, int head_dim,
+                            const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
+                            int cache_dtype, int layer, int num_blocks, int block_size, const int32_t* block_tables,
+                            int table_rows, int table_stride, const int32_t* seq_start, const int32_t* seq_ctx0,
+                            int n_seqs, float scale, void* out, int64_t ld_out, int dtype, void* workspace,
+                            size_t workspace_bytes, int32_t* status, b2_stream_t stream);
 
 /* ---------------------------------------------------------------- greedy sampling
  * out[r] = first index of the maximum of logits[r, 0:cols]   (execution_engine.py:103,133) */

@@ -17,8 +17,8 @@ import torch
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libb2tp.so")
 
 B2_OK, B2_EINVAL, B2_ETIMEOUT, B2_ECUDA, B2_ENOTSUP, B2_ERANGE = 0, 1, 2, 3, 4, 5
-B2_F32, B2_BF16 = 0, 1
-B2_DEV_RANGE, B2_DEV_PIPE_TIMEOUT, B2_DEV_PEER_TIMEOUT = 1, 2, 4
+B2_F32, B2_BF16, B2_I8, B2_E4M3 = 0, 1, 2, 3
+B2_DEV_RANGE, B2_DEV_PIPE_TIMEOUT, B2_DEV_PEER_TIMEOUT, B2_DEV_NO_BLOCKS = 1, 2, 4, 8
 
 _c_void_p = ctypes.c_void_p
 _c_int = ctypes.c_int
@@ -92,6 +92,33 @@ _SIGS = {
                                        _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int,
                                        _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int,
                                        _c_void_p, _c_size, _c_void_p, _c_void_p]),
+    "b2_block_tables_extend": (_c_int, [_c_void_p, _c_int, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p,
+                                        _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
+                                        _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
+    "b2_block_tables_truncate": (_c_int, [_c_void_p, _c_int, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p,
+                                          _c_int, _c_void_p, _c_void_p, _c_void_p]),
+    "b2_qk_norm_rope_kv_write": (_c_int, [_c_void_p, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_void_p,
+                                          _c_void_p, _c_float, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
+                                          _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_void_p, _c_int,
+                                          _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_void_p, _c_void_p]),
+    "b2_qk_norm_rope_kv_write_q8": (_c_int, [_c_void_p, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_void_p,
+                                             _c_void_p, _c_float, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
+                                             _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_void_p, _c_int,
+                                             _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int,
+                                             _c_int, _c_int, _c_void_p, _c_void_p]),
+    "b2_kv_read_q8": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int,
+                               _c_int, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p,
+                               _c_void_p]),
+    "b2_paged_attention_q8_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int]),
+    "b2_paged_attention_q8": (_c_int, [_c_void_p, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_void_p,
+                                       _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_int,
+                                       _c_int, _c_void_p, _c_void_p, _c_int, _c_float, _c_void_p, _c_i64,
+                                       _c_int, _c_void_p, _c_size, _c_void_p, _c_void_p]),
+    "b2_prefill_attention_q8_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int, _c_int]),
+    "b2_prefill_attention_q8": (_c_int, [_c_void_p, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_void_p,
+                                         _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int,
+                                         _c_void_p, _c_int, _c_int, _c_void_p, _c_void_p, _c_int, _c_float,
+                                         _c_void_p, _c_i64, _c_int, _c_void_p, _c_size, _c_void_p, _c_void_p]),
 }
 
 _lib: Optional[ctypes.CDLL] = None
@@ -137,7 +164,9 @@ _LAUNCHING = {"b2_embedding", "b2_rmsnorm", "b2_linear", "b2_linear_qkv", "b2_li
               "b2_rope_kv_write", "b2_paged_attention", "b2_argmax", "b2_allreduce_sum", "b2_allreduce_rmsnorm",
               "b2_row_parallel_linear", "b2_allreduce_rmsnorm_sharded", "b2_paged_attention_noalloc",
               "b2_argmax_allgather", "b2_linear_residual_norm", "b2_linear_qkv_rownorm", "b2_linear_swiglu_rownorm",
-              "b2_linear_qkv_rope_kv", "b2_prefill_attention", "b2_prefill_attention_tc"}
+              "b2_linear_qkv_rope_kv", "b2_prefill_attention", "b2_prefill_attention_tc", "b2_block_tables_extend",
+              "b2_block_tables_truncate", "b2_qk_norm_rope_kv_write", "b2_qk_norm_rope_kv_write_q8", "b2_kv_read_q8",
+              "b2_paged_attention_q8", "b2_prefill_attention_q8"}
 
 
 def check(rc: int, what: str = ""):
@@ -165,6 +194,24 @@ def dtype_code(dt: torch.dtype) -> int:
     if dt == torch.bfloat16:
         return B2_BF16
     raise B2Error(f"unsupported dtype {dt}; use torch.float32 or torch.bfloat16")
+
+
+def cache_dtype_code(dt: torch.dtype) -> int:
+    """Element type of the 8-bit KV cache."""
+    if dt == torch.int8:
+        return B2_I8
+    if dt == torch.float8_e4m3fn:
+        return B2_E4M3
+    raise B2Error(f"unsupported cache dtype {dt}; use torch.int8 or torch.float8_e4m3fn")
+
+
+def cache_torch_dtype(name) -> torch.dtype:
+    """The 8-bit cache type a configuration names: ``"int8"`` or ``"fp8_e4m3"``."""
+    if name in (torch.int8, "int8"):
+        return torch.int8
+    if name in (torch.float8_e4m3fn, "fp8_e4m3"):
+        return torch.float8_e4m3fn
+    raise B2Error(f"unsupported KV cache dtype {name!r}; use 'int8' or 'fp8_e4m3'")
 
 
 def torch_dtype(name) -> torch.dtype:
@@ -227,6 +274,8 @@ def raise_for_status(v: int, what: str = "kernel"):
     if v:
         if v & B2_DEV_PEER_TIMEOUT:
             raise TimeoutError(f"{what}: a tensor-parallel peer did not arrive before the all-reduce timeout")
+        if v & B2_DEV_NO_BLOCKS:
+            raise MemoryError(f"{what}: the free ring holds fewer KV blocks than the step needs")
         if v & B2_DEV_RANGE:
             raise IndexError(f"{what}: position, block-table entry or token id out of range")
         raise B2Error(f"{what}: device error bits {v:#x}")

@@ -1,0 +1,475 @@
+// Per-head RMS norm of q and k, rotary embedding and the paged KV write in one pass, into a
+// cache of the model's type or of 8 bits; and the read-back of 8-bit tiles.
+//
+// The rotation and the slots are those of engine/model/attention.py:46-63 and :166-184; the
+// reference has neither the norms nor an 8-bit cache.  For each token and q or k head x
+//   y = x * rsqrt(mean(x^2) + eps) * weight   (no norm where the weight pointer is null)
+//   out[d] = y[d] cos[d] - y[d + h] sin[d],  out[d + h] = y[d + h] cos[d + h] + y[d] sin[d + h],
+// h = head_dim / 2, all in float32 and rounded once when it is stored.  Values are stored as
+// they are.
+//
+// Layout of the work: a group of head_dim / 16 lanes holds one (token, head), each lane 8
+// elements of the lower half and the 8 they rotate with in the upper one, so a head is read
+// and written in 16-byte pieces, the rotation stays within a lane and the mean takes
+// log2(head_dim / 16) shuffles.
+//
+// 8-bit tiles.  The tokens of a call that fall into one block form a run; one warp per (run,
+// head) holds the run's values in registers, takes their largest magnitude and writes codes
+// and scale.  Where the run begins inside a block, the slots before it are history: the tile
+// keeps its old scale if that is larger, else the old codes are rounded again under the new
+// one (code * old / new, to nearest), which a tile's growing maximum makes ever rarer.
+#include "q8.cuh"
+
+namespace b2 {
+namespace {
+
+struct NormRopeParams {
+  const void* qkv;
+  int64_t ld_qkv;
+  int n_tokens, nq, nkv;
+  const float* q_weight;
+  const float* k_weight;
+  float eps;
+  const int64_t* rope_pos;
+  const int64_t* store_pos;
+  const int32_t* table_index;
+  const int32_t* tables;
+  int table_rows, table_stride, num_blocks, bs;
+  const float* cos;
+  const float* sin;
+  int max_seq_len;
+  void* q_out;
+  void* k_cache;
+  void* v_cache;
+  float* k_scale;
+  float* v_scale;
+  int chunk;  // tokens whose runs one block of the tile kernel looks for
+  int32_t* status;
+};
+
+// 8 elements as float32.
+__device__ __forceinline__ void ld8(const float* p, float (&v)[8]) {
+  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ void ld8(const __nv_bfloat16* p, float (&v)[8]) { load16_f32<__nv_bfloat16>(p, v); }
+__device__ __forceinline__ void st8(float* p, const float (&v)[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void st8(__nv_bfloat16* p, const float (&v)[8]) {
+  uint4 o;
+  uint32_t* w = reinterpret_cast<uint32_t*>(&o);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  *reinterpret_cast<uint4*>(p) = o;
+}
+
+// Norm (weight not null) and rotation of one head held by a group of LANES lanes.
+template <int LANES>
+__device__ __forceinline__ void norm_rotate(float (&lo)[8], float (&hi)[8], const float* weight, float eps,
+                                            const float* cos, const float* sin, int li) {
+  constexpr int HALF = LANES * 8;
+  if (weight) {
+    // the other groups of the warp may hold value heads, which do not come here
+    const unsigned group = (LANES == 32 ? 0xffffffffu : (1u << LANES) - 1) << (threadIdx.x % 32 / LANES * LANES);
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss = fmaf(lo[e], lo[e], fmaf(hi[e], hi[e], ss));
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(group, ss, o);
+    const float r = rsqrtf(ss * (1.f / (2 * HALF)) + eps);
+    float wl[8], wh[8];
+    ld8(weight + li * 8, wl);
+    ld8(weight + HALF + li * 8, wh);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      lo[e] = lo[e] * r * wl[e];
+      hi[e] = hi[e] * r * wh[e];
+    }
+  }
+  float cl[8], sl[8], ch[8], sh[8];
+  ld8(cos + li * 8, cl);
+  ld8(sin + li * 8, sl);
+  ld8(cos + HALF + li * 8, ch);
+  ld8(sin + HALF + li * 8, sh);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    // two roundings a product, as the separate rotation kernel: without norms and in the
+    // model's type the two give the same bits
+    const float a = __fadd_rn(__fmul_rn(lo[e], cl[e]), __fmul_rn(-hi[e], sl[e]));
+    const float b = __fadd_rn(__fmul_rn(hi[e], ch[e]), __fmul_rn(lo[e], sh[e]));
+    lo[e] = a;
+    hi[e] = b;
+  }
+}
+
+struct Place {
+  bool rope_ok, slot_ok;
+  int64_t rope;  // position in the tables
+  int64_t block;
+  int64_t pos;  // position in the cache
+  int row;
+};
+
+__device__ __forceinline__ Place place_of(const NormRopeParams& p, int tok) {
+  Place r;
+  r.rope = p.rope_pos[tok];
+  r.pos = p.store_pos ? p.store_pos[tok] : r.rope;
+  r.row = p.table_index ? p.table_index[tok] : tok;
+  r.rope_ok = r.rope >= 0 && r.rope < p.max_seq_len;
+  r.block = -1;
+  if (r.pos >= 0 && r.pos / p.bs < p.table_stride && r.row >= 0 && r.row < p.table_rows)
+    r.block = p.tables[(int64_t)r.row * p.table_stride + r.pos / p.bs];
+  r.slot_ok = r.block >= 0 && r.block < p.num_blocks;
+  return r;
+}
+
+// One (token, head) per lane group: q heads, and with KV the k and v heads of a cache of the
+// model's type.
+template <typename T, int HD, bool KV>
+__global__ void __launch_bounds__(128) qk_norm_rope_kernel(NormRopeParams p) {
+  pdl_wait();
+  pdl_trigger();
+  constexpr int LANES = HD / 16, GROUPS = 128 / LANES, HALF = HD / 2;
+  const int li = threadIdx.x % LANES, grp = threadIdx.x / LANES;
+  const int heads = KV ? p.nq + 2 * p.nkv : p.nq;
+  const int64_t item = (int64_t)blockIdx.x * GROUPS + grp;
+  const int64_t tok_l = item / heads;
+  const bool live = tok_l < p.n_tokens;
+  const int tok = live ? (int)tok_l : p.n_tokens - 1, h = (int)(item % heads);
+  const Place at = place_of(p, tok);
+  const T* src = reinterpret_cast<const T*>(p.qkv) + (int64_t)tok * p.ld_qkv + (int64_t)h * HD + li * 8;
+  float lo[8], hi[8];
+  ld8(src, lo);
+  ld8(src + HALF, hi);
+  if (live && h == 0 && li == 0 && !(at.rope_ok && at.slot_ok)) raise_status(p.status, B2_DEV_RANGE);
+  if (h < p.nq + p.nkv) {
+    const int64_t rope = at.rope_ok ? at.rope : 0;
+    norm_rotate<LANES>(lo, hi, h < p.nq ? p.q_weight : p.k_weight, p.eps, p.cos + rope * HD, p.sin + rope * HD, li);
+  }
+  if (!live || !at.rope_ok) return;
+  T* dst;
+  if (h < p.nq) {
+    dst = reinterpret_cast<T*>(p.q_out) + ((int64_t)tok * p.nq + h) * HD;
+  } else {
+    if (!at.slot_ok) return;
+    const int g = h < p.nq + p.nkv ? h - p.nq : h - p.nq - p.nkv;
+    T* cache = reinterpret_cast<T*>(h < p.nq + p.nkv ? p.k_cache : p.v_cache);
+    dst = cache + ((at.block * p.bs + at.pos % p.bs) * p.nkv + g) * HD;
+  }
+  st8(dst + li * 8, lo);
+  st8(dst + HALF + li * 8, hi);
+}
+
+// Runs and tiles of the 8-bit cache: one warp per (k or v, head), walking the runs that begin
+// among the block's `chunk` tokens.
+template <typename T, int HD, int CODE>
+__global__ void __launch_bounds__(128) kv_write_q8_kernel(NormRopeParams p) {
+  pdl_wait();
+  pdl_trigger();
+  constexpr int LANES = HD / 16, G = 32 / LANES, ITERS = kQ8Block / G, HALF = HD / 2;
+  const int lane = threadIdx.x & 31, li = lane % LANES, grp = lane / LANES;
+  const int head = blockIdx.y * 4 + (threadIdx.x >> 5);  // k heads, then v heads
+  if (head >= 2 * p.nkv) return;
+  const bool is_k = head < p.nkv;
+  const int g = is_k ? head : head - p.nkv;
+  uint8_t* cache = reinterpret_cast<uint8_t*>(is_k ? p.k_cache : p.v_cache);
+  float* scales = is_k ? p.k_scale : p.v_scale;
+  const int t0 = blockIdx.x * p.chunk, t1 = min(p.n_tokens, t0 + p.chunk);
+  for (int t = t0; t < t1; ++t) {
+    const Place at = place_of(p, t);
+    const int off = (int)(at.pos & (kQ8Block - 1));
+    if (!at.slot_ok) continue;
+    if (t > 0 && off > 0) {  // not the first token of its run?
+      const int64_t before = p.store_pos ? p.store_pos[t - 1] : p.rope_pos[t - 1];
+      const int row = p.table_index ? p.table_index[t - 1] : t - 1;
+      if (row == at.row && before + 1 == at.pos) continue;
+    }
+    // Length of the run: lanes 0..15 look at the tokens that could follow.
+    bool in = lane < kQ8Block - off && t + lane < p.n_tokens;
+    if (in) {
+      const int64_t pos = p.store_pos ? p.store_pos[t + lane] : p.rope_pos[t + lane];
+      const int row = p.table_index ? p.table_index[t + lane] : t + lane;
+      in = row == at.row && pos == at.pos + lane;
+    }
+    const int len = __ffs(~__ballot_sync(0xffffffffu, in)) - 1;
+
+    float lo[ITERS][8], hi[ITERS][8];
+    bool have[ITERS];
+    float amax = 0.f;
+    bool bad = false;
+#pragma unroll
+    for (int it = 0; it < ITERS; ++it) {
+      const int i = it * G + grp;
+      have[it] = i < len;
+      const int tok = have[it] ? t + i : t;
+      int64_t rope = p.rope_pos[tok];
+      if (rope < 0 || rope >= p.max_seq_len) {  // reported by the q heads; the token is not stored
+        have[it] = false;
+        rope = 0;
+      }
+      const T* src = reinterpret_cast<const T*>(p.qkv) + (int64_t)tok * p.ld_qkv + (int64_t)(p.nq + head) * HD + li * 8;
+      ld8(src, lo[it]);
+      ld8(src + HALF, hi[it]);
+      if (is_k) norm_rotate<LANES>(lo[it], hi[it], p.k_weight, p.eps, p.cos + rope * HD, p.sin + rope * HD, li);
+      if (have[it]) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          amax = fmaxf(amax, fmaxf(fabsf(lo[it][e]), fabsf(hi[it][e])));
+          bad |= !(fabsf(lo[it][e]) <= 3.402823466e38f) || !(fabsf(hi[it][e]) <= 3.402823466e38f);
+        }
+      }
+    }
+    amax = warp_max(amax);
+    bad = __any_sync(0xffffffffu, bad);
+    float scale = amax / Q8<CODE>::kTop;
+    if (!(scale >= kQ8Tiny)) scale = 0.f;
+    if (bad) scale = __int_as_float(0x7fffffff);
+    const int64_t si = q8_scale(at.block, p.nkv, g);
+    uint8_t* tile = cache + q8_tile(at.block, p.nkv, g, HD);
+    if (off > 0) {
+      const float old = scales[si];
+      if (old >= scale || old != old) {
+        scale = old;
+      } else if (scale == scale) {  // the tile's maximum grew: round the history again
+        const float ratio = old / scale;
+#pragma unroll
+        for (int it = 0; it < ITERS; ++it) {
+          const int slot = it * G + grp;
+          if (slot < off) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              uint2* w = reinterpret_cast<uint2*>(tile + slot * HD + half * HALF + li * 8);
+              uint2 c = *w;
+              float v[4];
+              Q8<CODE>::decode4(c.x, v);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v[e] *= ratio;
+              c.x = Q8<CODE>::encode4(v);
+              Q8<CODE>::decode4(c.y, v);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v[e] *= ratio;
+              c.y = Q8<CODE>::encode4(v);
+              *w = c;
+            }
+          }
+        }
+      }
+      __syncwarp();  // every lane has read the old scale
+    }
+    const float inv = scale > 0.f ? 1.f / scale : 0.f;  // 0 for a tile of zeros and for NaN
+#pragma unroll
+    for (int it = 0; it < ITERS; ++it) {
+      if (!have[it]) continue;
+      const int slot = off + it * G + grp;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const float(&y)[8] = half ? hi[it] : lo[it];
+        float v[4];
+        uint2 c;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = y[e] * inv;
+        c.x = Q8<CODE>::encode4(v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = y[4 + e] * inv;
+        c.y = Q8<CODE>::encode4(v);
+        *reinterpret_cast<uint2*>(tile + slot * HD + half * HALF + li * 8) = c;
+      }
+    }
+    if (lane == 0) scales[si] = scale;
+    __syncwarp();  // a token given twice finds the tile as this run left it
+  }
+}
+
+// out[i, token, head, :] = code * scale of block ids[i], [n, 16, nkv, head_dim].
+template <typename T, int CODE>
+__global__ void __launch_bounds__(128) kv_read_q8_kernel(const uint8_t* k_cache, const uint8_t* v_cache,
+                                                         const float* k_scale, const float* v_scale, int num_blocks,
+                                                         int nkv, int hd, const int32_t* ids, int n, T* k_out,
+                                                         T* v_out, int32_t* status) {
+  pdl_wait();
+  pdl_trigger();
+  const int per = kQ8Block * nkv * hd / 8;  // 8-element pieces of one block
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= (int64_t)n * per) return;
+  const int b = (int)(i / per), w = (int)(i % per);
+  const int d = w % (hd / 8) * 8, slot = w / (hd / 8) % kQ8Block, g = w / (hd / 8) / kQ8Block;
+  const int64_t blk = ids[b];
+  const bool ok = blk >= 0 && blk < num_blocks;
+  if (!ok && w == 0) raise_status(status, B2_DEV_RANGE);
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv) {
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (ok) {
+      const uint2 c = *reinterpret_cast<const uint2*>((kv ? v_cache : k_cache) + q8_tile(blk, nkv, g, hd) + slot * hd + d);
+      const float s = (kv ? v_scale : k_scale)[q8_scale(blk, nkv, g)];
+      float a[4];
+      Q8<CODE>::decode4(c.x, a);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = a[e] * s;
+      Q8<CODE>::decode4(c.y, a);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[4 + e] = a[e] * s;
+    }
+    st8((kv ? v_out : k_out) + (((int64_t)b * kQ8Block + slot) * nkv + g) * hd + d, v);
+  }
+}
+
+int check_norm_rope(const char* name, const NormRopeParams& p, int hd, int layer, int dtype) {
+  B2_CHECK_ARG(p.n_tokens >= 0 && p.nq > 0 && p.nkv > 0, "%s: bad head counts", name);
+  B2_CHECK_ARG(valid_dtype(dtype), "%s: bad dtype", name);
+  if (hd != 32 && hd != 64 && hd != 128) return fail(B2_ENOTSUP, "%s: head_dim %d not supported (32, 64, 128)", name, hd);
+  B2_CHECK_ARG(p.ld_qkv >= ((int64_t)p.nq + 2 * (int64_t)p.nkv) * hd, "%s: ld_qkv too small", name);
+  B2_CHECK_ARG(p.num_blocks > 0 && p.bs > 0 && p.table_stride > 0 && p.table_rows > 0 && layer >= 0 &&
+                   p.max_seq_len > 0, "%s: bad cache geometry", name);
+  if (p.n_tokens == 0) return B2_OK;
+  B2_CHECK_ARG(p.qkv && p.rope_pos && p.tables && p.cos && p.sin && p.q_out && p.k_cache && p.v_cache,
+               "%s: null pointer", name);
+  B2_CHECK_ARG(p.table_index || p.n_tokens <= p.table_rows, "%s: %d tokens for %d table rows", name, p.n_tokens,
+               p.table_rows);
+  const size_t esz = dtype_bytes(dtype);
+  B2_CHECK_ARG(((uintptr_t)p.qkv % 16) == 0 && ((p.ld_qkv * esz) % 16) == 0 && ((uintptr_t)p.q_out % 16) == 0 &&
+                   ((uintptr_t)p.k_cache % 16) == 0 && ((uintptr_t)p.v_cache % 16) == 0 &&
+                   ((uintptr_t)p.cos % 16) == 0 && ((uintptr_t)p.sin % 16) == 0 &&
+                   ((uintptr_t)p.q_weight % 16) == 0 && ((uintptr_t)p.k_weight % 16) == 0,
+               "%s: buffers must be 16-byte aligned", name);
+  return B2_OK;
+}
+
+template <typename T, int HD, bool KV>
+int launch_rope(const NormRopeParams& p, cudaStream_t s) {
+  constexpr int GROUPS = 128 / (HD / 16);
+  const int64_t items = (int64_t)p.n_tokens * (KV ? p.nq + 2 * p.nkv : p.nq);
+  const int64_t grid = (items + GROUPS - 1) / GROUPS;
+  B2_CHECK_ARG(grid <= 0x7fffffff, "qk_norm_rope: %d tokens are too many for one call", p.n_tokens);
+  B2_TRY_CUDA(launch_pdl((qk_norm_rope_kernel<T, HD, KV>), dim3((unsigned)grid), dim3(128), 0, s, p));
+  return B2_OK;
+}
+
+template <typename T, int HD>
+int launch_q8(const NormRopeParams& p0, int cache_dtype, cudaStream_t s) {
+  NormRopeParams p = p0;
+  int rc = launch_rope<T, HD, false>(p, s);
+  if (rc) return rc;
+  p.chunk = p.n_tokens >= 2048 ? 16 : 1;
+  const dim3 grid((p.n_tokens + p.chunk - 1) / p.chunk, (2 * p.nkv + 3) / 4);
+  B2_CHECK_ARG(grid.y <= 65535, "qk_norm_rope: %d kv heads are too many", p.nkv);
+  if (cache_dtype == B2_I8)
+    B2_TRY_CUDA(launch_pdl((kv_write_q8_kernel<T, HD, B2_I8>), grid, dim3(128), 0, s, p));
+  else
+    B2_TRY_CUDA(launch_pdl((kv_write_q8_kernel<T, HD, B2_E4M3>), grid, dim3(128), 0, s, p));
+  return B2_OK;
+}
+
+}  // namespace
+}  // namespace b2
+
+extern "C" {
+
+int b2_qk_norm_rope_kv_write(const void* qkv, int64_t ld_qkv, int n_tokens, int nq, int nkv, int head_dim,
+                             const float* q_weight, const float* k_weight, float eps, const int64_t* rope_pos,
+                             const int64_t* store_pos, const int32_t* table_index, const int32_t* block_tables,
+                             int table_rows, int table_stride, int num_blocks, int block_size, const float* cos,
+                             const float* sin, int max_seq_len, void* q_out, void* k_cache, void* v_cache, int layer,
+                             int dtype, int32_t* status, b2_stream_t stream) {
+  using namespace b2;
+  NormRopeParams p{qkv, ld_qkv, n_tokens, nq, nkv, q_weight, k_weight, eps, rope_pos, store_pos, table_index,
+                   block_tables, table_rows, table_stride, num_blocks, block_size, cos, sin, max_seq_len, q_out,
+                   k_cache, v_cache, nullptr, nullptr, 0, status};
+  const int rc = check_norm_rope("b2_qk_norm_rope_kv_write", p, head_dim, layer, dtype);
+  if (rc || n_tokens == 0) return rc;
+  const size_t off = (size_t)layer * num_blocks * block_size * nkv * head_dim * dtype_bytes(dtype);
+  p.k_cache = static_cast<char*>(k_cache) + off;
+  p.v_cache = static_cast<char*>(v_cache) + off;
+#define B2_ROPE_CASE(T, HD) return launch_rope<T, HD, true>(p, stream)
+  if (dtype == B2_BF16) {
+    if (head_dim == 32) B2_ROPE_CASE(__nv_bfloat16, 32);
+    if (head_dim == 64) B2_ROPE_CASE(__nv_bfloat16, 64);
+    B2_ROPE_CASE(__nv_bfloat16, 128);
+  }
+  if (head_dim == 32) B2_ROPE_CASE(float, 32);
+  if (head_dim == 64) B2_ROPE_CASE(float, 64);
+  B2_ROPE_CASE(float, 128);
+#undef B2_ROPE_CASE
+}
+
+int b2_qk_norm_rope_kv_write_q8(const void* qkv, int64_t ld_qkv, int n_tokens, int nq, int nkv, int head_dim,
+                                const float* q_weight, const float* k_weight, float eps, const int64_t* rope_pos,
+                                const int64_t* store_pos, const int32_t* table_index, const int32_t* block_tables,
+                                int table_rows, int table_stride, int num_blocks, int block_size, const float* cos,
+                                const float* sin, int max_seq_len, void* q_out, void* k_cache, void* v_cache,
+                                float* k_scale, float* v_scale, int cache_dtype, int layer, int dtype,
+                                int32_t* status, b2_stream_t stream) {
+  using namespace b2;
+  NormRopeParams p{qkv, ld_qkv, n_tokens, nq, nkv, q_weight, k_weight, eps, rope_pos, store_pos, table_index,
+                   block_tables, table_rows, table_stride, num_blocks, block_size, cos, sin, max_seq_len, q_out,
+                   k_cache, v_cache, k_scale, v_scale, 0, status};
+  B2_CHECK_ARG(valid_q8_dtype(cache_dtype), "b2_qk_norm_rope_kv_write_q8: bad cache dtype");
+  if (block_size != kQ8Block)
+    return fail(B2_ENOTSUP, "b2_qk_norm_rope_kv_write_q8: block_size %d (16 only)", block_size);
+  const int rc = check_norm_rope("b2_qk_norm_rope_kv_write_q8", p, head_dim, layer, dtype);
+  if (rc || n_tokens == 0) return rc;
+  B2_CHECK_ARG(k_scale && v_scale, "b2_qk_norm_rope_kv_write_q8: null scales");
+  const size_t tiles = (size_t)layer * num_blocks * nkv;
+  p.k_cache = static_cast<char*>(k_cache) + tiles * kQ8Block * head_dim;
+  p.v_cache = static_cast<char*>(v_cache) + tiles * kQ8Block * head_dim;
+  p.k_scale = k_scale + tiles;
+  p.v_scale = v_scale + tiles;
+#define B2_Q8_CASE(T, HD) return launch_q8<T, HD>(p, cache_dtype, stream)
+  if (dtype == B2_BF16) {
+    if (head_dim == 32) B2_Q8_CASE(__nv_bfloat16, 32);
+    if (head_dim == 64) B2_Q8_CASE(__nv_bfloat16, 64);
+    B2_Q8_CASE(__nv_bfloat16, 128);
+  }
+  if (head_dim == 32) B2_Q8_CASE(float, 32);
+  if (head_dim == 64) B2_Q8_CASE(float, 64);
+  B2_Q8_CASE(float, 128);
+#undef B2_Q8_CASE
+}
+
+int b2_kv_read_q8(const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
+                  int cache_dtype, int layer, int num_blocks, int block_size, int nkv, int head_dim,
+                  const int32_t* block_ids, int n_blocks, void* k_out, void* v_out, int out_dtype, int32_t* status,
+                  b2_stream_t stream) {
+  using namespace b2;
+  B2_CHECK_ARG(valid_q8_dtype(cache_dtype), "b2_kv_read_q8: bad cache dtype");
+  B2_CHECK_ARG(valid_dtype(out_dtype), "b2_kv_read_q8: bad dtype");
+  B2_CHECK_ARG(num_blocks > 0 && nkv > 0 && head_dim > 0 && layer >= 0 && n_blocks >= 0,
+               "b2_kv_read_q8: bad cache geometry");
+  if (block_size != kQ8Block) return fail(B2_ENOTSUP, "b2_kv_read_q8: block_size %d (16 only)", block_size);
+  if (head_dim != 32 && head_dim != 64 && head_dim != 128)
+    return fail(B2_ENOTSUP, "b2_kv_read_q8: head_dim %d not supported (32, 64, 128)", head_dim);
+  if (n_blocks == 0) return B2_OK;
+  B2_CHECK_ARG(k_cache && v_cache && k_scale && v_scale && block_ids && k_out && v_out, "b2_kv_read_q8: null pointer");
+  B2_CHECK_ARG(((uintptr_t)k_cache % 16) == 0 && ((uintptr_t)v_cache % 16) == 0 && ((uintptr_t)k_out % 16) == 0 &&
+                   ((uintptr_t)v_out % 16) == 0, "b2_kv_read_q8: buffers must be 16-byte aligned");
+  const size_t tiles = (size_t)layer * num_blocks * nkv;
+  const uint8_t* kc = static_cast<const uint8_t*>(k_cache) + tiles * kQ8Block * head_dim;
+  const uint8_t* vc = static_cast<const uint8_t*>(v_cache) + tiles * kQ8Block * head_dim;
+  const int64_t pieces = (int64_t)n_blocks * kQ8Block * nkv * head_dim / 8;
+  const int64_t grid = (pieces + 127) / 128;
+  B2_CHECK_ARG(grid <= 0x7fffffff && (int64_t)kQ8Block * nkv * head_dim <= 0x7fffffff,
+               "b2_kv_read_q8: %d blocks are too many for one call", n_blocks);
+  auto go = [&](auto kernel, auto* ko, auto* vo) -> int {
+    B2_TRY_CUDA(launch_pdl(kernel, dim3((unsigned)grid), dim3(128), 0, stream, kc, vc, k_scale + tiles,
+                           v_scale + tiles, num_blocks, nkv, head_dim, block_ids, n_blocks, ko, vo, status));
+    return B2_OK;
+  };
+  if (out_dtype == B2_BF16) {
+    auto* ko = static_cast<__nv_bfloat16*>(k_out);
+    auto* vo = static_cast<__nv_bfloat16*>(v_out);
+    return cache_dtype == B2_I8 ? go(kv_read_q8_kernel<__nv_bfloat16, B2_I8>, ko, vo)
+                                : go(kv_read_q8_kernel<__nv_bfloat16, B2_E4M3>, ko, vo);
+  }
+  auto* ko = static_cast<float*>(k_out);
+  auto* vo = static_cast<float*>(v_out);
+  return cache_dtype == B2_I8 ? go(kv_read_q8_kernel<float, B2_I8>, ko, vo)
+                              : go(kv_read_q8_kernel<float, B2_E4M3>, ko, vo);
+}
+
+}  // extern "C"

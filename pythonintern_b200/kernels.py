@@ -9,7 +9,7 @@ Device-side range errors are collected in a per-device status word; call
 from __future__ import annotations
 
 import math
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -339,4 +339,261 @@ def argmax(logits: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Te
         out = torch.empty(logits.shape[0], dtype=torch.int64, device=logits.device)
     check(_lib.lib().b2_argmax(ptr(logits), logits.stride(0), logits.shape[0], logits.shape[1], ptr(out),
                                stream_ptr(logits.device)), "b2_argmax")
+    return out
+
+
+# ------------------------------------------------------------------ block tables and slot maps
+class SlotMap(NamedTuple):
+    """The maps ``block_tables_extend`` builds for a step's new tokens, on the device."""
+    seq_start: torch.Tensor    # int32 [n_seqs + 1]: rows [seq_start[s], seq_start[s+1]) are sequence s
+    positions: torch.Tensor    # int64 [max_tokens]: position of the token in its sequence
+    table_index: torch.Tensor  # int32 [max_tokens]: its sequence (block-table row)
+    slots: torch.Tensor        # int64 [max_tokens]: block * block_size + offset
+    ctx_lens: torch.Tensor     # int32 [max_tokens]: positions + 1
+    last_rows: torch.Tensor    # int64 [n_seqs]: the sequence's last new token, -1 where it has none
+
+
+def _check(t: torch.Tensor, name: str, dtype: torch.dtype, numel: int, device: torch.device):
+    """A contiguous CUDA tensor of at least ``numel`` elements of ``dtype`` on ``device``."""
+    if t.dtype != dtype or t.device != device or not t.is_contiguous() or t.numel() < numel:
+        raise _lib.B2Error(f"{name} must be a contiguous {dtype} tensor of at least {numel} elements on {device}; "
+                           f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _call(name: str, device: torch.device, *args):
+    """One launching entry point on ``device`` (made current for the call if it is not) and its stream."""
+    fn = getattr(_lib.lib(), name)
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, status_ptr(device), stream_ptr(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, status_ptr(device), stream_ptr(device))
+    check(rc, name)
+
+
+def _check_tables(tables: torch.Tensor):
+    require_cuda(tables, "tables")
+    if tables.dim() != 2 or tables.dtype != torch.int32 or not tables.is_contiguous():
+        raise _lib.B2Error("tables must be a contiguous int32 matrix [sequences, blocks]")
+
+
+def _ring_args(device, free_ring, free_state):
+    _check(free_ring, "free_ring", torch.int32, 1, device)
+    _check(free_state, "free_state", torch.int32, 4, device)
+    return free_ring.numel()
+
+
+def block_tables_extend(tables: torch.Tensor, lens: torch.Tensor, new_lens: torch.Tensor, max_tokens: int,
+                        block_size: int, free_ring: Optional[torch.Tensor] = None,
+                        free_state: Optional[torch.Tensor] = None, num_blocks: Optional[int] = None,
+                        out: Optional[SlotMap] = None) -> SlotMap:
+    """Block tables and slot maps of a step's new tokens, built on the GPU from request lengths.
+
+    ``tables`` int32 [n_seqs, width], ``lens`` int32 [n_seqs] (tokens held), ``new_lens`` int32
+    [n_seqs].  With a free ring (int32 [num_blocks] ids, state int32 [4] = head, count, 0, 0) every
+    sequence takes the blocks its new tokens need, FIFO like the host's free list
+    (engine/model/kv_cache.py:172-227), and ``lens`` grows; without one (give ``num_blocks``) the
+    tables are taken as they are and only the maps are built.  Map entries behind the step's last
+    token are left as they were.  Too few free blocks (``MemoryError``) or a length out of range
+    (``IndexError``) are reported by ``_lib.check_device_status`` and change nothing.
+    """
+    _check_tables(tables)
+    dev = tables.device
+    n, width = tables.shape
+    _check(lens, "lens", torch.int32, n, dev)
+    _check(new_lens, "new_lens", torch.int32, n, dev)
+    if (free_ring is None) != (free_state is None):
+        raise _lib.B2Error("free_ring and free_state come together")
+    if free_ring is not None:
+        num_blocks = _ring_args(dev, free_ring, free_state)
+    elif num_blocks is None:
+        raise _lib.B2Error("num_blocks is needed without a free ring")
+    if out is None:
+        i64 = torch.empty(2 * max_tokens + n, dtype=torch.int64, device=dev)
+        i32 = torch.empty(2 * max_tokens + n + 1, dtype=torch.int32, device=dev)
+        positions, slots, last_rows = i64.split((max_tokens, max_tokens, n))
+        table_index, ctx_lens, seq_start = i32.split((max_tokens, max_tokens, n + 1))
+        out = SlotMap(seq_start, positions, table_index, slots, ctx_lens, last_rows)
+    else:
+        _check(out.seq_start, "seq_start", torch.int32, n + 1, dev)
+        _check(out.positions, "positions", torch.int64, max_tokens, dev)
+        _check(out.table_index, "table_index", torch.int32, max_tokens, dev)
+        _check(out.slots, "slots", torch.int64, max_tokens, dev)
+        _check(out.ctx_lens, "ctx_lens", torch.int32, max_tokens, dev)
+        _check(out.last_rows, "last_rows", torch.int64, n, dev)
+    _call("b2_block_tables_extend", dev, ptr(tables), n, width, ptr(lens), ptr(new_lens), block_size, ptr(free_ring),
+          num_blocks, ptr(free_state), max_tokens, ptr(out.seq_start), ptr(out.positions), ptr(out.table_index),
+          ptr(out.slots), ptr(out.ctx_lens), ptr(out.last_rows))
+    return out
+
+
+def block_tables_truncate(tables: torch.Tensor, lens: torch.Tensor, keep_lens: torch.Tensor, block_size: int,
+                          free_ring: torch.Tensor, free_state: torch.Tensor):
+    """Cuts every sequence back to ``keep_lens`` tokens (0 frees it): the blocks behind them go to
+    the tail of the free ring in sequence order (kv_cache.py:215-227), their table entries to -1."""
+    _check_tables(tables)
+    dev = tables.device
+    n, width = tables.shape
+    _check(lens, "lens", torch.int32, n, dev)
+    _check(keep_lens, "keep_lens", torch.int32, n, dev)
+    num_blocks = _ring_args(dev, free_ring, free_state)
+    _call("b2_block_tables_truncate", dev, ptr(tables), n, width, ptr(lens), ptr(keep_lens), block_size,
+          ptr(free_ring), num_blocks, ptr(free_state))
+
+
+# ------------------------------------------------------------------ q/k norms + RoPE + paged KV write
+def _norm_rope_args(qkv, nq, nkv, hd, q_weight, k_weight, eps, rope_pos, store_pos, table_index, block_tables, cos,
+                    sin, q_out):
+    """Checks the arguments both cache types share; returns the leading C arguments (up to block_tables' stride)."""
+    require_cuda(qkv, "qkv")
+    dev = qkv.device
+    if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] < (nq + 2 * nkv) * hd:
+        raise _lib.B2Error(f"qkv must be [tokens, >= {(nq + 2 * nkv) * hd}] with contiguous rows")
+    n = qkv.shape[0]
+    for t, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        if t is not None:
+            _check(t, name, torch.float32, hd, dev)
+    _check(rope_pos, "rope_pos", torch.int64, n, dev)
+    if store_pos is not None:
+        _check(store_pos, "store_pos", torch.int64, n, dev)
+    if table_index is not None:
+        _check(table_index, "table_index", torch.int32, n, dev)
+    _check_tables(block_tables)
+    _check(cos, "cos", torch.float32, hd, dev)
+    _check(sin, "sin", torch.float32, cos.numel(), dev)
+    _check(q_out, "q_out", qkv.dtype, n * nq * hd, dev)
+    return (ptr(qkv), qkv.stride(0) if n > 1 else max(qkv.stride(0), qkv.shape[1]), n, nq, nkv, hd, ptr(q_weight),
+            ptr(k_weight), float(eps), ptr(rope_pos), ptr(store_pos), ptr(table_index), ptr(block_tables),
+            block_tables.shape[0], block_tables.shape[1])
+
+
+def qk_norm_rope_kv_write(qkv: torch.Tensor, nq: int, nkv: int, head_dim: int, q_weight: Optional[torch.Tensor],
+                          k_weight: Optional[torch.Tensor], eps: float, rope_pos: torch.Tensor,
+                          store_pos: Optional[torch.Tensor], table_index: Optional[torch.Tensor],
+                          block_tables: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, q_out: torch.Tensor,
+                          k_cache: torch.Tensor, v_cache: torch.Tensor, layer: int):
+    """``rope_kv_write`` with an RMS norm of every q and k head (weights float32 [head_dim], None: no
+    norm) before the rotation, in the same pass (engine/model/attention.py:46-63, :166-184)."""
+    args = _norm_rope_args(qkv, nq, nkv, head_dim, q_weight, k_weight, eps, rope_pos, store_pos, table_index,
+                           block_tables, cos, sin, q_out)
+    _check_cache(k_cache, v_cache, layer, (nkv, head_dim), qkv.dtype, qkv.device, 2)
+    _, NB, bs, _, _ = k_cache.shape
+    _call("b2_qk_norm_rope_kv_write", qkv.device, *args, NB, bs, ptr(cos), ptr(sin), cos.shape[0], ptr(q_out),
+          ptr(k_cache), ptr(v_cache), layer, dtype_code(qkv.dtype))
+
+
+def _check_cache(k_cache, v_cache, layer, tail, dtype, device, at):
+    """Both caches: contiguous, 5 dimensions, of ``dtype``, with ``tail`` as their dimensions from ``at + 1``."""
+    for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        if (t.dim() != 5 or t.dtype != dtype or t.device != device or not t.is_contiguous()
+                or t.shape != k_cache.shape or tuple(t.shape[at + 1:at + 1 + len(tail)]) != tail):
+            raise _lib.B2Error(f"{name} must be a contiguous {dtype} cache of {tail} on {device}; got {t.dtype} "
+                               f"{tuple(t.shape)} on {t.device}")
+    if not 0 <= layer < k_cache.shape[0]:
+        raise IndexError(f"layer {layer} of a cache with {k_cache.shape[0]}")
+
+
+def _q8_cache(k_cache, v_cache, k_scale, v_scale, layer, nkv, hd, device):
+    """Checks an 8-bit cache [L, blocks, nkv, 16, hd] and its scales [L, blocks, nkv]; returns (type code, blocks, 16)."""
+    code = _lib.cache_dtype_code(k_cache.dtype)
+    _check_cache(k_cache, v_cache, layer, (nkv,), k_cache.dtype, device, 1)
+    if k_cache.shape[4] != hd:
+        raise _lib.B2Error(f"the cache holds heads of {k_cache.shape[4]}, not {hd}")
+    for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+        _check(t, name, torch.float32, 1, device)
+        if t.shape != k_cache.shape[:3]:
+            raise _lib.B2Error(f"{name} must be {tuple(k_cache.shape[:3])}, got {tuple(t.shape)}")
+    return code, k_cache.shape[1], k_cache.shape[3]
+
+
+def qk_norm_rope_kv_write_q8(qkv: torch.Tensor, nq: int, nkv: int, head_dim: int, q_weight: Optional[torch.Tensor],
+                             k_weight: Optional[torch.Tensor], eps: float, rope_pos: torch.Tensor,
+                             store_pos: Optional[torch.Tensor], table_index: Optional[torch.Tensor],
+                             block_tables: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, q_out: torch.Tensor,
+                             k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                             v_scale: torch.Tensor, layer: int):
+    """``qk_norm_rope_kv_write`` into the 8-bit cache: codes int8 or float8_e4m3fn [L, blocks, nkv, 16,
+    head_dim] with a float32 scale per (layer, block, kv head).  The tokens of a sequence must be
+    consecutive and ascending; see include/b2tp.h for the rounding of blocks that are filled in steps."""
+    args = _norm_rope_args(qkv, nq, nkv, head_dim, q_weight, k_weight, eps, rope_pos, store_pos, table_index,
+                           block_tables, cos, sin, q_out)
+    code, NB, bs = _q8_cache(k_cache, v_cache, k_scale, v_scale, layer, nkv, head_dim, qkv.device)
+    _call("b2_qk_norm_rope_kv_write_q8", qkv.device, *args, NB, bs, ptr(cos), ptr(sin), cos.shape[0], ptr(q_out),
+          ptr(k_cache), ptr(v_cache), ptr(k_scale), ptr(v_scale), code, layer, dtype_code(qkv.dtype))
+
+
+def kv_read_q8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, layer: int,
+               block_ids: torch.Tensor, dtype: torch.dtype):
+    """The values (code * scale) of blocks ``block_ids`` (int32) of one layer of the 8-bit cache:
+    (k, v), each [n, 16, nkv, head_dim] of ``dtype`` (engine/model/kv_cache.py:121-147)."""
+    require_cuda(k_cache, "k_cache")
+    dev = k_cache.device
+    nkv, hd = k_cache.shape[2], k_cache.shape[4]
+    code, NB, bs = _q8_cache(k_cache, v_cache, k_scale, v_scale, layer, nkv, hd, dev)
+    _check(block_ids, "block_ids", torch.int32, 0, dev)
+    n = block_ids.numel()
+    k, v = torch.empty(2, n, bs, nkv, hd, dtype=dtype, device=dev).unbind(0)
+    _call("b2_kv_read_q8", dev, ptr(k_cache), ptr(v_cache), ptr(k_scale), ptr(v_scale), code, layer, NB, bs, nkv, hd,
+          ptr(block_ids), n, ptr(k), ptr(v), dtype_code(dtype))
+    return k, v
+
+
+# ------------------------------------------------------------------ attention over the 8-bit cache
+def _q8_attention_io(q, nq, hd, out):
+    require_cuda(q, "q")
+    if q.dim() != 2 or q.stride(1) != 1 or q.shape[1] < nq * hd:
+        raise _lib.B2Error(f"q must be [rows, >= {nq * hd}] with contiguous rows")
+    if out is None:
+        return torch.empty(q.shape[0], nq * hd, dtype=q.dtype, device=q.device)
+    if (out.dim() != 2 or out.dtype != q.dtype or out.device != q.device or out.shape[0] < q.shape[0]
+            or out.shape[1] < nq * hd or out.stride(1) != 1):
+        raise _lib.B2Error(f"out must be a {q.dtype} matrix of at least {(q.shape[0], nq * hd)} on {q.device}")
+    return out
+
+
+def _rows_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def paged_attention_q8(q: torch.Tensor, nq: int, nkv: int, head_dim: int, k_cache: torch.Tensor,
+                       v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, layer: int,
+                       block_tables: torch.Tensor, table_index: Optional[torch.Tensor], ctx_lens: torch.Tensor,
+                       compat_pad: bool, scale: float, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``paged_attention`` over the 8-bit cache, one query token per row; q bf16 or float32."""
+    out = _q8_attention_io(q, nq, head_dim, out)
+    n, dev = q.shape[0], q.device
+    code, NB, bs = _q8_cache(k_cache, v_cache, k_scale, v_scale, layer, nkv, head_dim, dev)
+    _check_tables(block_tables)
+    _check(ctx_lens, "ctx_lens", torch.int32, n, dev)
+    if table_index is not None:
+        _check(table_index, "table_index", torch.int32, n, dev)
+    nbytes = _lib.lib().b2_paged_attention_q8_workspace_bytes(n, nq, nkv, head_dim)
+    # scratch of this call alone: another stream or graph may run at the same time
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _call("b2_paged_attention_q8", dev, ptr(q), _rows_stride(q), n, nq, nkv, head_dim, ptr(k_cache), ptr(v_cache),
+          ptr(k_scale), ptr(v_scale), code, layer, NB, bs, ptr(block_tables), block_tables.shape[0],
+          block_tables.shape[1], ptr(table_index), ptr(ctx_lens), 1 if compat_pad else 0, float(scale), ptr(out),
+          _rows_stride(out), dtype_code(q.dtype), ptr(ws), nbytes)
+    return out
+
+
+def prefill_attention_q8(q: torch.Tensor, nq: int, nkv: int, head_dim: int, k_cache: torch.Tensor,
+                         v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, layer: int,
+                         block_tables: torch.Tensor, seq_start: torch.Tensor, n_seqs: int, scale: float,
+                         seq_ctx0: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``prefill_attention`` over the 8-bit cache: many tokens per sequence (a prompt, a chunk behind
+    cached tokens, drafted tokens), causal; q bf16 or float32."""
+    out = _q8_attention_io(q, nq, head_dim, out)
+    n, dev = q.shape[0], q.device
+    code, NB, bs = _q8_cache(k_cache, v_cache, k_scale, v_scale, layer, nkv, head_dim, dev)
+    _check_tables(block_tables)
+    _check(seq_start, "seq_start", torch.int32, n_seqs + 1, dev)
+    if seq_ctx0 is not None:
+        _check(seq_ctx0, "seq_ctx0", torch.int32, n_seqs, dev)
+    nbytes = _lib.lib().b2_prefill_attention_q8_workspace_bytes(n, nq, nkv, head_dim, n_seqs)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _call("b2_prefill_attention_q8", dev, ptr(q), _rows_stride(q), n, nq, nkv, head_dim, ptr(k_cache), ptr(v_cache),
+          ptr(k_scale), ptr(v_scale), code, layer, NB, bs, ptr(block_tables), block_tables.shape[0],
+          block_tables.shape[1], ptr(seq_start), ptr(seq_ctx0), n_seqs, float(scale), ptr(out), _rows_stride(out),
+          dtype_code(q.dtype), ptr(ws), nbytes)
     return out
