@@ -311,14 +311,14 @@ int b2_kv_read_q8(const void* k_cache, const void* v_cache, const float* k_scale
  * *_workspace_bytes() bytes, in any state; calls that may overlap on the GPU need one each.
  * A row that sees no key gives zeros; rows behind the last sequence of a prefill are left as
  * they were.  Keys behind a row's context are never used, whatever their codes and scales. */
-size_t b2_paged_attention_q8_workspace_bytes(int n_rows, int nq, int nkv, int head_dim);
+size_t b2_paged_attention_q8_workspace_bytes(int n_rows, int nq, int nkv, int head_dim, int dtype);
 int b2_paged_attention_q8(const void* q, int64_t ld_q, int n_rows, int nq, int nkv, int head_dim, const void* k_cache,
                           const void* v_cache, const float* k_scale, const float* v_scale, int cache_dtype, int layer,
                           int num_blocks, int block_size, const int32_t* block_tables, int table_rows,
                           int table_stride, const int32_t* table_index, const int32_t* ctx_lens, int compat_pad,
                           float scale, void* out, int64_t ld_out, int dtype, void* workspace, size_t workspace_bytes,
                           int32_t* status, b2_stream_t stream);
-size_t b2_prefill_attention_q8_workspace_bytes(int n_rows, int nq, int nkv, int head_dim, int n_seqs);
+size_t b2_prefill_attention_q8_workspace_bytes(int n_rows, int nq, int nkv, int head_dim, int n_seqs, int dtype);
 int b2_prefill_attention_q8(const void* q, int64_t ld_q, int n_rows, int nq, int nkv, int head_dim,
                             const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
                             int cache_dtype, int layer, int num_blocks, int block_size, const int32_t* block_tables,

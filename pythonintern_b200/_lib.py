@@ -109,12 +109,12 @@ _SIGS = {
     "b2_kv_read_q8": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int,
                                _c_int, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p,
                                _c_void_p]),
-    "b2_paged_attention_q8_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int]),
+    "b2_paged_attention_q8_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int, _c_int]),
     "b2_paged_attention_q8": (_c_int, [_c_void_p, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_void_p,
                                        _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_int,
                                        _c_int, _c_void_p, _c_void_p, _c_int, _c_float, _c_void_p, _c_i64,
                                        _c_int, _c_void_p, _c_size, _c_void_p, _c_void_p]),
-    "b2_prefill_attention_q8_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int, _c_int]),
+    "b2_prefill_attention_q8_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int]),
     "b2_prefill_attention_q8": (_c_int, [_c_void_p, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_void_p,
                                          _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int,
                                          _c_void_p, _c_int, _c_int, _c_void_p, _c_void_p, _c_int, _c_float,

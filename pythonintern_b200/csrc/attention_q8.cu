@@ -3,6 +3,33 @@
 // For a query at position p of a sequence, with the tile scales ks, vs of each block:
 //   s_t = scale * ks[block(t)] * (q . kc_t),   out = sum_t softmax(s)_t * vs[block(t)] * vc_t,
 // over the keys t the query may see; a query that sees none gives zeros.
+//
+// Work.  A tile is up to 8 * NT (query token, q head) columns that share a kv head: the heads
+// of one decode row, or those of consecutive tokens of one sequence.  It reads ceil(keys / 16)
+// blocks; the blocks of all tiles and heads in a row form one line of steps, cut into equal
+// chunks, one per resident warp, so ragged contexts cost no more than even ones.  A warp works
+// alone (no barrier in the loop).  A tile that lies in one chunk is finished there; the pieces of
+// others go to the workspace as softmax states and are joined by a second kernel.  Every CTA
+// finds the cut by itself from the lengths, so nothing waits on the host.
+//
+// One step.  S^T[16 keys x 8 NT] = K Q^T and O^T[head_dim x 8 NT] += V^T P^T on
+// mma.sync.m16n8k16 with float16 operands and float32 sums.  A code of 8 bits is exact in
+// float16, so nothing is rounded on the way in: codes go from global memory straight into the
+// registers of the A fragments.
+//  * K: lane (r, t) = (lane / 4, lane % 4) reads head_dim / 4 contiguous codes of keys r and
+//    r + 8.  The order of the head_dim axis inside the product is free, so its codes are taken
+//    as the k indexes of that lane and q is laid out to match.
+//  * V: the lane reads head_dim / 8 codes of the keys 2t, 2t+1, 2t+8, 2t+9; a byte shuffle pairs
+//    two keys' codes of one dimension, which is the transposed operand without shared memory.
+//  * P^T leaves the S^T fragments for the B fragments by an 8x8 transpose in registers.
+//  * q is scaled by a power of two per column, so that its largest magnitude is near 2^14, and
+//    split: one float16 term holds bf16 (values 2^-38 below the largest are cut), two hold
+//    float32 up to 2^-22 of an element.
+// Softmax statistics are float32.  P = 2^(s - m) vs 2^(m - m2) is rounded to float16 (to two
+// terms for float32 queries): the reference m2 follows the largest s + log2(vs), so a scale that
+// differs by orders of magnitude between blocks costs no precision.  The references move only
+// when a value would pass 2^15 and then to 2^8 above the value, so the common step needs no
+// maximum across lanes, only one vote.
 #include "q8.cuh"
 
 namespace b2 {
@@ -32,91 +59,710 @@ struct Q8AttnParams {
   void* out;
   int64_t ld_out;
   int32_t* status;
+  // workspace
+  int* ws_tiles;    // [4]: tiles of the call
+  int4* ws_pairs;   // [tiles * nkv]: first and last warp, sequence, first token
+  float4* ws_stat;  // [slots][columns]: m, l, m2
+  float* ws_o;      // [slots][columns][head_dim]
 };
 
-constexpr int kRowThreads = 128;
 
-// The simplest form: one CTA per (query row, q head), 128 keys at a time.
-template <typename T, int HD, int CODE>
-__global__ void __launch_bounds__(kRowThreads) q8_attn_row_kernel(Q8AttnParams p) {
+// ------------------------------------------------------------------ the cut of the work
+constexpr int kWarps = 4;
+constexpr int kGroups = 1024;  // prefix sums kept in shared memory
+constexpr int kMinChunk = 4;   // steps a warp takes at least
+
+struct Unit {  // a decode row, or a sequence of a prefill
+  int start, len, ctx0;  // first row of q, tokens, keys before the first token
+  bool bad;
+};
+
+__device__ __forceinline__ int table_row(const Q8AttnParams& p, int u) {
+  return !p.seq_start && p.table_index ? p.table_index[u] : u;
+}
+
+__device__ __forceinline__ Unit unit_of(const Q8AttnParams& p, int u) {
+  Unit r{u, 0, 0, false};
+  const int64_t most = (int64_t)p.table_stride * kQ8Block;
+  if (!p.seq_start) {
+    const int row = table_row(p, u), ctx = p.ctx_lens[u];
+    const bool there = row >= 0 && row < p.table_rows;
+    r.bad = !there || ctx > most;
+    const int keys = there ? (int)min((int64_t)ctx, most) : 0;  // a context past its table row: the row's keys
+    r.len = keys > 0 ? 1 : 0;
+    r.ctx0 = keys - 1;
+  } else {
+    const int a = p.seq_start[u], b = p.seq_start[u + 1];
+    const int ctx0 = p.seq_ctx0 ? p.seq_ctx0[u] : 0;
+    r.bad = a < 0 || b > p.n_rows || b < a || ctx0 < 0 || (b > a && (int64_t)ctx0 + b - a > most);
+    if (!r.bad) {
+      r.start = a;
+      r.len = b - a;
+      r.ctx0 = ctx0;
+    }
+  }
+  return r;
+}
+
+__device__ __forceinline__ int blocks_of(int64_t keys) { return (int)((keys + kQ8Block - 1) / kQ8Block); }
+
+// Blocks of the first x tiles of a unit: sum over j = 1..x of ceil((ctx0 + min(j qt, len)) / 16).
+// Over the full tiles the remainders repeat with period 16 / gcd(qt, 16), and every further
+// period adds the same number to each of its terms.
+__device__ __forceinline__ int64_t blocks_before(const Unit& u, int qt, int x) {
+  const int full = min(x, u.len / qt);
+  int per = kQ8Block;
+  while (per > 1 && (qt * (per / 2)) % kQ8Block == 0) per /= 2;
+  const int64_t rounds = full / per, add = (int64_t)qt * per / kQ8Block;
+  int64_t one = 0;
+  for (int j = 1; j <= min(per, full); ++j) one += blocks_of((int64_t)u.ctx0 + j * qt);
+  int64_t sum = rounds * one + per * add * (rounds * (rounds - 1) / 2);
+  if (rounds == 0) sum = one;
+  else
+    for (int j = (int)rounds * per + 1; j <= full; ++j) sum += blocks_of((int64_t)u.ctx0 + (int64_t)j * qt);
+  if (x > full) sum += blocks_of((int64_t)u.ctx0 + u.len);
+  return sum;
+}
+
+__device__ __forceinline__ int tiles_of(const Unit& u, int qt) { return (u.len + qt - 1) / qt; }
+
+struct Cut {
+  int64_t total;  // steps of the call, all kv heads
+  int64_t chunk;  // steps per warp
+  int tiles;
+  int max_ctx;    // longest context (compat_pad)
+};
+
+// Prefix sums over groups of units: sm_steps[i] blocks (of one kv head) and sm_tiles[i] tiles
+// before group i.  Called by the whole CTA.
+__device__ Cut make_cut(const Q8AttnParams& p, int qt, int n_units, int per_group, int64_t* sm_steps, int* sm_tiles,
+                        int warps, bool report) {
+  __shared__ int64_t w_steps[kWarps];
+  __shared__ int w_tiles[kWarps], w_ctx[kWarps];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = kWarps * 32;
+  const int groups = (n_units + per_group - 1) / per_group;
+  const int per_thread = (groups + threads - 1) / threads;
+  int64_t steps = 0;
+  int tiles = 0, max_ctx = 0;
+  bool bad = false;
+  const int g0 = min(groups, tid * per_thread), g1 = min(groups, g0 + per_thread);
+  for (int g = g0; g < g1; ++g) {
+    sm_steps[g] = steps;
+    sm_tiles[g] = tiles;
+    for (int u = g * per_group; u < min(n_units, (g + 1) * per_group); ++u) {
+      const Unit x = unit_of(p, u);
+      bad |= x.bad;
+      const int n = tiles_of(x, qt);
+      steps += blocks_before(x, qt, n);
+      tiles += n;
+      if (p.compat_pad) max_ctx = max(max_ctx, p.ctx_lens[u]);
+    }
+  }
+  if (report && bad) raise_status(p.status, B2_DEV_RANGE);
+  int64_t inc_s = steps;
+  int inc_t = tiles;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t a = __shfl_up_sync(0xffffffffu, inc_s, o);
+    const int b = __shfl_up_sync(0xffffffffu, inc_t, o);
+    max_ctx = max(max_ctx, __shfl_xor_sync(0xffffffffu, max_ctx, o));
+    if (lane >= o) {
+      inc_s += a;
+      inc_t += b;
+    }
+  }
+  if (lane == 31) {
+    w_steps[warp] = inc_s;
+    w_tiles[warp] = inc_t;
+    w_ctx[warp] = max_ctx;
+  }
+  __syncthreads();
+  Cut c{0, 0, 0, 0};
+  int64_t base_s = inc_s - steps;
+  int base_t = inc_t - tiles;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) {
+      base_s += w_steps[w];
+      base_t += w_tiles[w];
+    }
+    c.total += w_steps[w];
+    c.tiles += w_tiles[w];
+    c.max_ctx = max(c.max_ctx, w_ctx[w]);
+  }
+  for (int g = g0; g < g1; ++g) {
+    sm_steps[g] += base_s;
+    sm_tiles[g] += base_t;
+  }
+  __syncthreads();
+  c.total *= p.nkv;
+  c.chunk = max((int64_t)kMinChunk, (c.total + warps - 1) / warps);
+  return c;
+}
+
+struct Place {  // where a step lies
+  Unit unit;
+  int u, j;       // unit and tile in it
+  int tile;       // number of the tile in the call
+  int g;          // kv head
+  int block;      // block in the tile
+  int blocks;     // blocks of the tile
+  int64_t begin;  // first step of (tile, kv head)
+};
+
+// Finds step x of the line; the same for all lanes of a warp.
+__device__ __forceinline__ Place find_step(const Q8AttnParams& p, int64_t x, int qt, int n_units, int per_group,
+                                           const int64_t* sm_steps, const int* sm_tiles) {
+  const int groups = (n_units + per_group - 1) / per_group;
+  int lo = 0, hi = groups - 1;
+  while (lo < hi) {  // the last group that begins at or before x (empty ones share their successor's begin)
+    const int mid = (lo + hi + 1) >> 1;
+    if (sm_steps[mid] * p.nkv <= x) lo = mid; else hi = mid - 1;
+  }
+  Place r;
+  r.u = lo * per_group;
+  r.tile = sm_tiles[lo];
+  int64_t before = sm_steps[lo];
+  for (;; ++r.u) {
+    r.unit = unit_of(p, r.u);
+    const int n = tiles_of(r.unit, qt);
+    const int64_t all = blocks_before(r.unit, qt, n);
+    if (x < (before + all) * p.nkv || r.u == n_units - 1) break;
+    before += all;
+    r.tile += n;
+  }
+  int a = 0, b = tiles_of(r.unit, qt) - 1;
+  while (a < b) {
+    const int mid = (a + b + 1) >> 1;
+    if ((before + blocks_before(r.unit, qt, mid)) * p.nkv <= x) a = mid; else b = mid - 1;
+  }
+  r.j = a;
+  r.tile += a;
+  before += blocks_before(r.unit, qt, a);
+  r.blocks = blocks_of((int64_t)r.unit.ctx0 + min((a + 1) * qt, r.unit.len));
+  const int64_t in = x - before * p.nkv;
+  r.g = (int)(in / r.blocks);
+  r.block = (int)(in % r.blocks);
+  r.begin = x - r.block;
+  return r;
+}
+
+// Moves to the first step of the next (tile, kv head).
+__device__ __forceinline__ void next_pair(const Q8AttnParams& p, Place& r, int qt) {
+  r.begin += r.blocks;
+  r.block = 0;
+  if (++r.g < p.nkv) return;
+  r.g = 0;
+  ++r.tile;
+  ++r.j;
+  while (r.j >= tiles_of(r.unit, qt)) {  // the caller has checked that there is another step
+    r.unit = unit_of(p, ++r.u);
+    r.j = 0;
+  }
+  r.blocks = blocks_of((int64_t)r.unit.ctx0 + min((r.j + 1) * qt, r.unit.len));
+}
+
+// ------------------------------------------------------------------ fragments
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
+
+// Two pairs of codes (the bytes 0, 1 and 2, 3 of x) as float16 pairs.
+template <int CODE>
+__device__ __forceinline__ void expand(uint32_t x, uint32_t& lo, uint32_t& hi) {
+  if constexpr (CODE == B2_I8) {
+    // 0x6400 | u is the float16 1024 + u for a byte u; u = code + 128
+    const uint32_t u = x ^ 0x80808080u;
+    const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));  // 1152
+    uint32_t a = prmt(u, 0x64646464u, 0x4140), b = prmt(u, 0x64646464u, 0x4342);
+    const __half2 ha = __hsub2(*reinterpret_cast<__half2*>(&a), bias), hb = __hsub2(*reinterpret_cast<__half2*>(&b), bias);
+    lo = *reinterpret_cast<const uint32_t*>(&ha);
+    hi = *reinterpret_cast<const uint32_t*>(&hb);
+  } else {
+    const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(x & 0xffffu), __NV_E4M3);
+    const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(x >> 16), __NV_E4M3);
+    lo = *reinterpret_cast<const uint32_t*>(&a);
+    hi = *reinterpret_cast<const uint32_t*>(&b);
+  }
+}
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <int BYTES>
+__device__ __forceinline__ void ld_codes(const uint8_t* p, uint32_t* w) {
+  if constexpr (BYTES == 16) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+  } else if constexpr (BYTES == 8) {
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+    w[0] = v.x; w[1] = v.y;
+  } else {
+    w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+  }
+}
+
+__device__ __forceinline__ void ld4q(const float* p, float (&v)[4]) {
+  const float4 a = *reinterpret_cast<const float4*>(p);
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+}
+__device__ __forceinline__ void ld4q(const __nv_bfloat16* p, float (&v)[4]) {
+  const uint2 a = *reinterpret_cast<const uint2*>(p);
+  v[0] = __uint_as_float(a.x << 16); v[1] = __uint_as_float(a.x & 0xffff0000u);
+  v[2] = __uint_as_float(a.y << 16); v[3] = __uint_as_float(a.y & 0xffff0000u);
+}
+
+template <typename T, int HD, int CODE, int NT>
+struct AttnCfg {
+  static constexpr int N = 8 * NT;                       // columns of a tile
+  static constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;   // float16 terms of q and P
+  static constexpr int KW = HD / 16;                     // words of codes a lane holds of a key; MMAs of S
+  static constexpr int VW = HD / 32;                     // and of a key's values
+  static constexpr int KB = KW >= 4 ? 16 : 4 * KW;       // bytes of one K load
+  static constexpr int SMEM_Q = kWarps * KW * NT * TERMS * 32 * 8;
+};
+
+// CTAs per SM the registers are limited for.
+template <int NT, int TERMS>
+constexpr int kCtas = NT * TERMS == 1 ? 4 : NT * TERMS == 2 ? 3 : 2;
+
+template <typename T, int HD, int CODE, int NT>
+__global__ void __launch_bounds__(kWarps * 32, kCtas<NT, (sizeof(T) == 4 ? 2 : 1)>)
+q8_attn_kernel(Q8AttnParams p, int qt, int n_units, int per_group) {
   pdl_wait();
   pdl_trigger();
-  __shared__ float sq[HD], sp[kRowThreads], red[32];
-  __shared__ int64_t sblk[kRowThreads];
-  const int row = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
-  const int g = h / (p.nq / p.nkv);
-  int trow, ctx;
-  if (p.seq_start) {
-    int s = -1;
-    for (int i = 0; i < p.n_seqs; ++i)
-      if (row >= p.seq_start[i] && row < p.seq_start[i + 1]) s = i;
-    if (s < 0) return;  // behind the last sequence: left as it was
-    trow = s;
-    ctx = (p.seq_ctx0 ? p.seq_ctx0[s] : 0) + row - p.seq_start[s] + 1;
-  } else {
-    trow = p.table_index ? p.table_index[row] : row;
-    ctx = max(0, p.ctx_lens[row]);
+  using C = AttnCfg<T, HD, CODE, NT>;
+  constexpr int KW = C::KW, VW = C::VW, TERMS = C::TERMS, N = C::N;
+  __shared__ int64_t sm_steps[kGroups];
+  __shared__ int sm_tiles[kGroups];
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int r8 = lane >> 2, t4 = lane & 3;
+  const int warps = gridDim.x * kWarps, w = blockIdx.x * kWarps + warp;
+  const int rep = p.nq / p.nkv;
+  uint2* sq = reinterpret_cast<uint2*>(smem) + warp * (KW * NT * TERMS * 32);
+
+  const Cut cut = make_cut(p, qt, n_units, per_group, sm_steps, sm_tiles, warps, blockIdx.x == 0);
+  // a seq_start that goes back may name more tokens than there are rows (and tiles than the
+  // workspace has room for): nothing is computed
+  const bool sane = !p.seq_start || (int64_t)cut.tiles <= (int64_t)(p.n_rows / qt) + n_units;
+  if (w == 0 && lane == 0) {
+    p.ws_tiles[0] = sane ? cut.tiles : 0;
+    if (!sane) raise_status(p.status, B2_DEV_RANGE);
   }
-  if (trow < 0 || trow >= p.table_rows || (int64_t)p.table_stride * kQ8Block < ctx) {
-    if (tid == 0) raise_status(p.status, B2_DEV_RANGE);
-    ctx = trow < 0 || trow >= p.table_rows ? 0 : p.table_stride * kQ8Block;
+  if (!sane) return;
+  if (!p.seq_start) {  // decode rows without keys
+    for (int u = blockIdx.x; u < n_units; u += gridDim.x) {
+      if (unit_of(p, u).len > 0) continue;
+      T* dst = reinterpret_cast<T*>(p.out) + (int64_t)u * p.ld_out;
+      for (int i = threadIdx.x; i < p.nq * HD; i += kWarps * 32) dst[i] = from_f32<T>(0.f);
+    }
   }
+  int64_t x = w * cut.chunk;
+  const int64_t x_end = min(cut.total, x + cut.chunk);
+  if (x >= x_end) return;
+  Place at = find_step(p, x, qt, n_units, per_group, sm_steps, sm_tiles);
+  constexpr int key_stride = HD;  // bytes between keys of a tile
+
+  for (bool first = true; x < x_end; first = false) {
+    const int i0 = at.block;
+    const int i1 = (int)min((int64_t)at.blocks, i0 + (x_end - x));
+    const int tok0 = at.j * qt, ntok = min(qt, at.unit.len - tok0);
+    const int ncol = ntok * rep;
+    const int pos0 = at.unit.ctx0 + tok0;           // position of the tile's first token
+    const int pos_last = pos0 + ntok - 1;
+    const int32_t* table = p.tables + (int64_t)table_row(p, at.u) * p.table_stride;
+    const uint8_t* kc = p.k_cache + (int64_t)at.g * (kQ8Block * HD);
+    const uint8_t* vc = p.v_cache + (int64_t)at.g * (kQ8Block * HD);
+    const int64_t blk_bytes = (int64_t)p.nkv * (kQ8Block * HD);
+
+    // q of the tile's columns into this warp's shared memory, as B fragments.
+    float colscale[NT][2];
+    int lim[NT][2];  // last key of the lane's columns
+    __syncwarp();
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int col = nt * 8 + r8;
+      float q[KW][4];
+      float big = 0.f;
+      const bool live = col < ncol;
+      const T* src = reinterpret_cast<const T*>(p.q) + (int64_t)(at.unit.start + tok0 + (live ? col / rep : 0)) * p.ld_q +
+                     (int64_t)(at.g * rep + (live ? col % rep : 0)) * HD;
+#pragma unroll
+      for (int k = 0; k < KW; ++k) {
+        const int d = KW >= 4 ? (k / 4) * 64 + t4 * 16 + (k % 4) * 4 : t4 * (KW * 4) + k * 4;
+        ld4q(src + d, q[k]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (!live) q[k][e] = 0.f;
+          big = fmaxf(big, fabsf(q[k][e]));
+        }
+      }
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+      // a power of two that brings `big` to [2^14, 2^15); in two factors, so that neither overflows
+      const int ex = big > 0.f && big <= 3.402823466e38f ? 14 - ilogbf(big) : 0;
+      const float up = ldexpf(1.f, ex / 2), up2 = ldexpf(1.f, ex - ex / 2);
+#pragma unroll
+      for (int k = 0; k < KW; ++k) {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = q[k][e] * up * up2;
+#pragma unroll
+        for (int term = 0; term < TERMS; ++term) {
+          uint2 f;
+          f.x = pack_f16(v[0], v[1]);
+          f.y = pack_f16(v[2], v[3]);
+          sq[((k * NT + nt) * TERMS + term) * 32 + lane] = f;
+          if (TERMS == 2) {
+            const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&f.x));
+            const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&f.y));
+            v[0] -= a.x; v[1] -= a.y; v[2] -= b.x; v[3] -= b.y;
+          }
+        }
+      }
+      const float back = live ? ldexpf(p.scale_log2, -ex) : 0.f;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int c = nt * 8 + 2 * t4 + e;
+        colscale[nt][e] = __shfl_sync(0xffffffffu, back, (2 * t4 + e) * 4);
+        lim[nt][e] = c < ncol ? pos0 + c / rep : -1;
+      }
+    }
+    __syncwarp();
+
+    float o[2 * VW][NT][4];
+    float m[NT][2], m2[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int d = 0; d < 2 * VW; ++d) o[d][nt][0] = o[d][nt][1] = o[d][nt][2] = o[d][nt][3] = 0.f;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        m[nt][e] = m2[nt][e] = -INFINITY;
+        l[nt][e] = 0.f;
+      }
+    }
+
+    // Block ids and scales, 32 steps at a time, one per lane.
+    int win = i0, ids = 0;
+    float kss = 0.f, vss = 0.f;
+    auto window = [&](int i) {
+      win = i;
+      int id = -1;
+      if (i + lane < i1) {
+        id = __ldg(table + i + lane);
+        if (id < 0 || id >= p.num_blocks) {
+          raise_status(p.status, B2_DEV_RANGE);
+          id = -1;
+        }
+      }
+      ids = id;
+      kss = id >= 0 ? __ldg(p.k_scale + q8_scale(id, p.nkv, at.g)) : 0.f;
+      vss = id >= 0 ? __ldg(p.v_scale + q8_scale(id, p.nkv, at.g)) : 0.f;
+    };
+    uint32_t kw[2][KW], vw[4][VW];
+    auto load_k = [&](int blk) {
+      const uint8_t* src = kc + (int64_t)max(blk, 0) * blk_bytes + r8 * key_stride + t4 * C::KB;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int k = 0; k < KW; k += C::KB / 4) ld_codes<C::KB>(src + h * 8 * key_stride + (k / 4) * 64, &kw[h][k]);
+    };
+    auto load_v = [&](int blk) {
+      const uint8_t* src = vc + (int64_t)max(blk, 0) * blk_bytes + 2 * t4 * key_stride + r8 * (4 * VW);
+#pragma unroll
+      for (int h = 0; h < 4; ++h) ld_codes<4 * VW>(src + ((h & 1) + (h >> 1) * 8) * key_stride, vw[h]);
+    };
+    window(i0);
+    int blk = __shfl_sync(0xffffffffu, ids, 0);
+    load_k(blk);
+    load_v(blk);
+
+    for (int i = i0; i < i1; ++i) {
+      const float ks = __shfl_sync(0xffffffffu, kss, i - win), vs = __shfl_sync(0xffffffffu, vss, i - win);
+      if (i + 1 < i1 && i + 1 - win == 32) window(i + 1);
+      const int nblk = __shfl_sync(0xffffffffu, ids, (i + 1 - win) & 31);
+      const bool more = i + 1 < i1;
+      if (blk < 0) {  // a block outside the pool: its keys are left out
+        if (more) {
+          load_k(nblk);
+          load_v(nblk);
+        }
+        blk = nblk;
+        continue;
+      }
+      float s[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KW; ++k) {
+        uint32_t a[4];
+        expand<CODE>(kw[0][k], a[0], a[2]);
+        expand<CODE>(kw[1][k], a[1], a[3]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int term = 0; term < TERMS; ++term) {
+            const uint2 b = sq[((k * NT + nt) * TERMS + term) * 32 + lane];
+            mma_f16(s[nt], a, b.x, b.y);
+          }
+      }
+      if (more) load_k(nblk);
+
+      // scores; the tail of the tile's keys is masked per column
+      const int key = i * kQ8Block + r8;
+      const bool tail = (i + 1) * kQ8Block - 1 > pos0;
+      const float lv = vs > 0.f ? __log2f(vs) : vs == 0.f ? -INFINITY : vs;
+      bool move = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float cs = colscale[nt][e] * ks;
+          float a = s[nt][e] * cs, b = s[nt][2 + e] * cs;
+          if (tail) {
+            if (key > lim[nt][e]) a = -INFINITY;
+            if (key + 8 > lim[nt][e]) b = -INFINITY;
+          }
+          s[nt][e] = a;
+          s[nt][2 + e] = b;
+          const float top = fminf(m[nt][e], m2[nt][e] - lv) + 15.f;
+          move |= a > top || b > top;
+        }
+      if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float mx = fmaxf(s[nt][e], s[nt][2 + e]);
+#pragma unroll
+            for (int sh = 4; sh < 32; sh <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, sh));
+            const float mn = fmaxf(m[nt][e], mx - 8.f), m2n = fmaxf(m2[nt][e], mx - 8.f + lv);
+            l[nt][e] *= mn == -INFINITY ? 1.f : exp2f(m[nt][e] - mn);
+            const float c = m2n == -INFINITY ? 1.f : exp2f(m2[nt][e] - m2n);
+            m[nt][e] = mn;
+            m2[nt][e] = m2n;
+#pragma unroll
+            for (int d = 0; d < 2 * VW; ++d) {
+              o[d][nt][e] *= c;
+              o[d][nt][2 + e] *= c;
+            }
+          }
+      }
+      uint32_t pb[NT][TERMS][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float pa[2], pc[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float f = vs == 0.f ? 0.f : vs * ex2(m[nt][e] - m2[nt][e]);
+          float a = ex2(s[nt][e] - m[nt][e]), b = ex2(s[nt][2 + e] - m[nt][e]);
+          pa[e] = a * f;
+          pc[e] = b * f;
+          if (tail) {
+            if (key > lim[nt][e]) a = pa[e] = 0.f;
+            if (key + 8 > lim[nt][e]) b = pc[e] = 0.f;
+          }
+          l[nt][e] += a + b;
+        }
+#pragma unroll
+        for (int term = 0; term < TERMS; ++term) {
+          const uint32_t lo = pack_f16(pa[0], pa[1]), hi = pack_f16(pc[0], pc[1]);
+          pb[nt][term][0] = transpose8x8(lo);
+          pb[nt][term][1] = transpose8x8(hi);
+          if (TERMS == 2) {
+            const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+            const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+            pa[0] -= fa.x; pa[1] -= fa.y; pc[0] -= fb.x; pc[1] -= fb.y;
+          }
+        }
+      }
+      if (tail && (i + 1) * kQ8Block - 1 > pos_last) {  // keys no column sees: whatever their codes
+        const int k0 = i * kQ8Block + 2 * t4;
+#pragma unroll
+        for (int h = 0; h < 4; ++h)
+          if (k0 + (h & 1) + (h >> 1) * 8 > pos_last) {
+#pragma unroll
+            for (int v = 0; v < VW; ++v) vw[h][v] = 0u;
+          }
+      }
+#pragma unroll
+      for (int v = 0; v < VW; ++v) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t sel = half ? 0x7362 : 0x5140;
+          uint32_t a[4];
+          expand<CODE>(prmt(vw[0][v], vw[1][v], sel), a[0], a[1]);
+          expand<CODE>(prmt(vw[2][v], vw[3][v], sel), a[2], a[3]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int term = 0; term < TERMS; ++term)
+              mma_f16(o[2 * v + half][nt], a, pb[nt][term][0], pb[nt][term][1]);
+        }
+      }
+      if (more) load_v(nblk);
+      blk = nblk;
+    }
+
+    // The lane holds, of columns 2 t4 and 2 t4 + 1 of every n-tile, dims r8 * HD/8 .. + HD/8 - 1.
+    const bool whole = i0 == 0 && i1 == at.blocks;
+    const int64_t slot = 2 * (int64_t)w + (first ? 0 : 1);
+    if (!whole && i0 == 0 && lane == 0) {
+      const int64_t last = (at.begin + at.blocks - 1) / cut.chunk;
+      p.ws_pairs[(int64_t)at.tile * p.nkv + at.g] = make_int4(w, (int)last, at.u, at.j | (first ? 0x40000000 : 0));
+    } else if (whole && lane == 0) {
+      p.ws_pairs[(int64_t)at.tile * p.nkv + at.g] = make_int4(0, -1, 0, 0);  // nothing to join
+    }
+    int npad = 0;
+    if (p.compat_pad) npad = max(0, cut.max_ctx - (pos0 + 1));
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float lt = l[nt][e];
+#pragma unroll
+        for (int sh = 4; sh < 32; sh <<= 1) lt += __shfl_xor_sync(0xffffffffu, lt, sh);
+        const int c = nt * 8 + 2 * t4 + e;
+        if (c >= ncol) continue;
+        float f = 1.f;
+        if (whole) {
+          float mm = m[nt][e];
+          if (npad > 0) {
+            const float mp = fmaxf(mm, 0.f);
+            lt = (mm == -INFINITY ? 0.f : lt * exp2f(mm - mp)) + (float)npad * exp2f(-mp);
+            mm = mp;
+          }
+          f = m2[nt][e] == -INFINITY ? (lt == lt ? 0.f : lt) : exp2f(m2[nt][e] - mm) / lt;
+        }
+        float v[4 * VW];
+#pragma unroll
+        for (int d = 0; d < 2 * VW; ++d) {
+          v[2 * d] = o[d][nt][e] * f;
+          v[2 * d + 1] = o[d][nt][2 + e] * f;
+        }
+        if (whole) {
+          T* dst = reinterpret_cast<T*>(p.out) + (int64_t)(at.unit.start + tok0 + c / rep) * p.ld_out +
+                   (int64_t)(at.g * rep + c % rep) * HD + r8 * (4 * VW);
+          if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int d = 0; d < VW; ++d)
+              reinterpret_cast<float4*>(dst)[d] = make_float4(v[4 * d], v[4 * d + 1], v[4 * d + 2], v[4 * d + 3]);
+          } else {
+#pragma unroll
+            for (int d = 0; d < VW; ++d) {
+              const __nv_bfloat162 a = __floats2bfloat162_rn(v[4 * d], v[4 * d + 1]);
+              const __nv_bfloat162 b = __floats2bfloat162_rn(v[4 * d + 2], v[4 * d + 3]);
+              reinterpret_cast<uint2*>(dst)[d] =
+                  make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+            }
+          }
+        } else {
+          float4* dst = reinterpret_cast<float4*>(p.ws_o + (slot * N + c) * HD + r8 * (4 * VW));
+#pragma unroll
+          for (int d = 0; d < VW; ++d) dst[d] = make_float4(v[4 * d], v[4 * d + 1], v[4 * d + 2], v[4 * d + 3]);
+          if (r8 == 0) p.ws_stat[slot * N + c] = make_float4(m[nt][e], lt, m2[nt][e], 0.f);
+        }
+      }
+    x += i1 - i0;
+    if (x < x_end) next_pair(p, at, qt);
+  }
+}
+
+// Joins the pieces of the tiles that several warps worked on.  One CTA per (tile, kv head);
+// its warps share the columns, and the pieces of a column where there are fewer columns than
+// warps.
+constexpr int kJoinWarps = 8;
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kJoinWarps * 32) q8_join_kernel(Q8AttnParams p, int qt, int columns) {
+  pdl_wait();
+  pdl_trigger();
+  constexpr int E = HD / 32;  // dims per lane
+  __shared__ float part[kJoinWarps][HD];
+  __shared__ int most[kJoinWarps];
+  const int rep = p.nq / p.nkv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = blockIdx.y;
+  if ((int)blockIdx.x >= p.ws_tiles[0]) return;
+  const int4 pair = p.ws_pairs[(int64_t)blockIdx.x * p.nkv + g];
+  if (pair.y < pair.x) return;  // one warp saw the whole tile
+  const Unit u = unit_of(p, pair.z);
+  const int tok0 = (pair.w & 0x3fffffff) * qt, n = pair.y - pair.x + 1;
+  const int64_t slot0 = 2 * (int64_t)pair.x + (pair.w & 0x40000000 ? 0 : 1);
+  const int ncol = min(qt, u.len - tok0) * rep;
   int npad = 0;
   if (p.compat_pad) {
     int mx = 0;
-    for (int i = 0; i < p.n_rows; ++i) mx = max(mx, p.ctx_lens[i]);
-    npad = max(0, mx - ctx);
-  }
-  const int32_t* table = p.tables + (int64_t)trow * p.table_stride;
-  const T* q = reinterpret_cast<const T*>(p.q) + (int64_t)row * p.ld_q + (int64_t)h * HD;
-  for (int d = tid; d < HD; d += kRowThreads) sq[d] = to_f32(q[d]);
-  float m = npad > 0 ? 0.f : -INFINITY, l = (float)npad, acc = 0.f;
-  for (int t0 = 0; t0 < ctx; t0 += kRowThreads) {
+    for (int i = threadIdx.x; i < p.n_rows; i += kJoinWarps * 32) mx = max(mx, p.ctx_lens[i]);
+    mx = __reduce_max_sync(0xffffffffu, mx);
+    if (lane == 0) most[warp] = mx;
     __syncthreads();
-    const int t = t0 + tid;
-    float s = -INFINITY;
-    int64_t blk = -1;
-    if (t < ctx) {
-      blk = table[t / kQ8Block];
-      if (blk < 0 || blk >= p.num_blocks) {
-        raise_status(p.status, B2_DEV_RANGE);
-        blk = -1;
-      } else {
-        const uint32_t* w = reinterpret_cast<const uint32_t*>(p.k_cache + q8_tile(blk, p.nkv, g, HD) + t % kQ8Block * HD);
-        float dot = 0.f;
-        for (int i = 0; i < HD / 4; ++i) {
-          float v[4];
-          Q8<CODE>::decode4(w[i], v);
-          for (int e = 0; e < 4; ++e) dot = fmaf(v[e], sq[i * 4 + e], dot);
+    for (int i = 0; i < kJoinWarps; ++i) mx = max(mx, most[i]);
+    npad = max(0, mx - (u.ctx0 + 1));
+  }
+  int share = 1;  // warps per column
+  while (share * 2 * ncol <= kJoinWarps) share *= 2;
+  for (int c0 = 0; c0 < ncol; c0 += kJoinWarps / share) {
+    const int c = c0 + warp / share, part_of = warp % share;
+    float M = npad > 0 ? 0.f : -INFINITY, l = 0.f, acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    auto where = [&](int k) { return (k == 0 ? slot0 : 2 * (int64_t)(pair.x + k)) * columns + c; };
+    if (c < ncol) {
+      for (int k = lane; k < n; k += 32) M = fmaxf(M, p.ws_stat[where(k)].x);
+      M = warp_max(M);
+      for (int k0 = 0; k0 < n; k0 += 32) {
+        float f = 0.f;
+        if (k0 + lane < n) {
+          const float4 st = p.ws_stat[where(k0 + lane)];
+          if (st.x != -INFINITY) l += st.y * exp2f(st.x - M);
+          else if (st.y != st.y) l = st.y;
+          if (st.z != -INFINITY) f = exp2f(st.z - M);
         }
-        s = dot * p.k_scale[q8_scale(blk, p.nkv, g)] * p.scale_log2;
+        const int most_k = min(32, n - k0);
+#pragma unroll 4
+        for (int i = part_of; i < most_k; i += share) {
+          const float fi = __shfl_sync(0xffffffffu, f, i);
+          const float* src = p.ws_o + where(k0 + i) * HD + lane * E;
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[e] = fmaf(src[e], fi, acc[e]);
+        }
       }
+      l = warp_sum(l) + (npad > 0 ? (float)npad * exp2f(-M) : 0.f);
     }
-    sblk[tid] = blk;
-    float mx = warp_max(s);
-    if ((tid & 31) == 0) red[tid >> 5] = mx;
-    __syncthreads();
-    mx = m;
-    for (int w = 0; w < kRowThreads / 32; ++w) mx = fmaxf(mx, red[w]);
-    const float corr = mx == -INFINITY ? 1.f : exp2f(m - mx);
-    sp[tid] = blk < 0 ? 0.f : exp2f(s - mx);
-    __syncthreads();
-    m = mx;
-    l *= corr;
-    acc *= corr;
-    const int n = min(kRowThreads, ctx - t0);
-    for (int i = 0; i < n; ++i) {
-      l += sp[i];
-      if (tid < HD && sblk[i] >= 0) {
-        float v[4];
-        Q8<CODE>::decode4(p.v_cache[q8_tile(sblk[i], p.nkv, g, HD) + (t0 + i) % kQ8Block * HD + tid], v);
-        acc = fmaf(sp[i] * p.v_scale[q8_scale(sblk[i], p.nkv, g)], v[0], acc);
-      }
+    if (share > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < E; ++e) part[warp][lane * E + e] = acc[e];
+      __syncthreads();
+      if (part_of == 0)
+        for (int w = 1; w < share; ++w)
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[e] += part[warp + w][lane * E + e];
     }
-  }
-  if (tid < HD) {
-    T* out = reinterpret_cast<T*>(p.out) + (int64_t)row * p.ld_out + (int64_t)h * HD;
-    out[tid] = from_f32<T>(l == 0.f ? 0.f : acc / l);
+    if (c < ncol && part_of == 0) {
+      T* dst = reinterpret_cast<T*>(p.out) + (int64_t)(u.start + tok0 + c / rep) * p.ld_out +
+               (int64_t)(g * rep + c % rep) * HD + lane * E;
+#pragma unroll
+      for (int e = 0; e < E; ++e) dst[e] = from_f32<T>(l == 0.f ? 0.f : acc[e] / l);
+    }
   }
 }
 
@@ -142,25 +788,81 @@ int check_q8_pointers(const char* name, const Q8AttnParams& p, int dtype) {
   return B2_OK;
 }
 
-template <typename T, int HD>
-int launch_rows(const Q8AttnParams& p, int cache_dtype, cudaStream_t s) {
-  const dim3 grid(p.n_rows, p.nq);
-  if (cache_dtype == B2_I8)
-    B2_TRY_CUDA(launch_pdl((q8_attn_row_kernel<T, HD, B2_I8>), grid, dim3(kRowThreads), 0, s, p));
-  else
-    B2_TRY_CUDA(launch_pdl((q8_attn_row_kernel<T, HD, B2_E4M3>), grid, dim3(kRowThreads), 0, s, p));
+
+// ------------------------------------------------------------------ host side
+size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+
+struct AttnPlan {
+  int nt, qt, units, per_group, ctas, slots;
+  int64_t tiles;  // at most
+  size_t pairs, stat, o, total;  // workspace offsets
+};
+
+// Columns of a tile.  A decode row has rep columns.  A sequence of a prefill has tokens * rep;
+// wide tiles read the cache once for more of them, narrow ones keep more warps resident and
+// waste fewer columns of the products, so the width follows the mean length.
+AttnPlan plan_of(int n_rows, int nq, int nkv, int hd, int n_seqs, bool prefill, int dtype) {
+  AttnPlan a{};
+  const int rep = nq / nkv, terms = dtype == B2_F32 ? 2 : 1;
+  const int64_t columns = prefill ? (int64_t)((n_rows + n_seqs - 1) / n_seqs) * rep : rep;
+  a.nt = columns <= 8 && rep <= 8 ? 1 : columns <= 16 || terms == 2 ? 2 : 4;
+  a.qt = prefill ? 8 * a.nt / rep : 1;
+  a.units = prefill ? n_seqs : n_rows;
+  a.per_group = (a.units + kGroups - 1) / kGroups;
+  const int w = a.nt * terms;
+  a.ctas = sm_count() * (w == 1 ? 4 : w == 2 ? 3 : 2);
+  a.slots = 2 * a.ctas * kWarps;
+  a.tiles = prefill ? (int64_t)n_rows / a.qt + n_seqs : n_rows;
+  a.pairs = 256;
+  a.stat = a.pairs + align256((size_t)a.tiles * nkv * sizeof(int4));
+  a.o = a.stat + align256((size_t)a.slots * 8 * a.nt * sizeof(float4));
+  a.total = a.o + (size_t)a.slots * 8 * a.nt * hd * sizeof(float);
+  return a;
+}
+
+template <typename T, int HD, int CODE, int NT>
+int launch_tiles(const Q8AttnParams& p, const AttnPlan& a, cudaStream_t s) {
+  using C = AttnCfg<T, HD, CODE, NT>;
+  B2_TRY_CUDA(launch_pdl((q8_attn_kernel<T, HD, CODE, NT>), dim3(a.ctas), dim3(kWarps * 32), C::SMEM_Q, s, p, a.qt,
+                         a.units, a.per_group));
+  B2_TRY_CUDA(launch_pdl((q8_join_kernel<T, HD>), dim3((unsigned)a.tiles, p.nkv), dim3(kJoinWarps * 32), 0, s, p, a.qt,
+                         8 * a.nt));
   return B2_OK;
 }
 
-int launch(const Q8AttnParams& p, int hd, int cache_dtype, int dtype, cudaStream_t s) {
-  if (dtype == B2_BF16) {
-    if (hd == 32) return launch_rows<__nv_bfloat16, 32>(p, cache_dtype, s);
-    if (hd == 64) return launch_rows<__nv_bfloat16, 64>(p, cache_dtype, s);
-    return launch_rows<__nv_bfloat16, 128>(p, cache_dtype, s);
+template <typename T, int HD, int CODE>
+int launch_nt(const Q8AttnParams& p, const AttnPlan& a, cudaStream_t s) {
+  if (a.nt == 1) return launch_tiles<T, HD, CODE, 1>(p, a, s);
+  if (a.nt == 2) return launch_tiles<T, HD, CODE, 2>(p, a, s);
+  if constexpr (sizeof(T) == 2) return launch_tiles<T, HD, CODE, 4>(p, a, s);
+  return fail(B2_ENOTSUP, "attention over the 8-bit cache: no tile of %d columns", 8 * a.nt);
+}
+
+template <typename T>
+int launch_hd(const Q8AttnParams& p, int hd, int code, const AttnPlan& a, cudaStream_t s) {
+  if (code == B2_I8) {
+    if (hd == 32) return launch_nt<T, 32, B2_I8>(p, a, s);
+    if (hd == 64) return launch_nt<T, 64, B2_I8>(p, a, s);
+    return launch_nt<T, 128, B2_I8>(p, a, s);
   }
-  if (hd == 32) return launch_rows<float, 32>(p, cache_dtype, s);
-  if (hd == 64) return launch_rows<float, 64>(p, cache_dtype, s);
-  return launch_rows<float, 128>(p, cache_dtype, s);
+  if (hd == 32) return launch_nt<T, 32, B2_E4M3>(p, a, s);
+  if (hd == 64) return launch_nt<T, 64, B2_E4M3>(p, a, s);
+  return launch_nt<T, 128, B2_E4M3>(p, a, s);
+}
+
+int launch(const char* name, Q8AttnParams& p, int hd, int cache_dtype, int dtype, void* workspace, size_t bytes,
+           cudaStream_t s) {
+  const AttnPlan a = plan_of(p.n_rows, p.nq, p.nkv, hd, p.n_seqs, p.seq_start != nullptr, dtype);
+  B2_CHECK_ARG(a.tiles <= 0x7fffffff && p.nkv <= 65535, "%s: too many tiles or kv heads", name);
+  B2_CHECK_ARG(workspace && bytes >= a.total, "%s: workspace of %zu bytes needed, %zu given", name, a.total, bytes);
+  B2_CHECK_ARG(((uintptr_t)workspace % 16) == 0, "%s: the workspace must be 16-byte aligned", name);
+  char* ws = static_cast<char*>(workspace);
+  p.ws_tiles = reinterpret_cast<int*>(ws);
+  p.ws_pairs = reinterpret_cast<int4*>(ws + a.pairs);
+  p.ws_stat = reinterpret_cast<float4*>(ws + a.stat);
+  p.ws_o = reinterpret_cast<float*>(ws + a.o);
+  return dtype == B2_BF16 ? launch_hd<__nv_bfloat16>(p, hd, cache_dtype, a, s)
+                          : launch_hd<float>(p, hd, cache_dtype, a, s);
 }
 
 void set_cache(Q8AttnParams& p, const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
@@ -177,7 +879,10 @@ void set_cache(Q8AttnParams& p, const void* k_cache, const void* v_cache, const 
 
 extern "C" {
 
-size_t b2_paged_attention_q8_workspace_bytes(int n_rows, int nq, int nkv, int head_dim) { return 0; }
+size_t b2_paged_attention_q8_workspace_bytes(int n_rows, int nq, int nkv, int head_dim, int dtype) {
+  if (n_rows <= 0 || nkv <= 0 || nq < nkv || nq / nkv > 16 || head_dim <= 0) return 0;
+  return b2::plan_of(n_rows, nq, nkv, head_dim, 0, false, dtype).total;
+}
 
 int b2_paged_attention_q8(const void* q, int64_t ld_q, int n_rows, int nq, int nkv, int head_dim, const void* k_cache,
                           const void* v_cache, const float* k_scale, const float* v_scale, int cache_dtype, int layer,
@@ -189,7 +894,7 @@ int b2_paged_attention_q8(const void* q, int64_t ld_q, int n_rows, int nq, int n
   const char* name = "b2_paged_attention_q8";
   Q8AttnParams p{q, ld_q, n_rows, nq, nkv, (const uint8_t*)k_cache, (const uint8_t*)v_cache, k_scale, v_scale,
                  num_blocks, block_tables, table_rows, table_stride, table_index, ctx_lens, compat_pad, nullptr,
-                 nullptr, 0, scale * 1.4426950408889634f, out, ld_out, status};
+                 nullptr, 0, scale * 1.4426950408889634f, out, ld_out, status, nullptr, nullptr, nullptr, nullptr};
   int rc = check_q8_attention(name, p, head_dim, cache_dtype, layer, block_size, dtype);
   if (rc || n_rows == 0) return rc;
   rc = check_q8_pointers(name, p, dtype);
@@ -197,10 +902,13 @@ int b2_paged_attention_q8(const void* q, int64_t ld_q, int n_rows, int nq, int n
   B2_CHECK_ARG(ctx_lens, "%s: null pointer", name);
   B2_CHECK_ARG(table_index || n_rows <= table_rows, "%s: %d rows for %d table rows", name, n_rows, table_rows);
   set_cache(p, k_cache, v_cache, k_scale, v_scale, layer, head_dim);
-  return launch(p, head_dim, cache_dtype, dtype, stream);
+  return launch(name, p, head_dim, cache_dtype, dtype, workspace, workspace_bytes, stream);
 }
 
-size_t b2_prefill_attention_q8_workspace_bytes(int n_rows, int nq, int nkv, int head_dim, int n_seqs) { return 0; }
+size_t b2_prefill_attention_q8_workspace_bytes(int n_rows, int nq, int nkv, int head_dim, int n_seqs, int dtype) {
+  if (n_rows <= 0 || n_seqs <= 0 || nkv <= 0 || nq < nkv || nq / nkv > 16 || head_dim <= 0) return 0;
+  return b2::plan_of(n_rows, nq, nkv, head_dim, n_seqs, true, dtype).total;
+}
 
 int b2_prefill_attention_q8(const void* q, int64_t ld_q, int n_rows, int nq, int nkv, int head_dim,
                             const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
@@ -212,7 +920,7 @@ int b2_prefill_attention_q8(const void* q, int64_t ld_q, int n_rows, int nq, int
   const char* name = "b2_prefill_attention_q8";
   Q8AttnParams p{q, ld_q, n_rows, nq, nkv, (const uint8_t*)k_cache, (const uint8_t*)v_cache, k_scale, v_scale,
                  num_blocks, block_tables, table_rows, table_stride, nullptr, nullptr, 0, seq_start, seq_ctx0, n_seqs,
-                 scale * 1.4426950408889634f, out, ld_out, status};
+                 scale * 1.4426950408889634f, out, ld_out, status, nullptr, nullptr, nullptr, nullptr};
   int rc = check_q8_attention(name, p, head_dim, cache_dtype, layer, block_size, dtype);
   if (rc) return rc;
   B2_CHECK_ARG(n_seqs >= 0, "%s: bad sizes", name);
@@ -222,7 +930,7 @@ int b2_prefill_attention_q8(const void* q, int64_t ld_q, int n_rows, int nq, int
   B2_CHECK_ARG(seq_start, "%s: null pointer", name);
   B2_CHECK_ARG(n_seqs <= table_rows, "%s: %d sequences for %d table rows", name, n_seqs, table_rows);
   set_cache(p, k_cache, v_cache, k_scale, v_scale, layer, head_dim);
-  return launch(p, head_dim, cache_dtype, dtype, stream);
+  return launch(name, p, head_dim, cache_dtype, dtype, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

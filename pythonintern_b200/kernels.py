@@ -567,7 +567,7 @@ def paged_attention_q8(q: torch.Tensor, nq: int, nkv: int, head_dim: int, k_cach
     _check(ctx_lens, "ctx_lens", torch.int32, n, dev)
     if table_index is not None:
         _check(table_index, "table_index", torch.int32, n, dev)
-    nbytes = _lib.lib().b2_paged_attention_q8_workspace_bytes(n, nq, nkv, head_dim)
+    nbytes = _lib.lib().b2_paged_attention_q8_workspace_bytes(n, nq, nkv, head_dim, dtype_code(q.dtype))
     # scratch of this call alone: another stream or graph may run at the same time
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _call("b2_paged_attention_q8", dev, ptr(q), _rows_stride(q), n, nq, nkv, head_dim, ptr(k_cache), ptr(v_cache),
@@ -590,7 +590,7 @@ def prefill_attention_q8(q: torch.Tensor, nq: int, nkv: int, head_dim: int, k_ca
     _check(seq_start, "seq_start", torch.int32, n_seqs + 1, dev)
     if seq_ctx0 is not None:
         _check(seq_ctx0, "seq_ctx0", torch.int32, n_seqs, dev)
-    nbytes = _lib.lib().b2_prefill_attention_q8_workspace_bytes(n, nq, nkv, head_dim, n_seqs)
+    nbytes = _lib.lib().b2_prefill_attention_q8_workspace_bytes(n, nq, nkv, head_dim, n_seqs, dtype_code(q.dtype))
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _call("b2_prefill_attention_q8", dev, ptr(q), _rows_stride(q), n, nq, nkv, head_dim, ptr(k_cache), ptr(v_cache),
           ptr(k_scale), ptr(v_scale), code, layer, NB, bs, ptr(block_tables), block_tables.shape[0],

@@ -472,7 +472,8 @@ def _stored(code, NB, nkv, hd, layers=1, seed=0):
 
 
 def _attend64(q, cache, layer, table, upto, scale, npad=0):
-    """One query token [nq, hd] over the first `upto` keys of `table`: (result, sum of p |v|) in float64."""
+    """One query token [nq, hd] over the first `upto` keys of `table`, in float64: the result, and what its
+    errors are measured by: sum of p |v|, and max(p vs) * sum of |code| (see _close)."""
     nkv, hd = cache[0].shape[2], cache[0].shape[4]
     q = q.double().cpu().view(nkv, -1, hd)
     nb = -(-upto // 16)
@@ -486,21 +487,31 @@ def _attend64(q, cache, layer, table, upto, scale, npad=0):
     s = torch.einsum("grd,gkd->grk", q, x[0]) * scale
     s = torch.where(ok, s, torch.tensor(-math.inf, dtype=torch.float64))
     s = torch.cat([s, torch.zeros(*s.shape[:2], npad, dtype=torch.float64)], -1)
-    if s.shape[-1] == 0 or bool(torch.isinf(s).all()):
+    if not ids or bool(torch.isinf(s).all()):
         z = torch.zeros(q.shape, dtype=torch.float64).reshape(-1)
-        return z, z
+        return z, (z, z)
     p = torch.softmax(s, -1)[..., :upto]
-    return (torch.einsum("grk,gkd->grd", p, x[1]).reshape(-1), torch.einsum("grk,gkd->grd", p, x[1].abs()).reshape(-1))
+    vs = torch.stack([cache[3][layer, max(b, 0)].cpu().double() for b in ids], 1).repeat_interleave(16, 1)[:, :upto]
+    codes = torch.stack([cache[1][layer, max(b, 0)].cpu().double() for b in ids]).transpose(0, 1).reshape(nkv, -1, hd)
+    loudest = (p * vs[:, None]).amax(-1)
+    small = loudest[..., None] * codes[:, :upto].abs().nan_to_num(0.0).sum(1)[:, None]
+    return (torch.einsum("grk,gkd->grd", p, x[1]).reshape(-1),
+            (torch.einsum("grk,gkd->grd", p, x[1].abs()).reshape(-1), small.reshape(-1)))
 
 
 def _close(got, want, size, dtype):
     """Elementwise: half a step of the output's type, half a float16 step of every probability
     (float32 queries: two float16 terms, 2^-22), and float32 scores and sums (the exponent of a
-    score of magnitude up to 2^5 errs by 2^5 * 2^-22, every sum by some 2^-20)."""
+    score of magnitude up to 2^5 errs by 2^5 * 2^-22, every sum by some 2^-20).  A float16 step is
+    relative only down to 2^-14; below, half a step is 2^-25.  The kernel holds the largest p * vs of a
+    tile at 2^8 or above, so a key's weight errs by at most 2^-33 of the largest one, and a sum over
+    keys by 2^-33 max(p vs) sum |code|: what is left where the key that takes the whole softmax holds
+    a code of exactly 0."""
+    size, small = size
     out = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24
     prob = 2.0 ** -11 if dtype == torch.bfloat16 else 2.0 ** -22
     err = (got.double().cpu() - want).abs()
-    limit = out * want.abs() + (prob + 2.0 ** -16) * size
+    limit = out * want.abs() + (prob + 2.0 ** -16) * size + 2.0 ** -33 * small
     assert torch.isfinite(got).all()
     assert (err <= limit * 1.01 + 1e-30).all(), float((err / (limit + 1e-30)).max())
 
