@@ -33,6 +33,13 @@
 #include "q8.cuh"
 
 namespace b2 {
+
+int prefill_attention_q8_tc(const void* q, int64_t ld_q, int n_rows, int nq, int nkv, const uint8_t* k_cache,
+                            const uint8_t* v_cache, const float* k_scale, const float* v_scale, int cache_dtype,
+                            int num_blocks, const int32_t* tables, int table_stride, const int32_t* seq_start,
+                            const int32_t* seq_ctx0, int n_seqs, float scale, void* out, int64_t ld_out,
+                            int32_t* status, cudaStream_t stream);
+
 namespace {
 
 struct Q8AttnParams {
@@ -790,6 +797,13 @@ int check_q8_pointers(const char* name, const Q8AttnParams& p, int dtype) {
 
 
 // ------------------------------------------------------------------ host side
+// Prefills of long enough pieces run on tcgen05 (prefill_q8_tc.cu).
+bool tensor_prefill(int n_rows, int n_seqs, int nq, int nkv, int hd, float scale, int dtype) {
+  const int rep = nq / nkv;
+  return dtype == B2_BF16 && hd == 128 && (rep == 1 || rep == 2 || rep == 4 || rep == 8) && scale > 0.f &&
+         n_rows >= 16 * n_seqs;
+}
+
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 struct AttnPlan {
@@ -930,6 +944,10 @@ int b2_prefill_attention_q8(const void* q, int64_t ld_q, int n_rows, int nq, int
   B2_CHECK_ARG(seq_start, "%s: null pointer", name);
   B2_CHECK_ARG(n_seqs <= table_rows, "%s: %d sequences for %d table rows", name, n_seqs, table_rows);
   set_cache(p, k_cache, v_cache, k_scale, v_scale, layer, head_dim);
+  if (tensor_prefill(n_rows, n_seqs, nq, nkv, head_dim, scale, dtype))
+    return prefill_attention_q8_tc(q, ld_q, n_rows, nq, nkv, p.k_cache, p.v_cache, p.k_scale, p.v_scale, cache_dtype,
+                                   num_blocks, block_tables, table_stride, seq_start, seq_ctx0, n_seqs, scale, out,
+                                   ld_out, status, stream);
   return launch(name, p, head_dim, cache_dtype, dtype, workspace, workspace_bytes, stream);
 }
 

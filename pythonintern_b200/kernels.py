@@ -355,7 +355,7 @@ class SlotMap(NamedTuple):
 
 def _check(t: torch.Tensor, name: str, dtype: torch.dtype, numel: int, device: torch.device):
     """A contiguous CUDA tensor of at least ``numel`` elements of ``dtype`` on ``device``."""
-    if t.dtype != dtype or t.device != device or not t.is_contiguous() or t.numel() < numel:
+    if t.dtype is not dtype or t.get_device() != device.index or not t.is_contiguous() or t.numel() < numel:
         raise _lib.B2Error(f"{name} must be a contiguous {dtype} tensor of at least {numel} elements on {device}; "
                            f"got {t.dtype} {tuple(t.shape)} on {t.device}")
 
@@ -363,11 +363,13 @@ def _check(t: torch.Tensor, name: str, dtype: torch.dtype, numel: int, device: t
 def _call(name: str, device: torch.device, *args):
     """One launching entry point on ``device`` (made current for the call if it is not) and its stream."""
     fn = getattr(_lib.lib(), name)
-    if torch.cuda.current_device() == device.index:
-        rc = fn(*args, status_ptr(device), stream_ptr(device))
+    at = device.index
+    stream = torch._C._cuda_getCurrentRawStream(at)  # stream_ptr without a Stream object: 0.1 instead of 2.3 us
+    if torch._C._cuda_getDevice() == at:
+        rc = fn(*args, status_ptr(device), stream)
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, status_ptr(device), stream_ptr(device))
+            rc = fn(*args, status_ptr(device), stream)
     check(rc, name)
 
 
@@ -411,8 +413,8 @@ def block_tables_extend(tables: torch.Tensor, lens: torch.Tensor, new_lens: torc
     if out is None:
         i64 = torch.empty(2 * max_tokens + n, dtype=torch.int64, device=dev)
         i32 = torch.empty(2 * max_tokens + n + 1, dtype=torch.int32, device=dev)
-        positions, slots, last_rows = i64.split((max_tokens, max_tokens, n))
-        table_index, ctx_lens, seq_start = i32.split((max_tokens, max_tokens, n + 1))
+        positions, slots, last_rows = i64.split_with_sizes((max_tokens, max_tokens, n))
+        table_index, ctx_lens, seq_start = i32.split_with_sizes((max_tokens, max_tokens, n + 1))
         out = SlotMap(seq_start, positions, table_index, slots, ctx_lens, last_rows)
     else:
         _check(out.seq_start, "seq_start", torch.int32, n + 1, dev)
@@ -532,7 +534,8 @@ def kv_read_q8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tens
     code, NB, bs = _q8_cache(k_cache, v_cache, k_scale, v_scale, layer, nkv, hd, dev)
     _check(block_ids, "block_ids", torch.int32, 0, dev)
     n = block_ids.numel()
-    k, v = torch.empty(2, n, bs, nkv, hd, dtype=dtype, device=dev).unbind(0)
+    k = torch.empty(n, bs, nkv, hd, dtype=dtype, device=dev)
+    v = torch.empty(n, bs, nkv, hd, dtype=dtype, device=dev)
     _call("b2_kv_read_q8", dev, ptr(k_cache), ptr(v_cache), ptr(k_scale), ptr(v_scale), code, layer, NB, bs, nkv, hd,
           ptr(block_ids), n, ptr(k), ptr(v), dtype_code(dtype))
     return k, v
