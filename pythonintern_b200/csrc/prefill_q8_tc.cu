@@ -2,7 +2,7 @@
 // (tcgen05 + TMEM), head_dim 128.
 //
 // The schedule of prefill_tc.cu (pairs of 128-row Q tiles sharing 64-key K/V tiles, S, P and O in
-// TMEM, one persistent CTA per SM), with converters in the producer's place for K and V: two warps
+// TMEM, one persistent CTA per SM), with converters in the producer's place for K and V: four warps
 // read the codes of a K/V tile a tile ahead into registers (per block and kv head one run of
 // 2 KB), widen them and store them as the swizzled operands of a three-stage ring.  K codes are exact in bf16
 // (q stays as it is) and V codes in f16 (P is rounded to f16, 2^-11), so the only rounding that
@@ -20,12 +20,18 @@ namespace pftc {
 namespace {
 
 constexpr int ST = 3;             // operand ring stages
-constexpr int kConvertWarps = 2;  // 12 warps: three per register file, so 168 registers each
-constexpr int kThreads = 32 * (2 + NG * kGroupWarps + kConvertWarps);  // producer, MMA, softmax, converter warps
+constexpr int kConvertWarps = 4;
+// Warpgroups: control (producer, MMA, two idle warps), two of softmax, converters.  The block is
+// launched with 128 registers a thread and hands them out again: 88 + 2 * 168 + 88 = 4 * 128.
+constexpr int kSoftmaxWarp = 4, kConvertWarp = kSoftmaxWarp + NG * kGroupWarps;
+constexpr int kThreads = 32 * (kConvertWarp + kConvertWarps);
+constexpr int kFewRegs = 88, kManyRegs = 168;
+static_assert(2 * kFewRegs + 2 * kManyRegs <= 4 * 128, "more registers than the block is launched with");
 // Layout (1024-byte aligned): operand ring, Q[NG][2]: 224 KB.
 constexpr uint32_t OFF_Q = ST * STAGE;
+constexpr int kSeqCache = 192;  // sequences whose lengths are kept in shared memory
 constexpr size_t SMEM = OFF_Q + NG * 2 * Q_BYTES + 1024;
-static_assert(SMEM + 512 <= 232448, "shared memory above the 227 KB a CTA may use");
+static_assert(SMEM + 8 * kSeqCache + 512 <= 232448, "shared memory above the 227 KB a CTA may use");
 constexpr float kRoom = 15.f;  // log2 of the largest P
 constexpr float kLift = 8.f;   // log2 of P's largest value when a reference has just moved
 
@@ -43,6 +49,11 @@ struct ParamsQ8 : Params {
 __host__ __device__ constexpr uint32_t instr_desc_f16(int m, int n) {
   return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
+
+template <int N>
+__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 
 // A sequence whose tokens do not fit its table row is left out (every role finds the same).
 __device__ __forceinline__ bool usable(const ParamsQ8& p, const Item& it, int lane) {
@@ -115,7 +126,7 @@ __device__ __forceinline__ void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
 
 template <int REP, int CODE>
 __global__ void __launch_bounds__(kThreads, 1)
-    prefill_q8_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const ParamsQ8 p) {
+    prefill_q8_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const ParamsQ8 params) {
   constexpr int QT = ROWS / REP;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t q_full[NG][2];
@@ -128,11 +139,23 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ __align__(8) uint64_t o_empty[NG];
   __shared__ __align__(8) uint64_t drain_bar;
   __shared__ uint32_t tmem_slot;
+  __shared__ int32_t seq_start[kSeqCache + 1], seq_ctx0[kSeqCache];
 
   pdl_wait();  // the metadata, q and the pool may come from the preceding kernels
   pdl_trigger();
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // every role looks its items up by itself: from shared memory, where the lengths fit
+  ParamsQ8 p = params;
+  if (p.n_seqs <= kSeqCache) {
+    for (int i = threadIdx.x; i <= p.n_seqs; i += kThreads) {
+      seq_start[i] = params.seq_start[i];
+      if (i < p.n_seqs && params.seq_ctx0) seq_ctx0[i] = params.seq_ctx0[i];
+    }
+    __syncthreads();
+    p.seq_start = seq_start;
+    if (params.seq_ctx0) p.seq_ctx0 = seq_ctx0;
+  }
   const int n_items = count_pairs(p, QT, lane) * p.nkv;
   if ((int)blockIdx.x >= n_items) return;  // nothing allocated yet
 
@@ -140,7 +163,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int g = 0; g < NG; ++g) {
       for (int b = 0; b < 2; ++b) {
         mbar_init(&q_full[g][b], 1);
-        mbar_init(&q_empty[g][b], 1);
+        mbar_init(&q_empty[g][b], kGroupWarps);
       }
       for (int b = 0; b < 2; ++b) mbar_init(&s_full[g][b], 1);
       for (int b = 0; b < 2; ++b) {
@@ -165,14 +188,25 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
 
-  if (warp == 0) {
+  // The first usable item after w (w becomes its number; n_items or more: none).
+  auto next_item = [&](int& w) -> Item {
+    Item it{};
+    for (w += gridDim.x; w < n_items; w += gridDim.x) {
+      it = find_item<QT>(p, w, lane);
+      if (usable(p, it, lane)) break;
+    }
+    return it;
+  };
+
+  if (warp < kSoftmaxWarp) {
+   regs_dec<kFewRegs>();
+   if (warp == 0) {
     // ---------------- TMA producer
     const uint64_t pol_q = policy_evict_first();
     int iq[NG] = {0, 0};  // Q loads into each group's buffer
     bool ok = true;
-    for (int w = blockIdx.x; w < n_items && ok; w += gridDim.x) {
-      const Item it = find_item<QT>(p, w, lane);
-      if (!usable(p, it, lane)) continue;
+    int w = (int)blockIdx.x - (int)gridDim.x;
+    for (Item it = next_item(w); w < n_items && ok; it = next_item(w)) {
       if (lane == 0) {
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
@@ -201,10 +235,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     }
     __syncwarp();
-  } else if (warp == 1) {
+   } else if (warp == 1) {
     // ---------------- MMA issuer
-    // The whole warp runs this control code, so that the operand descriptors stay in uniform
-    // registers; one elected lane issues every tcgen05.mma and tcgen05.commit.  The tensor
+    // The whole warp runs this control code; one elected lane issues a batch of tcgen05.mma with
+    // its commit.  (An election for every MMA, as in the bf16 kernel, takes its issue slots from
+    // sixteen warps here: 307 against 269 us at 16 x 1024 tokens.)  The tensor
     // cores queue only about one MMA ahead, so a wait on a barrier that has already completed
     // (a few hundred cycles for the answer) would leave them idle: the barrier of the next
     // step is tested before the current step's MMAs are issued (peek) and only waited for
@@ -236,18 +271,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       ahead();
       const uint32_t p_tmem = tmem + g * GROUP_COLS + COL_S + pb * KT;  // P(jp) in S buffer jp & 1
       const uint32_t v_addr = smem_u32(smem + (size_t)st * STAGE + 2 * HALF);
+      if (elect_one()) {
 #pragma unroll
-      for (int kk = 0; kk < KT / 16; ++kk)  // 16 keys per MMA: +8 TMEM columns of P, +2 KB of V rows
-        if (elect_one())
+        for (int kk = 0; kk < KT / 16; ++kk)  // 16 keys per MMA: +8 TMEM columns of P, +2 KB of V rows
           umma_bf16_ts(tmem + g * GROUP_COLS + COL_O, p_tmem + kk * 8,
                        smem_desc_sw128_mn(v_addr + kk * 2048, HALF, 1024), idesc_pv, (first && kk == 0) ? 0u : 1u);
-      if (elect_one()) umma_commit(&pv_done[g][pb]);
+        umma_commit(&pv_done[g][pb]);
+      }
       ++jp[g];
       return true;
     };
-    for (int w = blockIdx.x; w < n_items && ok; w += gridDim.x) {
-      const Item it = find_item<QT>(p, w, lane);
-      if (!usable(p, it, lane)) continue;
+    int w = (int)blockIdx.x - (int)gridDim.x;
+    Item it = next_item(w);
+    while (w < n_items && ok) {
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         if (it.nt[g] == 0 || !ok) continue;
@@ -273,18 +309,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           const int b = js[g] & 1;
           const uint32_t q_addr = smem_u32(smem + OFF_Q + (g * 2 + qb[g]) * Q_BYTES);
+          if (elect_one()) {
 #pragma unroll
-          for (int half = 0; half < 2; ++half)
+            for (int half = 0; half < 2; ++half)
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              if (elect_one())
+              for (int kk = 0; kk < 4; ++kk)
                 umma_bf16(tmem + g * GROUP_COLS + COL_S + b * KT, smem_desc_sw128(q_addr + half * Q_HALF) + 2 * kk,
                           smem_desc_sw128(k_addr + half * HALF) + 2 * kk, idesc_s, (half | kk) ? 1u : 0u);
-          if (elect_one()) umma_commit(&s_full[g][b]);
-          ++js[g];
-          if (j == it.n_kv[g] - 1) {  // every S MMA of this item has read Q_g
-            if (elect_one()) umma_commit(&q_empty[g][qb[g]]);
+            umma_commit(&s_full[g][b]);
           }
+          ++js[g];
         }
         if (j >= 1) {
           const int pst = (J - 1) % ST;
@@ -297,10 +331,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (elect_one()) umma_commit(&kv_empty[pst]);  // both groups' S and PV of tile j - 1 are issued
         }
       }
-      if (ok && it.n_kv[0] > 0) {  // the item's last tile (J is already the next tile's index)
+      const Item item = it;
+      it = next_item(w);  // looked up while the softmax of the last tile runs
+      if (ok) {  // the item's last tile (J is already the next tile's index)
         const int pst = (J - 1) % ST;
-        const bool two = it.n_kv[1] == it.n_kv[0];
-        const bool first = it.n_kv[0] == 1;
+        const bool two = item.n_kv[1] == item.n_kv[0];
+        const bool first = item.n_kv[0] == 1;
         ok = issue_pv(0, pst, first, [&] {
           if (two) peek_pf(1);
           else peek_kv(J);
@@ -314,61 +350,72 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (elect_one()) umma_commit(&drain_bar);
     mbar_wait(&drain_bar, 0, 100000000ull);
     __syncwarp();
-  } else if (warp < 2 + NG * kGroupWarps) {
+   }
+  } else if (warp < kConvertWarp) {
+    regs_inc<kManyRegs>();
     // ---------------- softmax: one thread per MMA row of its group's Q tile
-    const int sw = warp - 2;                 // 0..7
+    const int sw = warp - kSoftmaxWarp;      // 0..7
     const int grp = sw / kGroupWarps;        // 0: the later Q tile, 1: the one before
     const int quarter = warp & 3;            // TMEM lane quarter this warp may access
     const int m = quarter * 32 + lane;
     const uint32_t trow = tmem + ((uint32_t)(quarter * 32) << 16) + grp * GROUP_COLS;
-    const int tk = m / REP, h = m % REP;
+    const int tk = m / REP;
     int js = 0;  // S tiles consumed by this group (the PV of tile js - 1 is the latest issued)
     bool ok = true;
     Peek pk_s{0u, 0u, false};  // the next S tile, tested while this tile's P is written
-    for (int w = blockIdx.x; w < n_items && ok; w += gridDim.x) {
-      const Item it = find_item<QT>(p, w, lane);
+    int w = (int)blockIdx.x - (int)gridDim.x;
+    Item next = next_item(w);
+    int items = 0;  // this group's Q tiles
+    while (w < n_items && ok) {
+      const Item it = next;
       // this group's tile (selected without indexing, so the item stays in registers)
       const int nt = grp ? it.nt[1] : it.nt[0];
       const int t0 = grp ? it.t0[1] : it.t0[0];
       const int n_kv = grp ? it.n_kv[1] : it.n_kv[0];
-      if (!usable(p, it, lane) || nt == 0) continue;
+      if (nt == 0) {
+        next = next_item(w);
+        continue;
+      }
       const bool row_ok = tk < nt;
       const int pos = it.ctx0 + t0 + tk;  // this row's token position (the last key it attends to)
       // P = 2^(s - m2) vs against the row's reference m2; l = sum 2^(s - m2) = sum of P / vs
       float m2_ref = -INFINITY, l_run = 0.f;
-      // Lane b < 4 prepares block b of a tile, a tile ahead (its id two ahead): the factor of its
-      // raw scores, log2 of the V scale and its reciprocal.  A block outside the pool has kc = -1.
+      // Lane b < 4 sees to block b of a tile: its id is read two tiles ahead, its scales one.  Of
+      // these every row needs the factor kc of its raw scores (-1: a block outside the pool), log2
+      // of the V scale and its reciprocal.
       auto id_of = [&](int j) -> int {
         const int bi = j * (KT / 16) + lane;
         if (lane >= KT / 16 || j >= n_kv || bi >= p.table_stride) return -1;
         const int blk = it.table[bi];
         return blk < p.num_blocks ? blk : -1;
       };
-      float kc_next, lv_next, rv_next;
-      auto prepare = [&](int id) {
-        const float ks = id >= 0 ? __ldg(p.k_scale + (int64_t)id * p.nkv + it.g) : 0.f;
-        float vs = id >= 0 ? __ldg(p.v_scale + (int64_t)id * p.nkv + it.g) : 1.f;
-        if (vs == 0.f) vs = kNoScale;  // a tile of zeros (the converters see to its codes)
-        kc_next = id < 0 ? -1.f : ks == 0.f ? kTiny : ks * p.scale_log2;  // not 0: -inf * 0
-        lv_next = __log2f(vs);
-        rv_next = 1.f / vs;
+      float ks_raw, vs_raw;
+      int id_raw;
+      auto fetch = [&](int id) {
+        id_raw = id;
+        ks_raw = id >= 0 ? __ldg(p.k_scale + (int64_t)id * p.nkv + it.g) : 0.f;
+        vs_raw = id >= 0 ? __ldg(p.v_scale + (int64_t)id * p.nkv + it.g) : 1.f;
       };
       int id_next = id_of(0);
-      prepare(id_next);
+      fetch(id_next);
       id_next = id_of(1);
       for (int j = 0; j < n_kv; ++j, ++js) {
         const int b = js & 1;
         const int k0 = j * KT;
+        // the scales were fetched a tile ago: their latency is behind the last tile's work
+        const float vs = vs_raw == 0.f ? kNoScale : vs_raw;  // a tile of zeros (the converters see to its codes)
+        const float kc_own = id_raw < 0 ? -1.f : ks_raw == 0.f ? kTiny : ks_raw * p.scale_log2;  // not 0: -inf * 0
+        const float lv_own = __log2f(vs), rv_own = __fdividef(1.f, vs);  // each within 2^-21
         float kc[KT / 16], lv[KT / 16], rv[KT / 16];
         bool gap = false;  // a block of the tile is outside the pool
 #pragma unroll
         for (int u = 0; u < KT / 16; ++u) {
-          kc[u] = __shfl_sync(0xffffffffu, kc_next, u);
-          lv[u] = __shfl_sync(0xffffffffu, lv_next, u);
-          rv[u] = __shfl_sync(0xffffffffu, rv_next, u);
+          kc[u] = __shfl_sync(0xffffffffu, kc_own, u);
+          lv[u] = __shfl_sync(0xffffffffu, lv_own, u);
+          rv[u] = __shfl_sync(0xffffffffu, rv_own, u);
           gap |= kc[u] < 0.f;
         }
-        prepare(id_next);
+        fetch(id_next);
         id_next = id_of(j + 2);
         // warp-uniform verdicts: the TMEM loads and stores below are .sync.aligned
         if (!__all_sync(0xffffffffu, wait_peeked(pk_s, &s_full[grp][b], (uint32_t)(js >> 1) & 1u))) {
@@ -468,51 +515,66 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&p_full[grp][b]);
       }
       if (!ok) break;
-      // O / l to global memory once the item's last PV has completed; then O may be reused
+      // O / l to global memory once the item's last PV has completed (the next item is looked up
+      // meanwhile); then O may be reused.  The rows go through this group's Q buffer, which no MMA
+      // reads any more, so that they are written whole: a thread's own row in 16-byte pieces would
+      // touch 32 rows with every store.
+      next = next_item(w);
       if (!__all_sync(0xffffffffu, mbar_wait(&pv_done[grp][(js - 1) & 1], (uint32_t)((js - 1) >> 1) & 1u))) {
         ok = false;
         break;
       }
       tc_fence_after();
       const float inv = l_run == 0.f ? 0.f : 1.f / l_run;  // a NaN stays one
-      __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.out) +
-                           (int64_t)(it.rs + t0 + tk) * p.ld_out + (int64_t)(it.g * REP + h) * HD;
+      const int qb = items++ & 1;
+      uint8_t* stage = smem + OFF_Q + (grp * 2 + qb) * Q_BYTES + quarter * 32 * (HD * 2);
 #pragma unroll 1
       for (int c = 0; c < HD; c += 32) {
         uint32_t o[32];
         tmem_ld32_nowait(trow + COL_O + c, o);
         tmem_wait_ld();
-        if (row_ok) {
 #pragma unroll
-          for (int u = 0; u < 32; u += 8) {
-            uint32_t wv[4];
+        for (int u = 0; u < 32; u += 8) {
+          uint32_t wv[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              __nv_bfloat162 h2 = __floats2bfloat162_rn(__uint_as_float(o[u + 2 * e]) * inv,
-                                                        __uint_as_float(o[u + 2 * e + 1]) * inv);
-              wv[e] = *reinterpret_cast<uint32_t*>(&h2);
-            }
-            *reinterpret_cast<uint4*>(dst + c + u) = make_uint4(wv[0], wv[1], wv[2], wv[3]);
+          for (int e = 0; e < 4; ++e) {
+            __nv_bfloat162 h2 = __floats2bfloat162_rn(__uint_as_float(o[u + 2 * e]) * inv,
+                                                      __uint_as_float(o[u + 2 * e + 1]) * inv);
+            wv[e] = *reinterpret_cast<uint32_t*>(&h2);
           }
+          const int piece = (c + u) / 8;  // of the row's sixteen, spread over the banks
+          *reinterpret_cast<uint4*>(stage + lane * (HD * 2) + (piece ^ (lane & 7)) * 16) =
+              make_uint4(wv[0], wv[1], wv[2], wv[3]);
         }
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&o_empty[grp]);
+      __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(p.out) + (int64_t)(it.rs + t0) * p.ld_out +
+                           (int64_t)it.g * REP * HD + (lane & 15) * 8;
+#pragma unroll 4
+      for (int i = 0; i < 16; ++i) {  // two rows at a time
+        const int r = 2 * i + (lane >> 4), row = quarter * 32 + r;
+        const uint4 v = *reinterpret_cast<const uint4*>(stage + r * (HD * 2) + ((lane & 15) ^ (r & 7)) * 16);
+        if (row / REP < nt) *reinterpret_cast<uint4*>(out + (int64_t)(row / REP) * p.ld_out + (row % REP) * HD) = v;
+      }
+      fence_proxy_async_smem();  // the buffer goes back to TMA
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_empty[grp][qb]);
     }
     if (!ok && lane == 0) raise_status(p.status, B2_DEV_PIPE_TIMEOUT);
   } else {
+    regs_dec<kFewRegs>();
     // ---------------- converters: codes to the operands, K exact in bf16, V exact in f16
     // 16-byte pieces of codes (16 dims of one key).  The eight threads of a store phase write two
     // keys' rows of one 64-dim half, whose swizzled chunks fall into different banks.
-    const int c = threadIdx.x - 32 * (2 + NG * kGroupWarps);
+    const int c = threadIdx.x - 32 * kConvertWarp;
     const int half = (c >> 3) & 1, key0 = (c >> 4) * 2 + ((c >> 2) & 1), ch = c & 3;
     constexpr int PIECES = KT * HD / 16 / (32 * kConvertWarps), KEYS = KT / PIECES;  // keys key0 + KEYS i
     int J = 0;
     bool ok = true;
-    for (int w = blockIdx.x; w < n_items && ok; w += gridDim.x) {
-      const Item it = find_item<QT>(p, w, lane);
-      if (!usable(p, it, lane)) continue;
+    int w = (int)blockIdx.x - (int)gridDim.x;
+    for (Item it = next_item(w); w < n_items && ok; it = next_item(w)) {
       const int last_pos = it.ctx0 + it.t0[0] + it.nt[0] - 1;  // tile 0 is the later one
       // Lane b < 4 holds the id of block b of a tile, read a tile ahead of its codes.  A block
       // outside the pool is reported (where a row attends to its keys) and block 0 read instead.

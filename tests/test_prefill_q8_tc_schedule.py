@@ -19,7 +19,7 @@ NG, ST, GW, CW = 2, 3, 4, 2
 def simulate(work, seed):
     rnd = random.Random(seed)
     q_full = [[Bar(1), Bar(1)] for _ in range(NG)]
-    q_empty = [[Bar(1), Bar(1)] for _ in range(NG)]
+    q_empty = [[Bar(GW), Bar(GW)] for _ in range(NG)]  # handed back by the epilogue, which stages rows there
     kv_full, kv_empty = [Bar(CW) for _ in range(ST)], [Bar(1) for _ in range(ST)]
     s_full = [[Bar(1), Bar(1)] for _ in range(NG)]
     p_full = [[Bar(GW), Bar(GW)] for _ in range(NG)]
@@ -27,6 +27,7 @@ def simulate(work, seed):
     o_empty = [Bar(GW) for _ in range(NG)]
     pending, commits = [], []                    # copies in any order; commits in issue order
     kv_tile = [[None] * CW for _ in range(ST)]   # the tile whose operands a stage holds, per converter warp
+    q_given = [[0] * GW for _ in range(NG)]      # Q tiles handed back, per softmax warp
     kv_done = set()                              # tiles whose PV MMAs have completed
 
     def producer():
@@ -37,6 +38,7 @@ def simulate(work, seed):
                     continue
                 while not q_empty[g][iq[g] & 1].ready(((iq[g] >> 1) & 1) ^ 1):
                     yield
+                assert min(q_given[g]) >= iq[g] - 1, "Q overwritten before the epilogue was done with it"
                 pending.append(q_full[g][iq[g] & 1])
                 iq[g] += 1
 
@@ -86,8 +88,6 @@ def simulate(work, seed):
                     if j < n_kv[g]:
                         commits.append((s_full[g][js[g] & 1], None))
                         js[g] += 1
-                        if j == n_kv[g] - 1:
-                            commits.append((q_empty[g][qb[g]], None))
                 if j >= 1:
                     for g in range(NG):
                         if j - 1 < n_kv[g]:
@@ -100,7 +100,7 @@ def simulate(work, seed):
                     yield from issue_pv(g, n_kv[0] == 1)
             commits.append((kv_empty[(J - 1) % ST], J - 1))
 
-    def softmax(grp):
+    def softmax(grp, wid):
         js = 0
         for tiles in work:
             if tiles[grp][1] == 0:
@@ -113,8 +113,12 @@ def simulate(work, seed):
             while not pv_done[grp][(js - 1) & 1].ready(((js - 1) >> 1) & 1):
                 yield
             o_empty[grp].arrive()
+            if rnd.random() < 0.5:
+                yield
+            q_given[grp][wid] += 1
+            q_empty[grp][(q_given[grp][wid] - 1) & 1].arrive()
 
-    roles = [producer(), mma()] + [converter(w) for w in range(CW)] + [softmax(g) for g in range(NG) for _ in range(GW)]
+    roles = [producer(), mma()] + [converter(w) for w in range(CW)] + [softmax(g, w) for g in range(NG) for w in range(GW)]
     alive = list(range(len(roles)))
     for _ in range(3_000_000):
         if not alive:
