@@ -14,23 +14,29 @@
 //
 // One step.  S^T[16 keys x 8 NT] = K Q^T and O^T[head_dim x 8 NT] += V^T P^T on
 // mma.sync.m16n8k16 with float16 operands and float32 sums.  A code of 8 bits is exact in
-// float16, so nothing is rounded on the way in: codes go from global memory straight into the
-// registers of the A fragments.
+// float16, so nothing is rounded on the way in.
+//  * The tiles of K and V (one block and kv head: 16 * head_dim bytes in one run) come by TMA into
+//    a ring of the warp's own, swizzled, two steps ahead and across the ends of tiles.
 //  * K: lane (r, t) = (lane / 4, lane % 4) reads head_dim / 4 contiguous codes of keys r and
 //    r + 8.  The order of the head_dim axis inside the product is free, so its codes are taken
 //    as the k indexes of that lane and q is laid out to match.
 //  * V: the lane reads head_dim / 8 codes of the keys 2t, 2t+1, 2t+8, 2t+9; a byte shuffle pairs
-//    two keys' codes of one dimension, which is the transposed operand without shared memory.
+//    two keys' codes of one dimension, which is the transposed operand.
 //  * P^T leaves the S^T fragments for the B fragments by an 8x8 transpose in registers.
 //  * q is scaled by a power of two per column, so that its largest magnitude is near 2^14, and
 //    split: one float16 term holds bf16 (values 2^-38 below the largest are cut), two hold
 //    float32 up to 2^-22 of an element.
-// Softmax statistics are float32.  P = 2^(s - m) vs 2^(m - m2) is rounded to float16 (to two
-// terms for float32 queries): the reference m2 follows the largest s + log2(vs), so a scale that
-// differs by orders of magnitude between blocks costs no precision.  The references move only
-// when a value would pass 2^15 and then to 2^8 above the value, so the common step needs no
-// maximum across lanes, only one vote.
+// Softmax statistics are float32: l = sum 2^(s - m), and P = 2^(s - m) vs 2^(m - m2) is rounded to
+// float16 (to two terms for float32 queries).  The second reference m2 follows the largest
+// s + log2(vs), so a scale that differs by orders of magnitude between blocks costs no precision.
+// References move only when a value would pass 2^15 and then to where it is 2^8, so the common
+// step needs no maximum across lanes, only one vote.
 #include "q8.cuh"
+#include "tc_ptx.cuh"
+
+#include <mutex>
+#include <set>
+#include <utility>
 
 namespace b2 {
 
@@ -76,7 +82,7 @@ struct Q8AttnParams {
 
 // ------------------------------------------------------------------ the cut of the work
 constexpr int kWarps = 4;
-constexpr int kGroups = 1024;  // prefix sums kept in shared memory
+constexpr int kGroups = 512;   // prefix sums kept in shared memory
 constexpr int kMinChunk = 4;   // steps a warp takes at least
 
 struct Unit {  // a decode row, or a sequence of a prefill
@@ -313,17 +319,13 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-template <int BYTES>
-__device__ __forceinline__ void ld_codes(const uint8_t* p, uint32_t* w) {
-  if constexpr (BYTES == 16) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
-    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-  } else if constexpr (BYTES == 8) {
-    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
-    w[0] = v.x; w[1] = v.y;
-  } else {
-    w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
-  }
+// The 16 rows of one (block, kv head) into shared memory, swizzled by the map.
+__device__ __forceinline__ void load_tile(void* dst, const CUtensorMap* map, uint64_t* bar, int row, int block) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::
+          "r"(tc::smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(tc::smem_u32(bar)), "r"(0), "r"(row), "r"(block)
+      : "memory");
 }
 
 __device__ __forceinline__ void ld4q(const float* p, float (&v)[4]) {
@@ -336,36 +338,67 @@ __device__ __forceinline__ void ld4q(const __nv_bfloat16* p, float (&v)[4]) {
   v[2] = __uint_as_float(a.y << 16); v[3] = __uint_as_float(a.y & 0xffff0000u);
 }
 
+constexpr int kStages = 3;          // tiles of K and V a warp holds or has in flight
+constexpr float kRoom = 15.f;       // log2 of the largest P
+constexpr float kLift = 8.f;        // log2 of the largest P when a reference has just moved
+constexpr float kNoRef = -1e30f;    // reference of a column that has seen no key
+
 template <typename T, int HD, int CODE, int NT>
 struct AttnCfg {
   static constexpr int N = 8 * NT;                       // columns of a tile
   static constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;   // float16 terms of q and P
   static constexpr int KW = HD / 16;                     // words of codes a lane holds of a key; MMAs of S
   static constexpr int VW = HD / 32;                     // and of a key's values
-  static constexpr int KB = KW >= 4 ? 16 : 4 * KW;       // bytes of one K load
-  static constexpr int SMEM_Q = kWarps * KW * NT * TERMS * 32 * 8;
+  static constexpr int TILE = kQ8Block * HD;             // bytes of codes of one block and head
+  static constexpr int Q_BYTES = KW * NT * TERMS * 32 * 8;
+  static constexpr int WARP_BYTES = kStages * 2 * TILE;  // the warp's ring of K and V tiles
+  // ring (1024-byte aligned for the swizzle), then the q fragments
+  static constexpr int SMEM = 1024 + kWarps * (WARP_BYTES + Q_BYTES);
 };
 
-// CTAs per SM the registers are limited for.
-template <int NT, int TERMS>
-constexpr int kCtas = NT * TERMS == 1 ? 4 : NT * TERMS == 2 ? 3 : 2;
+// Byte offset of 16-byte chunk `chunk` of key row `row` in a tile that TMA has stored with the
+// swizzle as wide as a row (128, 64 or 32 bytes).
+template <int HD>
+__device__ __forceinline__ int tile_at(int row, int chunk) {
+  constexpr int CHUNKS = HD / 16;
+  return row * HD + ((chunk ^ (row * HD / 128 & (CHUNKS - 1))) << 4);
+}
+
+// CTAs per SM that the registers are limited for and the shared memory holds.
+constexpr int ctas_per_sm(int nt, int terms) { return nt * terms <= 2 ? 3 : 2; }
+
+// Up to 32 consecutive steps of one (tile, kv head); lane i holds what step i needs.
+struct Window {
+  Place at;       // of the first step
+  int cnt;        // steps; 0: behind the warp's chunk
+  int id;         // block id, -1 outside the pool
+  float ks, vs;   // scales
+};
 
 template <typename T, int HD, int CODE, int NT>
-__global__ void __launch_bounds__(kWarps * 32, kCtas<NT, (sizeof(T) == 4 ? 2 : 1)>)
-q8_attn_kernel(Q8AttnParams p, int qt, int n_units, int per_group) {
+__global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(NT, sizeof(T) == 4 ? 2 : 1))
+q8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const Q8AttnParams p,
+               int qt, int n_units, int per_group) {
   pdl_wait();
   pdl_trigger();
   using C = AttnCfg<T, HD, CODE, NT>;
   constexpr int KW = C::KW, VW = C::VW, TERMS = C::TERMS, N = C::N;
   __shared__ int64_t sm_steps[kGroups];
   __shared__ int sm_tiles[kGroups];
-  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ __align__(8) uint64_t full[kWarps][kStages];
+  extern __shared__ uint8_t smem_raw[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int r8 = lane >> 2, t4 = lane & 3;
   const int warps = gridDim.x * kWarps, w = blockIdx.x * kWarps + warp;
   const int rep = p.nq / p.nkv;
-  uint2* sq = reinterpret_cast<uint2*>(smem) + warp * (KW * NT * TERMS * 32);
+  uint8_t* smem = smem_raw + ((1024 - (tc::smem_u32(smem_raw) & 1023)) & 1023);
+  uint8_t* ring = smem + warp * C::WARP_BYTES;
+  uint2* sq = reinterpret_cast<uint2*>(smem + kWarps * C::WARP_BYTES + warp * C::Q_BYTES);
 
+  if (lane == 0) {
+    for (int i = 0; i < kStages; ++i) tc::mbar_init(&full[warp][i], 1);
+    tc::fence_mbar_init();
+  }
   const Cut cut = make_cut(p, qt, n_units, per_group, sm_steps, sm_tiles, warps, blockIdx.x == 0);
   // a seq_start that goes back may name more tokens than there are rows (and tiles than the
   // workspace has room for): nothing is computed
@@ -382,143 +415,177 @@ q8_attn_kernel(Q8AttnParams p, int qt, int n_units, int per_group) {
       for (int i = threadIdx.x; i < p.nq * HD; i += kWarps * 32) dst[i] = from_f32<T>(0.f);
     }
   }
-  int64_t x = w * cut.chunk;
-  const int64_t x_end = min(cut.total, x + cut.chunk);
-  if (x >= x_end) return;
-  Place at = find_step(p, x, qt, n_units, per_group, sm_steps, sm_tiles);
-  constexpr int key_stride = HD;  // bytes between keys of a tile
+  const int64_t x_begin = w * cut.chunk, x_end = min(cut.total, x_begin + cut.chunk);
+  if (x_begin >= x_end) return;
 
-  for (bool first = true; x < x_end; first = false) {
-    const int i0 = at.block;
-    const int i1 = (int)min((int64_t)at.blocks, i0 + (x_end - x));
+  int64_t left = x_end - x_begin;  // steps behind the windows taken so far
+  auto ids_of = [&](Window& win) {  // sets cnt from the place, starts the loads of the ids
+    win.cnt = (int)min((int64_t)min(32, win.at.blocks - win.at.block), left);
+    left -= win.cnt;
+    int id = -1;
+    if (lane < win.cnt) id = __ldg(p.tables + (int64_t)table_row(p, win.at.u) * p.table_stride + win.at.block + lane);
+    win.id = id;
+  };
+  auto scales_of = [&](Window& win) {
+    const bool in_pool = win.id >= 0 && win.id < p.num_blocks;
+    if (lane < win.cnt && !in_pool) raise_status(p.status, B2_DEV_RANGE);
+    if (!in_pool) win.id = -1;
+    const int64_t at = in_pool ? q8_scale(win.id, p.nkv, win.at.g) : 0;
+    win.ks = __ldg(p.k_scale + at);
+    win.vs = __ldg(p.v_scale + at);
+  };
+  // The window behind `win` in the warp's chunk.
+  auto window_after = [&](const Window& win) -> Window {
+    Window nx;
+    nx.at = win.at;
+    nx.cnt = 0;
+    nx.id = -1;
+    if (left == 0) return nx;
+    nx.at.block += win.cnt;
+    if (nx.at.block == nx.at.blocks) next_pair(p, nx.at, qt);
+    ids_of(nx);
+    return nx;
+  };
+
+  int n_used = 0, n_open = 0;  // steps consumed; tiles in the ring or on their way
+  auto issue = [&](const Window& win, int i) {
+    const int slot = (n_used + n_open) % kStages;
+    const int id = __shfl_sync(0xffffffffu, win.id, i);
+    ++n_open;
+    if (lane == 0) {
+      uint64_t* bar = &full[warp][slot];
+      if (id >= 0 && id < p.num_blocks) {
+        uint8_t* dst = ring + slot * 2 * C::TILE;
+        tc::mbar_arrive_expect_tx(bar, 2 * C::TILE);
+        load_tile(dst, &tmK, bar, win.at.g * kQ8Block, id);
+        load_tile(dst + C::TILE, &tmV, bar, win.at.g * kQ8Block, id);
+      } else {
+        tc::mbar_arrive(bar);  // nothing to wait for: the step is left out
+      }
+    }
+  };
+
+  Window cur, nxt;
+  cur.at = find_step(p, x_begin, qt, n_units, per_group, sm_steps, sm_tiles);
+  ids_of(cur);
+  nxt = window_after(cur);
+  int sent = 0, sent_nxt = 0;  // steps of either window whose tiles were asked for
+  auto top_up = [&]() {
+    while (n_open < kStages) {
+      if (sent < cur.cnt) issue(cur, sent++);
+      else if (sent_nxt < nxt.cnt) issue(nxt, sent_nxt++);
+      else break;
+    }
+  };
+  top_up();
+  scales_of(cur);
+
+  float colscale[NT][2];
+  int lim[NT][2];  // last key of the lane's columns
+  float o[2 * VW][NT][4];
+  float m[NT][2], m2[NT][2], lift[NT][2], l[NT][2];  // references, 2^(m - m2), sums
+  int i0 = 0;          // first block of the current (tile, kv head) that this warp sees
+  bool start = true;   // a (tile, kv head) begins with this window
+  bool first = true, ok = true;
+
+  while (cur.cnt > 0) {
+    const Place& at = cur.at;
     const int tok0 = at.j * qt, ntok = min(qt, at.unit.len - tok0);
     const int ncol = ntok * rep;
-    const int pos0 = at.unit.ctx0 + tok0;           // position of the tile's first token
+    const int pos0 = at.unit.ctx0 + tok0;  // position of the tile's first token
     const int pos_last = pos0 + ntok - 1;
-    const int32_t* table = p.tables + (int64_t)table_row(p, at.u) * p.table_stride;
-    const uint8_t* kc = p.k_cache + (int64_t)at.g * (kQ8Block * HD);
-    const uint8_t* vc = p.v_cache + (int64_t)at.g * (kQ8Block * HD);
-    const int64_t blk_bytes = (int64_t)p.nkv * (kQ8Block * HD);
-
-    // q of the tile's columns into this warp's shared memory, as B fragments.
-    float colscale[NT][2];
-    int lim[NT][2];  // last key of the lane's columns
-    __syncwarp();
+    if (start) {
+      start = false;
+      // A (tile, kv head) begins: q of its columns into the warp's shared memory as B fragments.
+      i0 = at.block;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int col = nt * 8 + r8;
-      float q[KW][4];
-      float big = 0.f;
-      const bool live = col < ncol;
-      const T* src = reinterpret_cast<const T*>(p.q) + (int64_t)(at.unit.start + tok0 + (live ? col / rep : 0)) * p.ld_q +
-                     (int64_t)(at.g * rep + (live ? col % rep : 0)) * HD;
+      for (int nt = 0; nt < NT; ++nt) {
+        const int col = nt * 8 + r8;
+        float q[KW][4];
+        float big = 0.f;
+        const bool live = col < ncol;
+        const T* src = reinterpret_cast<const T*>(p.q) +
+                       (int64_t)(at.unit.start + tok0 + (live ? col / rep : 0)) * p.ld_q +
+                       (int64_t)(at.g * rep + (live ? col % rep : 0)) * HD + t4 * (HD / 4);
 #pragma unroll
-      for (int k = 0; k < KW; ++k) {
-        const int d = KW >= 4 ? (k / 4) * 64 + t4 * 16 + (k % 4) * 4 : t4 * (KW * 4) + k * 4;
-        ld4q(src + d, q[k]);
+        for (int k = 0; k < KW; ++k) {
+          ld4q(src + k * 4, q[k]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (!live) q[k][e] = 0.f;
-          big = fmaxf(big, fabsf(q[k][e]));
-        }
-      }
-      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-      // a power of two that brings `big` to [2^14, 2^15); in two factors, so that neither overflows
-      const int ex = big > 0.f && big <= 3.402823466e38f ? 14 - ilogbf(big) : 0;
-      const float up = ldexpf(1.f, ex / 2), up2 = ldexpf(1.f, ex - ex / 2);
-#pragma unroll
-      for (int k = 0; k < KW; ++k) {
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = q[k][e] * up * up2;
-#pragma unroll
-        for (int term = 0; term < TERMS; ++term) {
-          uint2 f;
-          f.x = pack_f16(v[0], v[1]);
-          f.y = pack_f16(v[2], v[3]);
-          sq[((k * NT + nt) * TERMS + term) * 32 + lane] = f;
-          if (TERMS == 2) {
-            const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&f.x));
-            const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&f.y));
-            v[0] -= a.x; v[1] -= a.y; v[2] -= b.x; v[3] -= b.y;
+          for (int e = 0; e < 4; ++e) {
+            if (!live) q[k][e] = 0.f;
+            big = fmaxf(big, fabsf(q[k][e]));
           }
         }
-      }
-      const float back = live ? ldexpf(p.scale_log2, -ex) : 0.f;
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+        // a power of two that brings `big` to [2^14, 2^15); in two factors, so that neither overflows
+        const int ex = big > 0.f && big <= 3.402823466e38f ? 14 - ilogbf(big) : 0;
+        const float up = ldexpf(1.f, ex / 2), up2 = ldexpf(1.f, ex - ex / 2);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int c = nt * 8 + 2 * t4 + e;
-        colscale[nt][e] = __shfl_sync(0xffffffffu, back, (2 * t4 + e) * 4);
-        lim[nt][e] = c < ncol ? pos0 + c / rep : -1;
+        for (int k = 0; k < KW; ++k) {
+          float v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = q[k][e] * up * up2;
+#pragma unroll
+          for (int term = 0; term < TERMS; ++term) {
+            uint2 f;
+            f.x = pack_f16(v[0], v[1]);
+            f.y = pack_f16(v[2], v[3]);
+            sq[((k * NT + nt) * TERMS + term) * 32 + lane] = f;
+            if (TERMS == 2) {
+              const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&f.x));
+              const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&f.y));
+              v[0] -= a.x; v[1] -= a.y; v[2] -= b.x; v[3] -= b.y;
+            }
+          }
+        }
+        const float back = live ? ldexpf(p.scale_log2, -ex) : 0.f;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int c = nt * 8 + 2 * t4 + e;
+          colscale[nt][e] = __shfl_sync(0xffffffffu, back, (2 * t4 + e) * 4);
+          lim[nt][e] = c < ncol ? pos0 + c / rep : -1;
+          m[nt][e] = m2[nt][e] = kNoRef;
+          lift[nt][e] = l[nt][e] = 0.f;
+        }
+#pragma unroll
+        for (int d = 0; d < 2 * VW; ++d) o[d][nt][0] = o[d][nt][1] = o[d][nt][2] = o[d][nt][3] = 0.f;
       }
     }
-    __syncwarp();
 
-    float o[2 * VW][NT][4];
-    float m[NT][2], m2[NT][2], l[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-      for (int d = 0; d < 2 * VW; ++d) o[d][nt][0] = o[d][nt][1] = o[d][nt][2] = o[d][nt][3] = 0.f;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        m[nt][e] = m2[nt][e] = -INFINITY;
-        l[nt][e] = 0.f;
+    for (int i = 0; i < cur.cnt; ++i) {
+      top_up();
+      if (i == 0) scales_of(nxt);  // its ids were asked for a window ago
+      const int blk = __shfl_sync(0xffffffffu, cur.id, i);
+      const float ks = __shfl_sync(0xffffffffu, cur.ks, i), vs = __shfl_sync(0xffffffffu, cur.vs, i);
+      const int slot = n_used % kStages;
+      if (!__all_sync(0xffffffffu, tc::mbar_wait(&full[warp][slot], (uint32_t)(n_used / kStages) & 1u))) {
+        ok = false;
+        break;
       }
-    }
-
-    // Block ids and scales, 32 steps at a time, one per lane.
-    int win = i0, ids = 0;
-    float kss = 0.f, vss = 0.f;
-    auto window = [&](int i) {
-      win = i;
-      int id = -1;
-      if (i + lane < i1) {
-        id = __ldg(table + i + lane);
-        if (id < 0 || id >= p.num_blocks) {
-          raise_status(p.status, B2_DEV_RANGE);
-          id = -1;
-        }
-      }
-      ids = id;
-      kss = id >= 0 ? __ldg(p.k_scale + q8_scale(id, p.nkv, at.g)) : 0.f;
-      vss = id >= 0 ? __ldg(p.v_scale + q8_scale(id, p.nkv, at.g)) : 0.f;
-    };
-    uint32_t kw[2][KW], vw[4][VW];
-    auto load_k = [&](int blk) {
-      const uint8_t* src = kc + (int64_t)max(blk, 0) * blk_bytes + r8 * key_stride + t4 * C::KB;
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int k = 0; k < KW; k += C::KB / 4) ld_codes<C::KB>(src + h * 8 * key_stride + (k / 4) * 64, &kw[h][k]);
-    };
-    auto load_v = [&](int blk) {
-      const uint8_t* src = vc + (int64_t)max(blk, 0) * blk_bytes + 2 * t4 * key_stride + r8 * (4 * VW);
-#pragma unroll
-      for (int h = 0; h < 4; ++h) ld_codes<4 * VW>(src + ((h & 1) + (h >> 1) * 8) * key_stride, vw[h]);
-    };
-    window(i0);
-    int blk = __shfl_sync(0xffffffffu, ids, 0);
-    load_k(blk);
-    load_v(blk);
-
-    for (int i = i0; i < i1; ++i) {
-      const float ks = __shfl_sync(0xffffffffu, kss, i - win), vs = __shfl_sync(0xffffffffu, vss, i - win);
-      if (i + 1 < i1 && i + 1 - win == 32) window(i + 1);
-      const int nblk = __shfl_sync(0xffffffffu, ids, (i + 1 - win) & 31);
-      const bool more = i + 1 < i1;
-      if (blk < 0) {  // a block outside the pool: its keys are left out
-        if (more) {
-          load_k(nblk);
-          load_v(nblk);
-        }
-        blk = nblk;
-        continue;
-      }
+      ++n_used;
+      --n_open;
+      if (blk < 0) continue;  // a block outside the pool: its keys are left out
+      const uint8_t* kt = ring + slot * 2 * C::TILE;
+      const uint8_t* vt = kt + C::TILE;
       float s[NT][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+      uint32_t kw[2][KW];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int row = r8 + 8 * h;
+        if constexpr (KW == 2) {
+          const uint2 v = *reinterpret_cast<const uint2*>(kt + tile_at<HD>(row, t4 >> 1) + (t4 & 1) * 8);
+          kw[h][0] = v.x; kw[h][1] = v.y;
+        } else {
+#pragma unroll
+          for (int k = 0; k < KW; k += 4) {
+            const uint4 v = *reinterpret_cast<const uint4*>(kt + tile_at<HD>(row, t4 * (KW / 4) + k / 4));
+            kw[h][k] = v.x; kw[h][k + 1] = v.y; kw[h][k + 2] = v.z; kw[h][k + 3] = v.w;
+          }
+        }
+      }
 #pragma unroll
       for (int k = 0; k < KW; ++k) {
         uint32_t a[4];
@@ -532,29 +599,46 @@ q8_attn_kernel(Q8AttnParams p, int qt, int n_units, int per_group) {
             mma_f16(s[nt], a, b.x, b.y);
           }
       }
-      if (more) load_k(nblk);
+      uint32_t vw[4][VW];
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        const int row = 2 * t4 + (h & 1) + (h >> 1) * 8;
+        if constexpr (VW == 4) {
+          const uint4 v = *reinterpret_cast<const uint4*>(vt + tile_at<HD>(row, r8));
+          vw[h][0] = v.x; vw[h][1] = v.y; vw[h][2] = v.z; vw[h][3] = v.w;
+        } else if constexpr (VW == 2) {
+          const uint2 v = *reinterpret_cast<const uint2*>(vt + tile_at<HD>(row, r8 >> 1) + (r8 & 1) * 8);
+          vw[h][0] = v.x; vw[h][1] = v.y;
+        } else {
+          vw[h][0] = *reinterpret_cast<const uint32_t*>(vt + tile_at<HD>(row, r8 >> 2) + (r8 & 3) * 4);
+        }
+      }
 
       // scores; the tail of the tile's keys is masked per column
-      const int key = i * kQ8Block + r8;
-      const bool tail = (i + 1) * kQ8Block - 1 > pos0;
-      const float lv = vs > 0.f ? __log2f(vs) : vs == 0.f ? -INFINITY : vs;
+      const int key0 = (at.block + i) * kQ8Block, key = key0 + r8;
+      const bool tail = key0 + kQ8Block - 1 > pos0;
+      if (tail) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            if (key > lim[nt][e]) s[nt][e] = -INFINITY;
+            if (key + 8 > lim[nt][e]) s[nt][2 + e] = -INFINITY;
+          }
+      }
+      const float lv = vs == 0.f ? -INFINITY : __log2f(vs);  // only places a reference: approximate
       bool move = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float cs = colscale[nt][e] * ks;
-          float a = s[nt][e] * cs, b = s[nt][2 + e] * cs;
-          if (tail) {
-            if (key > lim[nt][e]) a = -INFINITY;
-            if (key + 8 > lim[nt][e]) b = -INFINITY;
-          }
-          s[nt][e] = a;
-          s[nt][2 + e] = b;
-          const float top = fminf(m[nt][e], m2[nt][e] - lv) + 15.f;
-          move |= a > top || b > top;
+          // a column that sees none of the block's keys takes nothing from its scales
+          const float cs = tail && key0 > lim[nt][e] ? 1.f : colscale[nt][e] * ks;
+          s[nt][e] *= cs;
+          s[nt][2 + e] *= cs;
+          move |= fmaxf(s[nt][e], s[nt][2 + e]) > fminf(m[nt][e], m2[nt][e] - lv) + kRoom;
         }
-      if (__any_sync(0xffffffffu, move)) {
+      if (__any_sync(0xffffffffu, move)) {  // references move, to 2^8 below their columns' largest
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -562,11 +646,12 @@ q8_attn_kernel(Q8AttnParams p, int qt, int n_units, int per_group) {
             float mx = fmaxf(s[nt][e], s[nt][2 + e]);
 #pragma unroll
             for (int sh = 4; sh < 32; sh <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, sh));
-            const float mn = fmaxf(m[nt][e], mx - 8.f), m2n = fmaxf(m2[nt][e], mx - 8.f + lv);
-            l[nt][e] *= mn == -INFINITY ? 1.f : exp2f(m[nt][e] - mn);
-            const float c = m2n == -INFINITY ? 1.f : exp2f(m2[nt][e] - m2n);
+            const float mn = fmaxf(m[nt][e], mx - kLift), m2n = fmaxf(m2[nt][e], mx - kLift + lv);
+            l[nt][e] *= ex2(m[nt][e] - mn);
+            const float c = ex2(m2[nt][e] - m2n);
             m[nt][e] = mn;
             m2[nt][e] = m2n;
+            lift[nt][e] = m2n == kNoRef ? 0.f : ex2(mn - m2n);
 #pragma unroll
             for (int d = 0; d < 2 * VW; ++d) {
               o[d][nt][e] *= c;
@@ -580,15 +665,12 @@ q8_attn_kernel(Q8AttnParams p, int qt, int n_units, int per_group) {
         float pa[2], pc[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float f = vs == 0.f ? 0.f : vs * ex2(m[nt][e] - m2[nt][e]);
-          float a = ex2(s[nt][e] - m[nt][e]), b = ex2(s[nt][2 + e] - m[nt][e]);
-          pa[e] = a * f;
-          pc[e] = b * f;
-          if (tail) {
-            if (key > lim[nt][e]) a = pa[e] = 0.f;
-            if (key + 8 > lim[nt][e]) b = pc[e] = 0.f;
-          }
-          l[nt][e] += a + b;
+          pa[e] = ex2(s[nt][e] - m[nt][e]);  // -inf gives 0
+          pc[e] = ex2(s[nt][2 + e] - m[nt][e]);
+          l[nt][e] += pa[e] + pc[e];
+          const float f = tail && key0 > lim[nt][e] ? 0.f : vs == 0.f ? 0.f : vs * lift[nt][e];
+          pa[e] *= f;
+          pc[e] *= f;
         }
 #pragma unroll
         for (int term = 0; term < TERMS; ++term) {
@@ -602,8 +684,9 @@ q8_attn_kernel(Q8AttnParams p, int qt, int n_units, int per_group) {
           }
         }
       }
-      if (tail && (i + 1) * kQ8Block - 1 > pos_last) {  // keys no column sees: whatever their codes
-        const int k0 = i * kQ8Block + 2 * t4;
+      // V of keys no column sees counts as 0, whatever its codes (an e4m3 NaN among them)
+      if (key0 + kQ8Block - 1 > pos_last) {
+        const int k0 = key0 + 2 * t4;
 #pragma unroll
         for (int h = 0; h < 4; ++h)
           if (k0 + (h & 1) + (h >> 1) * 8 > pos_last) {
@@ -626,71 +709,81 @@ q8_attn_kernel(Q8AttnParams p, int qt, int n_units, int per_group) {
               mma_f16(o[2 * v + half][nt], a, pb[nt][term][0], pb[nt][term][1]);
         }
       }
-      if (more) load_v(nblk);
-      blk = nblk;
+      __syncwarp();  // every lane has read the tile: its slot may be asked for again
     }
+    if (!ok) break;
 
-    // The lane holds, of columns 2 t4 and 2 t4 + 1 of every n-tile, dims r8 * HD/8 .. + HD/8 - 1.
-    const bool whole = i0 == 0 && i1 == at.blocks;
-    const int64_t slot = 2 * (int64_t)w + (first ? 0 : 1);
-    if (!whole && i0 == 0 && lane == 0) {
-      const int64_t last = (at.begin + at.blocks - 1) / cut.chunk;
-      p.ws_pairs[(int64_t)at.tile * p.nkv + at.g] = make_int4(w, (int)last, at.u, at.j | (first ? 0x40000000 : 0));
-    } else if (whole && lane == 0) {
-      p.ws_pairs[(int64_t)at.tile * p.nkv + at.g] = make_int4(0, -1, 0, 0);  // nothing to join
-    }
-    int npad = 0;
-    if (p.compat_pad) npad = max(0, cut.max_ctx - (pos0 + 1));
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float lt = l[nt][e];
-#pragma unroll
-        for (int sh = 4; sh < 32; sh <<= 1) lt += __shfl_xor_sync(0xffffffffu, lt, sh);
-        const int c = nt * 8 + 2 * t4 + e;
-        if (c >= ncol) continue;
-        float f = 1.f;
-        if (whole) {
-          float mm = m[nt][e];
-          if (npad > 0) {
-            const float mp = fmaxf(mm, 0.f);
-            lt = (mm == -INFINITY ? 0.f : lt * exp2f(mm - mp)) + (float)npad * exp2f(-mp);
-            mm = mp;
-          }
-          f = m2[nt][e] == -INFINITY ? (lt == lt ? 0.f : lt) : exp2f(m2[nt][e] - mm) / lt;
-        }
-        float v[4 * VW];
-#pragma unroll
-        for (int d = 0; d < 2 * VW; ++d) {
-          v[2 * d] = o[d][nt][e] * f;
-          v[2 * d + 1] = o[d][nt][2 + e] * f;
-        }
-        if (whole) {
-          T* dst = reinterpret_cast<T*>(p.out) + (int64_t)(at.unit.start + tok0 + c / rep) * p.ld_out +
-                   (int64_t)(at.g * rep + c % rep) * HD + r8 * (4 * VW);
-          if constexpr (sizeof(T) == 4) {
-#pragma unroll
-            for (int d = 0; d < VW; ++d)
-              reinterpret_cast<float4*>(dst)[d] = make_float4(v[4 * d], v[4 * d + 1], v[4 * d + 2], v[4 * d + 3]);
-          } else {
-#pragma unroll
-            for (int d = 0; d < VW; ++d) {
-              const __nv_bfloat162 a = __floats2bfloat162_rn(v[4 * d], v[4 * d + 1]);
-              const __nv_bfloat162 b = __floats2bfloat162_rn(v[4 * d + 2], v[4 * d + 3]);
-              reinterpret_cast<uint2*>(dst)[d] =
-                  make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-            }
-          }
-        } else {
-          float4* dst = reinterpret_cast<float4*>(p.ws_o + (slot * N + c) * HD + r8 * (4 * VW));
-#pragma unroll
-          for (int d = 0; d < VW; ++d) dst[d] = make_float4(v[4 * d], v[4 * d + 1], v[4 * d + 2], v[4 * d + 3]);
-          if (r8 == 0) p.ws_stat[slot * N + c] = make_float4(m[nt][e], lt, m2[nt][e], 0.f);
-        }
+    const bool done = at.block + cur.cnt == at.blocks;
+    if (done || nxt.cnt == 0) {
+      // The lane holds, of columns 2 t4 and 2 t4 + 1 of every n-tile, dims r8 * HD/8 .. + HD/8 - 1.
+      const bool whole = i0 == 0 && done;
+      const int64_t slot = 2 * (int64_t)w + (first ? 0 : 1);
+      if (i0 == 0 && lane == 0) {
+        const int64_t last = (at.begin + at.blocks - 1) / cut.chunk;
+        p.ws_pairs[(int64_t)at.tile * p.nkv + at.g] =
+            whole ? make_int4(0, -1, 0, 0)  // nothing to join
+                  : make_int4(w, (int)last, at.u, at.j | (first ? 0x40000000 : 0));
       }
-    x += i1 - i0;
-    if (x < x_end) next_pair(p, at, qt);
+      const int npad = p.compat_pad ? max(0, cut.max_ctx - (pos0 + 1)) : 0;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float lt = l[nt][e];
+#pragma unroll
+          for (int sh = 4; sh < 32; sh <<= 1) lt += __shfl_xor_sync(0xffffffffu, lt, sh);
+          const int c = nt * 8 + 2 * t4 + e;
+          if (c >= ncol) continue;
+          float f = 1.f;
+          if (whole) {
+            if (npad > 0) lt += (float)npad * exp2f(-m[nt][e]);  // keys of score 0 and value 0
+            f = m2[nt][e] == kNoRef ? (lt == lt ? 0.f : lt) : exp2f(m2[nt][e] - m[nt][e]) / lt;
+          }
+          float v[4 * VW];
+#pragma unroll
+          for (int d = 0; d < 2 * VW; ++d) {
+            v[2 * d] = o[d][nt][e] * f;
+            v[2 * d + 1] = o[d][nt][2 + e] * f;
+          }
+          if (whole) {
+            T* dst = reinterpret_cast<T*>(p.out) + (int64_t)(at.unit.start + tok0 + c / rep) * p.ld_out +
+                     (int64_t)(at.g * rep + c % rep) * HD + r8 * (4 * VW);
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+              for (int d = 0; d < VW; ++d)
+                reinterpret_cast<float4*>(dst)[d] = make_float4(v[4 * d], v[4 * d + 1], v[4 * d + 2], v[4 * d + 3]);
+            } else {
+#pragma unroll
+              for (int d = 0; d < VW; ++d) {
+                const __nv_bfloat162 a = __floats2bfloat162_rn(v[4 * d], v[4 * d + 1]);
+                const __nv_bfloat162 b = __floats2bfloat162_rn(v[4 * d + 2], v[4 * d + 3]);
+                reinterpret_cast<uint2*>(dst)[d] =
+                    make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+              }
+            }
+          } else {
+            float4* dst = reinterpret_cast<float4*>(p.ws_o + (slot * N + c) * HD + r8 * (4 * VW));
+#pragma unroll
+            for (int d = 0; d < VW; ++d) dst[d] = make_float4(v[4 * d], v[4 * d + 1], v[4 * d + 2], v[4 * d + 3]);
+            if (r8 == 0) p.ws_stat[slot * N + c] = make_float4(m[nt][e], lt, m2[nt][e], 0.f);
+          }
+        }
+      first = false;
+      start = true;
+    }
+    cur = nxt;
+    sent = sent_nxt;
+    sent_nxt = 0;
+    nxt = window_after(cur);
+  }
+  if (!ok) {
+    // Copies still in flight (only after a wait ran out) land before the CTA exits.
+    if (lane == 0) {
+      raise_status(p.status, B2_DEV_PIPE_TIMEOUT);
+      for (int i = 0; i < n_open; ++i)
+        tc::mbar_wait(&full[warp][(n_used + i) % kStages], (uint32_t)((n_used + i) / kStages) & 1u, 100000000ull);
+    }
+    __syncwarp();
   }
 }
 
@@ -728,7 +821,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) q8_join_kernel(Q8AttnParams p
   while (share * 2 * ncol <= kJoinWarps) share *= 2;
   for (int c0 = 0; c0 < ncol; c0 += kJoinWarps / share) {
     const int c = c0 + warp / share, part_of = warp % share;
-    float M = npad > 0 ? 0.f : -INFINITY, l = 0.f, acc[E];
+    float M = kNoRef, l = 0.f, acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
     auto where = [&](int k) { return (k == 0 ? slot0 : 2 * (int64_t)(pair.x + k)) * columns + c; };
@@ -739,9 +832,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) q8_join_kernel(Q8AttnParams p
         float f = 0.f;
         if (k0 + lane < n) {
           const float4 st = p.ws_stat[where(k0 + lane)];
-          if (st.x != -INFINITY) l += st.y * exp2f(st.x - M);
-          else if (st.y != st.y) l = st.y;
-          if (st.z != -INFINITY) f = exp2f(st.z - M);
+          l = fmaf(st.y, exp2f(st.x - M), l);
+          f = exp2f(st.z - M);
         }
         const int most_k = min(32, n - k0);
 #pragma unroll 4
@@ -823,8 +915,7 @@ AttnPlan plan_of(int n_rows, int nq, int nkv, int hd, int n_seqs, bool prefill, 
   a.qt = prefill ? 8 * a.nt / rep : 1;
   a.units = prefill ? n_seqs : n_rows;
   a.per_group = (a.units + kGroups - 1) / kGroups;
-  const int w = a.nt * terms;
-  a.ctas = sm_count() * (w == 1 ? 4 : w == 2 ? 3 : 2);
+  a.ctas = sm_count() * ctas_per_sm(a.nt, terms);
   a.slots = 2 * a.ctas * kWarps;
   a.tiles = prefill ? (int64_t)n_rows / a.qt + n_seqs : n_rows;
   a.pairs = 256;
@@ -834,11 +925,47 @@ AttnPlan plan_of(int n_rows, int nq, int nkv, int hd, int n_seqs, bool prefill, 
   return a;
 }
 
+// One layer's cache as [blocks][kv heads * 16 tokens][head_dim] bytes, in boxes of one (block, kv
+// head), swizzled as wide as a row.
+int encode_cache(CUtensorMap* m, const void* cache, int num_blocks, int nkv, int hd) {
+  auto fn = tc::encode_fn();
+  if (!fn) return fail(B2_ECUDA, "cuTensorMapEncodeTiled unavailable");
+  const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)nkv * kQ8Block, (cuuint64_t)num_blocks};
+  const cuuint64_t strides[2] = {(cuuint64_t)hd, (cuuint64_t)nkv * kQ8Block * hd};
+  const cuuint32_t box[3] = {(cuuint32_t)hd, kQ8Block, 1}, es[3] = {1, 1, 1};
+  const CUtensorMapSwizzle swizzle = hd == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                                     : hd == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                : CU_TENSOR_MAP_SWIZZLE_32B;
+  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(cache), dims, strides, box, es,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(B2_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return B2_OK;
+}
+
+// Opts a kernel into `bytes` of dynamic shared memory once per (kernel, device).
+int allow_smem(const void* fn, size_t bytes) {
+  static std::mutex mu;
+  static std::set<std::pair<const void*, int>> done;
+  int dev = 0;
+  B2_TRY_CUDA(cudaGetDevice(&dev));
+  std::lock_guard<std::mutex> lock(mu);
+  if (done.count({fn, dev})) return B2_OK;
+  B2_TRY_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  done.insert({fn, dev});
+  return B2_OK;
+}
+
 template <typename T, int HD, int CODE, int NT>
 int launch_tiles(const Q8AttnParams& p, const AttnPlan& a, cudaStream_t s) {
   using C = AttnCfg<T, HD, CODE, NT>;
-  B2_TRY_CUDA(launch_pdl((q8_attn_kernel<T, HD, CODE, NT>), dim3(a.ctas), dim3(kWarps * 32), C::SMEM_Q, s, p, a.qt,
-                         a.units, a.per_group));
+  CUtensorMap mk, mv;
+  int rc = encode_cache(&mk, p.k_cache, p.num_blocks, p.nkv, HD);
+  if (rc == B2_OK) rc = encode_cache(&mv, p.v_cache, p.num_blocks, p.nkv, HD);
+  if (rc == B2_OK) rc = allow_smem((const void*)q8_attn_kernel<T, HD, CODE, NT>, C::SMEM);
+  if (rc) return rc;
+  B2_TRY_CUDA(launch_pdl((q8_attn_kernel<T, HD, CODE, NT>), dim3(a.ctas), dim3(kWarps * 32), C::SMEM, s, mk, mv, p,
+                         a.qt, a.units, a.per_group));
   B2_TRY_CUDA(launch_pdl((q8_join_kernel<T, HD>), dim3((unsigned)a.tiles, p.nkv), dim3(kJoinWarps * 32), 0, s, p, a.qt,
                          8 * a.nt));
   return B2_OK;

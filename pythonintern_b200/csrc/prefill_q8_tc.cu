@@ -8,10 +8,8 @@
 // (q stays as it is) and V codes in f16 (P is rounded to f16, 2^-11), so the only rounding that
 // prefill over the model's type does not have is the cache's own.  The scales stay out of the
 // operands: a K scale multiplies its 16 columns of S in the softmax, a V scale its 16 columns of
-// P: P = 2^(s - m2) vs against a reference m2 that follows the largest s + log2(vs), so f16 keeps
-// its precision however the scales of blocks differ, and l = sum 2^(s - m2) is taken as the sum of
-// P / vs block by block, which costs no second exponential.
-//
+// P.  l is summed against a reference m that follows the scores, P against a second one, m2, that
+// follows the largest s + log2(vs), so f16 keeps its precision however the scales of blocks differ.
 #include "prefill_tc.cuh"
 #include "q8.cuh"
 
@@ -35,8 +33,7 @@ static_assert(SMEM + 8 * kSeqCache + 512 <= 232448, "shared memory above the 227
 constexpr float kRoom = 15.f;  // log2 of the largest P
 constexpr float kLift = 8.f;   // log2 of P's largest value when a reference has just moved
 
-constexpr float kTiny = 1e-37f;          // stands for a K scale of 0
-constexpr float kNoScale = 0x1p-90f;     // stands for a V scale of 0
+constexpr float kTiny = 1e-37f;  // stands for a K scale of 0: -inf * 0 is not -inf
 
 struct ParamsQ8 : Params {
   const uint8_t* k_cache;
@@ -81,6 +78,11 @@ __device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) {
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t r;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
@@ -378,11 +380,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const bool row_ok = tk < nt;
       const int pos = it.ctx0 + t0 + tk;  // this row's token position (the last key it attends to)
-      // P = 2^(s - m2) vs against the row's reference m2; l = sum 2^(s - m2) = sum of P / vs
-      float m2_ref = -INFINITY, l_run = 0.f;
-      // Lane b < 4 sees to block b of a tile: its id is read two tiles ahead, its scales one.  Of
-      // these every row needs the factor kc of its raw scores (-1: a block outside the pool), log2
-      // of the V scale and its reciprocal.
+      // l = sum e, e = 2^(s - m); P = e vs 2^(m - m2) in f16, so that m2 follows s + log2(vs)
+      float m_ref = -INFINITY, m2_ref = -INFINITY, lift = 0.f, l_run = 0.f;
+      // Lane b < 4 sees to block b of a tile: its id is read two tiles ahead, its scales one.  Every
+      // row needs the factor kc of its raw scores (-1: a block outside the pool) and the V scale.
       auto id_of = [&](int j) -> int {
         const int bi = j * (KT / 16) + lane;
         if (lane >= KT / 16 || j >= n_kv || bi >= p.table_stride) return -1;
@@ -403,16 +404,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int b = js & 1;
         const int k0 = j * KT;
         // the scales were fetched a tile ago: their latency is behind the last tile's work
-        const float vs = vs_raw == 0.f ? kNoScale : vs_raw;  // a tile of zeros (the converters see to its codes)
-        const float kc_own = id_raw < 0 ? -1.f : ks_raw == 0.f ? kTiny : ks_raw * p.scale_log2;  // not 0: -inf * 0
-        const float lv_own = __log2f(vs), rv_own = __fdividef(1.f, vs);  // each within 2^-21
-        float kc[KT / 16], lv[KT / 16], rv[KT / 16];
+        const float kc_own = id_raw < 0 ? -1.f : ks_raw == 0.f ? kTiny : ks_raw * p.scale_log2;
+        float kc[KT / 16], vs[KT / 16];
         bool gap = false;  // a block of the tile is outside the pool
 #pragma unroll
         for (int u = 0; u < KT / 16; ++u) {
           kc[u] = __shfl_sync(0xffffffffu, kc_own, u);
-          lv[u] = __shfl_sync(0xffffffffu, lv_own, u);
-          rv[u] = __shfl_sync(0xffffffffu, rv_own, u);
+          vs[u] = __shfl_sync(0xffffffffu, vs_raw, u);
           gap |= kc[u] < 0.f;
         }
         fetch(id_next);
@@ -441,26 +439,32 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int u = 0; u < KT / 16; ++u)
             if (!row_ok || k0 + u * 16 > pos || kc[u] < 0.f) {
               kc[u] = kTiny;
-              lv[u] = rv[u] = 0.f;
+              vs[u] = 0.f;
             }
         }
-        float mx2 = -INFINITY;
+        float mx = -INFINITY, mx2 = -INFINITY;
 #pragma unroll
         for (int u = 0; u < KT / 16; ++u) {
           const float* t = sv + u * 16;
           const float a = max3(t[0], t[1], t[2]), c = max3(t[3], t[4], t[5]), d = max3(t[6], t[7], t[8]);
           const float f = max3(t[9], t[10], t[11]), g = max3(t[12], t[13], t[14]);
-          mx2 = fmaxf(mx2, fmaf(fmaxf(max3(a, c, d), max3(f, g, t[15])), kc[u], lv[u]));
+          const float top = fmaxf(max3(a, c, d), max3(f, g, t[15])) * kc[u];
+          mx = fmaxf(mx, top);
+          mx2 = fmaxf(mx2, vs[u] == 0.f ? -INFINITY : top + __log2f(vs[u]));  // only places a reference
         }
-        // the reference moves when a P would pass 2^15, to 2^8 below the largest
+        // the references move when a value would pass 2^15, to where it is 2^8
         bool need = false;
         float corr = 1.f;
-        if (mx2 > m2_ref + kRoom) {
-          const float m2n = mx2 - kLift;
-          need = m2_ref != -INFINITY;  // else the row's O is empty
-          corr = exp2f(m2_ref - m2n);
-          l_run *= corr;
+        if (mx > m_ref + kRoom || mx2 > m2_ref + kRoom) {
+          const float mn = fmaxf(m_ref, mx - kLift), m2n = fmaxf(m2_ref, mx2 - kLift);
+          l_run *= exp2f(m_ref - mn);  // from -inf: times 0, and l_run is 0
+          if (m2_ref != -INFINITY) {   // else the row's O is empty
+            need = m2n != m2_ref;
+            corr = exp2f(m2_ref - m2n);
+          }
+          m_ref = mn;
           m2_ref = m2n;
+          lift = m2n == -INFINITY ? 0.f : exp2f(mn - m2n);
         }
         if (__any_sync(0xffffffffu, need)) {
           // O must hold PV(js - 1) before it is rescaled (need implies j >= 1)
@@ -469,7 +473,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             break;
           }
           tc_fence_after();
-          if (!need) corr = 1.f;
 #pragma unroll 1
           for (int c = 0; c < HD; c += 32) {
             uint32_t o[32];
@@ -481,30 +484,33 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           tmem_wait_st();
         }
-        // P = exp2(raw * kc + (log2 vs - m2)) in f16; a row with nothing visible keeps P = 0
-        // (m2 = -inf is replaced by 0).  Pairs of keys share the packed float32 instructions.
-        const float m_sub = m2_ref == -INFINITY ? 0.f : m2_ref;
+        // e = exp2(raw * kc - m), P = e * vs * 2^(m - m2) in f16; a row with nothing visible keeps
+        // P = 0 (m = -inf is replaced by 0).  Pairs of keys share the packed float32 instructions.
+        const float m_sub = m_ref == -INFINITY ? 0.f : m_ref;
+        const uint64_t c2 = pack2(-m_sub, -m_sub);
         uint32_t pw[32];  // the row's P in f16 pairs: word w holds keys 2w (low half) and 2w + 1
 #pragma unroll
         for (int u = 0; u < KT / 16; ++u) {
           // the next S tile this group consumes (in this item or the next): ask now, so that the
           // answer has arrived when this tile is done
           if (u == 1) peek(pk_s, &s_full[grp][(js + 1) & 1], (uint32_t)((js + 1) >> 1) & 1u);
-          const uint64_t k2 = pack2(kc[u], kc[u]), c2 = pack2(lv[u] - m_sub, lv[u] - m_sub);
+          const float f = vs[u] == 0.f ? 0.f : vs[u] * lift;
+          const uint64_t k2 = pack2(kc[u], kc[u]), f2 = pack2(f, f);
           uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
           for (int e2 = 0; e2 < 8; ++e2) {
             const int e = u * 16 + e2 * 2;
             float x0, x1;
             unpack2(fma2(pack2(sv[e], sv[e + 1]), k2, c2), x0, x1);
-            const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);  // -inf gives 0
-            sum[e2 & 1] = add2(sum[e2 & 1], pack2(p0, p1));
-            const __half2 h2 = __floats2half2_rn(p0, p1);
+            const uint64_t e12 = pack2(ex2_approx(x0), ex2_approx(x1));  // -inf gives 0
+            sum[e2 & 1] = add2(sum[e2 & 1], e12);
+            unpack2(mul2(e12, f2), x0, x1);
+            const __half2 h2 = __floats2half2_rn(x0, x1);
             pw[u * 8 + e2] = *reinterpret_cast<const uint32_t*>(&h2);
           }
           float s0, s1;
           unpack2(add2(sum[0], sum[1]), s0, s1);
-          l_run = fmaf(s0 + s1, rv[u], l_run);
+          l_run += s0 + s1;
         }
         // P over the first 32 columns of this S buffer (read above): the A operand of PV(js),
         // which the tensor cores run before S(js + 2) rewrites the buffer
@@ -525,7 +531,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         break;
       }
       tc_fence_after();
-      const float inv = l_run == 0.f ? 0.f : 1.f / l_run;  // a NaN stays one
+      // O and l have references of their own; a row without weight gives 0 (NaN if a tile it saw is)
+      const float inv = m2_ref == -INFINITY ? (l_run == l_run ? 0.f : l_run) : exp2f(m2_ref - m_ref) / l_run;
       const int qb = items++ & 1;
       uint8_t* stage = smem + OFF_Q + (grp * 2 + qb) * Q_BYTES + quarter * 32 * (HD * 2);
 #pragma unroll 1
@@ -586,8 +593,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (bi * 16 <= last_pos) raise_status(p.status, B2_DEV_RANGE);
         return -1;
       };
-      // blocks whose V codes count: in the pool, and with a scale (0: a tile of zeros)
-      auto live_of = [&](int id) -> bool { return id >= 0 && __ldg(p.v_scale + (int64_t)id * p.nkv + it.g) != 0.f; };
       uint4 kcode[PIECES], vcode[PIECES];
       const int64_t at = ((int64_t)it.g * 16 + key0) * HD + half * 64 + ch * 16;
       auto load = [&](const uint8_t* cache, int ids, uint4 (&code)[PIECES]) {
@@ -600,14 +605,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       };
       int ids = id_of(0), ids_next = id_of(1);
-      bool live = live_of(ids);
       load(p.k_cache, ids, kcode);
       load(p.v_cache, ids, vcode);
       for (int j = 0; j < it.n_kv[0]; ++j, ++J) {
         const int st = J % ST;
-        const unsigned in_use = __ballot_sync(0xffffffffu, live);
+        const unsigned in_pool = __ballot_sync(0xffffffffu, ids >= 0);
         ids = ids_next;
-        live = live_of(ids);
         ids_next = id_of(j + 2);
         if (!__all_sync(0xffffffffu, mbar_wait(&kv_empty[st], ((uint32_t)(J / ST) & 1u) ^ 1u))) {
           ok = false;
@@ -630,7 +633,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < PIECES; ++i) {
           // keys that no row sees: whatever their codes (an e4m3 NaN among them), V is 0
           const int key = key0 + KEYS * i;
-          if (j * KT + key > last_pos || !(in_use >> (key / 16) & 1)) vcode[i] = make_uint4(0, 0, 0, 0);
+          if (j * KT + key > last_pos || !(in_pool >> (key / 16) & 1)) vcode[i] = make_uint4(0, 0, 0, 0);
           uint4 a, b;
           widen<CODE, false>(vcode[i].x, a.x, a.y);
           widen<CODE, false>(vcode[i].y, a.z, a.w);

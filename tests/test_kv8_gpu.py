@@ -600,6 +600,33 @@ def test_paged_attention_q8_wide_ranges(dtype):
         _close(out[r], want, size, dtype)
 
 
+@pytest.mark.parametrize("lens,ctx0", [([90, 40], [100, 0]), ([3, 2], [100, 7])])
+@pytest.mark.parametrize("nq,nkv", [(4, 2), (6, 2)])
+def test_prefill_attention_q8_wide_ranges(nq, nkv, lens, ctx0):
+    """The same for the kernels of many tokens per sequence."""
+    hd = 128
+    tab, NB = _tables_for([-(-(c + n) // 16) for c, n in zip(ctx0, lens)], 2, 1)
+    cache = _stored("int8", NB, nkv, hd, seed=4)
+    cache[3] *= torch.exp2(torch.randint(-20, 20, cache[3].shape, generator=gen(5)).float()).to(DEV)
+    for j in (0, 1):
+        cache[3][0, tab[0, j]] = 0
+    cache[3][0, tab[1, 0]] = 0
+    cache[2][0, tab[0, 2]] = 0
+    q = torch.randn(sum(lens), nq * hd, generator=gen(6))
+    q[::3] *= 6
+    q[1::5] *= 2.0 ** -60
+    q = q.to(DEV, torch.bfloat16)
+    start = [0, lens[0], sum(lens)]
+    out = kernels.prefill_attention_q8(q, nq, nkv, hd, *cache, 0, torch.from_numpy(tab).to(DEV), i32(start), 2,
+                                       1 / math.sqrt(hd), seq_ctx0=i32(ctx0))
+    _lib.check_device_status(DEV, "prefill")
+    for s, n in enumerate(lens):
+        for i in range(n):
+            r = start[s] + i
+            want, size = _attend64(q[r], cache, 0, tab[s].tolist(), ctx0[s] + i + 1, 1 / math.sqrt(hd))
+            _close(out[r], want, size, torch.bfloat16)
+
+
 @pytest.mark.parametrize("code", ["int8", "e4m3"])
 def test_attention_q8_ignores_what_lies_behind_the_context(code):
     """Codes (NaN ones too) behind the context, blocks behind it and their scales change nothing."""
