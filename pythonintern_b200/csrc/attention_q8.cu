@@ -36,6 +36,7 @@
 
 #include <mutex>
 #include <set>
+#include <type_traits>
 #include <utility>
 
 namespace b2 {
@@ -73,8 +74,8 @@ struct Q8AttnParams {
   int64_t ld_out;
   int32_t* status;
   // workspace
-  int* ws_tiles;    // [4]: tiles of the call
-  int4* ws_pairs;   // [tiles * nkv]: first and last warp, sequence, first token
+  int* ws_tiles;    // [2]: tiles of the call, steps per warp
+  int4* ws_pairs;   // [tiles * nkv]: first warp, last step from the warp's first on, unit, tile in it
   float4* ws_stat;  // [slots][columns]: m, l, m2
   float* ws_o;      // [slots][columns][head_dim]
 };
@@ -82,33 +83,32 @@ struct Q8AttnParams {
 
 // ------------------------------------------------------------------ the cut of the work
 constexpr int kWarps = 4;
-constexpr int kGroups = 512;   // prefix sums kept in shared memory
-constexpr int kMinChunk = 4;   // steps a warp takes at least
+constexpr int kGroups = 256;   // prefix sums kept in shared memory
+constexpr int kMinChunk = 2;   // steps a warp takes at least
 
 struct Unit {  // a decode row, or a sequence of a prefill
   int start, len, ctx0;  // first row of q, tokens, keys before the first token
-  bool bad;
 };
 
 __device__ __forceinline__ int table_row(const Q8AttnParams& p, int u) {
   return !p.seq_start && p.table_index ? p.table_index[u] : u;
 }
 
-__device__ __forceinline__ Unit unit_of(const Q8AttnParams& p, int u) {
-  Unit r{u, 0, 0, false};
+__device__ __forceinline__ Unit unit_of(const Q8AttnParams& p, int u, bool& bad) {
+  Unit r{u, 0, 0};
   const int64_t most = (int64_t)p.table_stride * kQ8Block;
   if (!p.seq_start) {
     const int row = table_row(p, u), ctx = p.ctx_lens[u];
     const bool there = row >= 0 && row < p.table_rows;
-    r.bad = !there || ctx > most;
+    bad = !there || ctx > most;
     const int keys = there ? (int)min((int64_t)ctx, most) : 0;  // a context past its table row: the row's keys
     r.len = keys > 0 ? 1 : 0;
     r.ctx0 = keys - 1;
   } else {
     const int a = p.seq_start[u], b = p.seq_start[u + 1];
     const int ctx0 = p.seq_ctx0 ? p.seq_ctx0[u] : 0;
-    r.bad = a < 0 || b > p.n_rows || b < a || ctx0 < 0 || (b > a && (int64_t)ctx0 + b - a > most);
-    if (!r.bad) {
+    bad = a < 0 || b > p.n_rows || b < a || ctx0 < 0 || (b > a && (int64_t)ctx0 + b - a > most);
+    if (!bad) {
       r.start = a;
       r.len = b - a;
       r.ctx0 = ctx0;
@@ -117,12 +117,20 @@ __device__ __forceinline__ Unit unit_of(const Q8AttnParams& p, int u) {
   return r;
 }
 
-__device__ __forceinline__ int blocks_of(int64_t keys) { return (int)((keys + kQ8Block - 1) / kQ8Block); }
+__device__ __forceinline__ Unit unit_of(const Q8AttnParams& p, int u) {
+  bool bad;
+  return unit_of(p, u, bad);
+}
+
+__device__ __forceinline__ int blocks_of(int64_t keys) {
+  return (int)((uint64_t)(keys + kQ8Block - 1) / kQ8Block);
+}
 
 // Blocks of the first x tiles of a unit: sum over j = 1..x of ceil((ctx0 + min(j qt, len)) / 16).
 // Over the full tiles the remainders repeat with period 16 / gcd(qt, 16), and every further
 // period adds the same number to each of its terms.
 __device__ __forceinline__ int64_t blocks_before(const Unit& u, int qt, int x) {
+  if (x <= 1) return x == 0 ? 0 : blocks_of((int64_t)u.ctx0 + min(qt, u.len));  // a decode row, say
   const int full = min(x, u.len / qt);
   int per = kQ8Block;
   while (per > 1 && (qt * (per / 2)) % kQ8Block == 0) per /= 2;
@@ -137,7 +145,7 @@ __device__ __forceinline__ int64_t blocks_before(const Unit& u, int qt, int x) {
   return sum;
 }
 
-__device__ __forceinline__ int tiles_of(const Unit& u, int qt) { return (u.len + qt - 1) / qt; }
+__device__ __forceinline__ int tiles_of(const Unit& u, int qt) { return u.len <= 1 ? u.len : (u.len + qt - 1) / qt; }
 
 struct Cut {
   int64_t total;  // steps of the call, all kv heads
@@ -146,10 +154,15 @@ struct Cut {
   int max_ctx;    // longest context (compat_pad)
 };
 
-// Prefix sums over groups of units: sm_steps[i] blocks (of one kv head) and sm_tiles[i] tiles
-// before group i.  Called by the whole CTA.
-__device__ Cut make_cut(const Q8AttnParams& p, int qt, int n_units, int per_group, int64_t* sm_steps, int* sm_tiles,
-                        int warps, bool report) {
+// What every CTA keeps in shared memory of the line of steps.
+struct Line {
+  int64_t steps[kGroups];  // blocks (of one kv head) before a group of units
+  int tiles[kGroups];      // tiles before it
+  Unit unit[kGroups];      // its first unit
+};
+
+// Prefix sums over groups of units.  Called by the whole CTA.
+__device__ Cut make_cut(const Q8AttnParams& p, int qt, int n_units, int per_group, Line& line, int warps, bool report) {
   __shared__ int64_t w_steps[kWarps];
   __shared__ int w_tiles[kWarps], w_ctx[kWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = kWarps * 32;
@@ -160,11 +173,13 @@ __device__ Cut make_cut(const Q8AttnParams& p, int qt, int n_units, int per_grou
   bool bad = false;
   const int g0 = min(groups, tid * per_thread), g1 = min(groups, g0 + per_thread);
   for (int g = g0; g < g1; ++g) {
-    sm_steps[g] = steps;
-    sm_tiles[g] = tiles;
+    line.steps[g] = steps;
+    line.tiles[g] = tiles;
     for (int u = g * per_group; u < min(n_units, (g + 1) * per_group); ++u) {
-      const Unit x = unit_of(p, u);
-      bad |= x.bad;
+      bool odd;
+      const Unit x = unit_of(p, u, odd);
+      if (u == g * per_group) line.unit[g] = x;
+      bad |= odd;
       const int n = tiles_of(x, qt);
       steps += blocks_before(x, qt, n);
       tiles += n;
@@ -204,12 +219,13 @@ __device__ Cut make_cut(const Q8AttnParams& p, int qt, int n_units, int per_grou
     c.max_ctx = max(c.max_ctx, w_ctx[w]);
   }
   for (int g = g0; g < g1; ++g) {
-    sm_steps[g] += base_s;
-    sm_tiles[g] += base_t;
+    line.steps[g] += base_s;
+    line.tiles[g] += base_t;
   }
   __syncthreads();
   c.total *= p.nkv;
-  c.chunk = max((int64_t)kMinChunk, (c.total + warps - 1) / warps);
+  const int64_t even = c.total >> 32 ? (c.total + warps - 1) / warps : ((uint32_t)c.total + warps - 1) / (uint32_t)warps;
+  c.chunk = max((int64_t)kMinChunk, even);
   return c;
 }
 
@@ -220,24 +236,23 @@ struct Place {  // where a step lies
   int g;          // kv head
   int block;      // block in the tile
   int blocks;     // blocks of the tile
-  int64_t begin;  // first step of (tile, kv head)
+  int begin;      // first step of (tile, kv head), counted from the warp's first
 };
 
 // Finds step x of the line; the same for all lanes of a warp.
 __device__ __forceinline__ Place find_step(const Q8AttnParams& p, int64_t x, int qt, int n_units, int per_group,
-                                           const int64_t* sm_steps, const int* sm_tiles) {
+                                           const Line& line) {
   const int groups = (n_units + per_group - 1) / per_group;
   int lo = 0, hi = groups - 1;
   while (lo < hi) {  // the last group that begins at or before x (empty ones share their successor's begin)
     const int mid = (lo + hi + 1) >> 1;
-    if (sm_steps[mid] * p.nkv <= x) lo = mid; else hi = mid - 1;
+    if (line.steps[mid] * p.nkv <= x) lo = mid; else hi = mid - 1;
   }
   Place r;
   r.u = lo * per_group;
-  r.tile = sm_tiles[lo];
-  int64_t before = sm_steps[lo];
-  for (;; ++r.u) {
-    r.unit = unit_of(p, r.u);
+  r.tile = line.tiles[lo];
+  int64_t before = line.steps[lo];
+  for (r.unit = line.unit[lo];; r.unit = unit_of(p, ++r.u)) {
     const int n = tiles_of(r.unit, qt);
     const int64_t all = blocks_before(r.unit, qt, n);
     if (x < (before + all) * p.nkv || r.u == n_units - 1) break;
@@ -254,14 +269,14 @@ __device__ __forceinline__ Place find_step(const Q8AttnParams& p, int64_t x, int
   before += blocks_before(r.unit, qt, a);
   r.blocks = blocks_of((int64_t)r.unit.ctx0 + min((a + 1) * qt, r.unit.len));
   const int64_t in = x - before * p.nkv;
-  r.g = (int)(in / r.blocks);
-  r.block = (int)(in % r.blocks);
-  r.begin = x - r.block;
+  r.g = in >> 32 ? (int)(in / r.blocks) : (int)((uint32_t)in / (uint32_t)r.blocks);
+  r.block = (int)(in - (int64_t)r.g * r.blocks);
+  r.begin = -r.block;
   return r;
 }
 
 // Moves to the first step of the next (tile, kv head).
-__device__ __forceinline__ void next_pair(const Q8AttnParams& p, Place& r, int qt) {
+__device__ __forceinline__ void next_pair(const Q8AttnParams& p, Place& r, int qt, int per_group, const Line& line) {
   r.begin += r.blocks;
   r.block = 0;
   if (++r.g < p.nkv) return;
@@ -269,7 +284,8 @@ __device__ __forceinline__ void next_pair(const Q8AttnParams& p, Place& r, int q
   ++r.tile;
   ++r.j;
   while (r.j >= tiles_of(r.unit, qt)) {  // the caller has checked that there is another step
-    r.unit = unit_of(p, ++r.u);
+    ++r.u;
+    r.unit = per_group == 1 ? line.unit[r.u] : unit_of(p, r.u);
     r.j = 0;
   }
   r.blocks = blocks_of((int64_t)r.unit.ctx0 + min((r.j + 1) * qt, r.unit.len));
@@ -278,10 +294,15 @@ __device__ __forceinline__ void next_pair(const Q8AttnParams& p, Place& r, int q
 // ------------------------------------------------------------------ fragments
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
 
-// Two pairs of codes (the bytes 0, 1 and 2, 3 of x) as float16 pairs.
-template <int CODE>
+// Two pairs of codes (the bytes 0, 1 and 2, 3 of x) as float16 pairs.  BIASED: as the float16
+// numbers (code + 128) * 2^-24, whose bits are the byte itself.
+template <int CODE, bool BIASED = false>
 __device__ __forceinline__ void expand(uint32_t x, uint32_t& lo, uint32_t& hi) {
-  if constexpr (CODE == B2_I8) {
+  if constexpr (BIASED) {
+    const uint32_t u = x ^ 0x80808080u;
+    lo = prmt(u, 0u, 0x4140);
+    hi = prmt(u, 0u, 0x4342);
+  } else if constexpr (CODE == B2_I8) {
     // 0x6400 | u is the float16 1024 + u for a byte u; u = code + 128
     const uint32_t u = x ^ 0x80808080u;
     const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));  // 1152
@@ -328,33 +349,61 @@ __device__ __forceinline__ void load_tile(void* dst, const CUtensorMap* map, uin
       : "memory");
 }
 
-__device__ __forceinline__ void ld4q(const float* p, float (&v)[4]) {
-  const float4 a = *reinterpret_cast<const float4*>(p);
+// Four elements of q, as they are in memory.
+template <typename T>
+struct Raw4 {
+  using Type = typename std::conditional<sizeof(T) == 4, float4, uint2>::type;
+};
+__device__ __forceinline__ void widen4(const float4& a, float (&v)[4]) {
   v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
 }
-__device__ __forceinline__ void ld4q(const __nv_bfloat16* p, float (&v)[4]) {
-  const uint2 a = *reinterpret_cast<const uint2*>(p);
+__device__ __forceinline__ void widen4(const uint2& a, float (&v)[4]) {
   v[0] = __uint_as_float(a.x << 16); v[1] = __uint_as_float(a.x & 0xffff0000u);
   v[2] = __uint_as_float(a.y << 16); v[3] = __uint_as_float(a.y & 0xffff0000u);
 }
 
-constexpr int kStages = 3;          // tiles of K and V a warp holds or has in flight
 constexpr float kRoom = 15.f;       // log2 of the largest P
 constexpr float kLift = 8.f;        // log2 of the largest P when a reference has just moved
 constexpr float kNoRef = -1e30f;    // reference of a column that has seen no key
+
+constexpr int ctas_per_sm(int nt, int terms) { return nt * terms <= 2 ? 3 : 2; }
 
 template <typename T, int HD, int CODE, int NT>
 struct AttnCfg {
   static constexpr int N = 8 * NT;                       // columns of a tile
   static constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;   // float16 terms of q and P
+  // S from K codes + 128 taken as float16 subnormals: q . (c + 128) - 128 sum(q), half the work of
+  // making signed numbers of them.  It costs S a rounding of 128 |sum q| in float32, nothing
+  // next to the float16 of P; float32 queries do without.
+  static constexpr bool BIASED = CODE == B2_I8 && TERMS == 1;
   static constexpr int KW = HD / 16;                     // words of codes a lane holds of a key; MMAs of S
   static constexpr int VW = HD / 32;                     // and of a key's values
   static constexpr int TILE = kQ8Block * HD;             // bytes of codes of one block and head
   static constexpr int Q_BYTES = KW * NT * TERMS * 32 * 8;
-  static constexpr int WARP_BYTES = kStages * 2 * TILE;  // the warp's ring of K and V tiles
+  // Tiles of K and V a warp holds or has in flight, and CTAs per SM that the registers are limited
+  // for and the shared memory holds.
+  static constexpr int STAGES = 3;
+  static constexpr int CTAS = ctas_per_sm(NT, TERMS);
+  static constexpr int WARP_BYTES = STAGES * 2 * TILE;
   // ring (1024-byte aligned for the swizzle), then the q fragments
   static constexpr int SMEM = 1024 + kWarps * (WARP_BYTES + Q_BYTES);
 };
+
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint2 lds8(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds4(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
 
 // Byte offset of 16-byte chunk `chunk` of key row `row` in a tile that TMA has stored with the
 // swizzle as wide as a row (128, 64 or 32 bytes).
@@ -364,28 +413,24 @@ __device__ __forceinline__ int tile_at(int row, int chunk) {
   return row * HD + ((chunk ^ (row * HD / 128 & (CHUNKS - 1))) << 4);
 }
 
-// CTAs per SM that the registers are limited for and the shared memory holds.
-constexpr int ctas_per_sm(int nt, int terms) { return nt * terms <= 2 ? 3 : 2; }
-
 // Up to 32 consecutive steps of one (tile, kv head); lane i holds what step i needs.
 struct Window {
-  Place at;       // of the first step
-  int cnt;        // steps; 0: behind the warp's chunk
-  int id;         // block id, -1 outside the pool
-  float ks, vs;   // scales
+  int cnt;       // steps; 0: behind the warp's chunk
+  int g;         // kv head
+  int id;        // block id, -1 outside the pool
+  float ks, vs;  // scales
 };
 
 template <typename T, int HD, int CODE, int NT>
-__global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(NT, sizeof(T) == 4 ? 2 : 1))
+__global__ void __launch_bounds__(kWarps * 32, (AttnCfg<T, HD, CODE, NT>::CTAS))
 q8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const Q8AttnParams p,
                int qt, int n_units, int per_group) {
   pdl_wait();
   pdl_trigger();
   using C = AttnCfg<T, HD, CODE, NT>;
-  constexpr int KW = C::KW, VW = C::VW, TERMS = C::TERMS, N = C::N;
-  __shared__ int64_t sm_steps[kGroups];
-  __shared__ int sm_tiles[kGroups];
-  __shared__ __align__(8) uint64_t full[kWarps][kStages];
+  constexpr int KW = C::KW, VW = C::VW, TERMS = C::TERMS, N = C::N, STAGES = C::STAGES;
+  __shared__ Line line;
+  __shared__ __align__(8) uint64_t full[kWarps][STAGES];
   extern __shared__ uint8_t smem_raw[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int r8 = lane >> 2, t4 = lane & 3;
@@ -393,63 +438,75 @@ q8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   const int rep = p.nq / p.nkv;
   uint8_t* smem = smem_raw + ((1024 - (tc::smem_u32(smem_raw) & 1023)) & 1023);
   uint8_t* ring = smem + warp * C::WARP_BYTES;
-  uint2* sq = reinterpret_cast<uint2*>(smem + kWarps * C::WARP_BYTES + warp * C::Q_BYTES);
+  const uint32_t ring_at = tc::smem_u32(ring);
+  uint2* sq = reinterpret_cast<uint2*>(smem + kWarps * C::WARP_BYTES + warp * C::Q_BYTES) + lane;
+  const uint32_t sq_at = tc::smem_u32(sq);
+  // what the lane reads of a tile: its codes of keys r8 (and, 8 rows on, r8 + 8), of keys 2 t4 and
+  // 2 t4 + 1 (and 8 rows on)
+  uint32_t k_off[KW == 8 ? 2 : 1], v_off[2];
+#pragma unroll
+  for (int c = 0; c < (KW == 8 ? 2 : 1); ++c)
+    k_off[c] = KW == 2 ? tile_at<HD>(r8, t4 >> 1) + (t4 & 1) * 8 : tile_at<HD>(r8, t4 * (KW / 4) + c);
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    v_off[h] = C::TILE + (VW == 4   ? tile_at<HD>(2 * t4 + h, r8)
+                          : VW == 2 ? tile_at<HD>(2 * t4 + h, r8 >> 1) + (r8 & 1) * 8
+                                    : tile_at<HD>(2 * t4 + h, r8 >> 2) + (r8 & 3) * 4);
 
   if (lane == 0) {
-    for (int i = 0; i < kStages; ++i) tc::mbar_init(&full[warp][i], 1);
+    for (int i = 0; i < STAGES; ++i) tc::mbar_init(&full[warp][i], 1);
     tc::fence_mbar_init();
   }
-  const Cut cut = make_cut(p, qt, n_units, per_group, sm_steps, sm_tiles, warps, blockIdx.x == 0);
+  const Cut cut = make_cut(p, qt, n_units, per_group, line, warps, blockIdx.x == 0);
   // a seq_start that goes back may name more tokens than there are rows (and tiles than the
   // workspace has room for): nothing is computed
   const bool sane = !p.seq_start || (int64_t)cut.tiles <= (int64_t)(p.n_rows / qt) + n_units;
   if (w == 0 && lane == 0) {
     p.ws_tiles[0] = sane ? cut.tiles : 0;
+    p.ws_tiles[1] = (int)cut.chunk;
     if (!sane) raise_status(p.status, B2_DEV_RANGE);
   }
   if (!sane) return;
-  if (!p.seq_start) {  // decode rows without keys
-    for (int u = blockIdx.x; u < n_units; u += gridDim.x) {
-      if (unit_of(p, u).len > 0) continue;
+  const int64_t x_begin = w * cut.chunk, x_end = min(cut.total, x_begin + cut.chunk);
+  if (!p.seq_start) {  // decode rows without keys: from the last warps, which have the least to do
+    for (int u = warps - 1 - w; u < n_units; u += warps) {
+      if ((per_group == 1 ? line.unit[u] : unit_of(p, u)).len > 0) continue;
       T* dst = reinterpret_cast<T*>(p.out) + (int64_t)u * p.ld_out;
-      for (int i = threadIdx.x; i < p.nq * HD; i += kWarps * 32) dst[i] = from_f32<T>(0.f);
+      for (int i = lane; i < p.nq * HD; i += 32) dst[i] = from_f32<T>(0.f);
     }
   }
-  const int64_t x_begin = w * cut.chunk, x_end = min(cut.total, x_begin + cut.chunk);
   if (x_begin >= x_end) return;
 
-  int64_t left = x_end - x_begin;  // steps behind the windows taken so far
-  auto ids_of = [&](Window& win) {  // sets cnt from the place, starts the loads of the ids
-    win.cnt = (int)min((int64_t)min(32, win.at.blocks - win.at.block), left);
+  int left = (int)(x_end - x_begin);  // steps behind the windows taken so far
+  // The window that begins at `from` (cnt 0 at the end of the chunk): starts the loads of its ids.
+  auto take = [&](const Place& from) -> Window {
+    Window win;
+    win.cnt = min(min(32, from.blocks - from.block), left);
     left -= win.cnt;
-    int id = -1;
-    if (lane < win.cnt) id = __ldg(p.tables + (int64_t)table_row(p, win.at.u) * p.table_stride + win.at.block + lane);
-    win.id = id;
+    win.g = from.g;
+    win.id = -1;
+    if (lane < win.cnt)
+      win.id = __ldg(p.tables + (int64_t)table_row(p, from.u) * p.table_stride + from.block + lane);
+    return win;
+  };
+  auto advance = [&](Place& pl, int cnt) {
+    pl.block += cnt;
+    if (pl.block == pl.blocks) next_pair(p, pl, qt, per_group, line);
   };
   auto scales_of = [&](Window& win) {
     const bool in_pool = win.id >= 0 && win.id < p.num_blocks;
     if (lane < win.cnt && !in_pool) raise_status(p.status, B2_DEV_RANGE);
     if (!in_pool) win.id = -1;
-    const int64_t at = in_pool ? q8_scale(win.id, p.nkv, win.at.g) : 0;
+    const int64_t at = in_pool ? q8_scale(win.id, p.nkv, win.g) : 0;
     win.ks = __ldg(p.k_scale + at);
     win.vs = __ldg(p.v_scale + at);
   };
-  // The window behind `win` in the warp's chunk.
-  auto window_after = [&](const Window& win) -> Window {
-    Window nx;
-    nx.at = win.at;
-    nx.cnt = 0;
-    nx.id = -1;
-    if (left == 0) return nx;
-    nx.at.block += win.cnt;
-    if (nx.at.block == nx.at.blocks) next_pair(p, nx.at, qt);
-    ids_of(nx);
-    return nx;
-  };
 
-  int n_used = 0, n_open = 0;  // steps consumed; tiles in the ring or on their way
+  int n_open = 0;                             // tiles in the ring or on their way
+  int at_slot = 0, at_phase = 0, to_slot = 0;  // next to consume (and its barrier's phase), next to ask for
   auto issue = [&](const Window& win, int i) {
-    const int slot = (n_used + n_open) % kStages;
+    const int slot = to_slot;
+    to_slot = to_slot == STAGES - 1 ? 0 : to_slot + 1;
     const int id = __shfl_sync(0xffffffffu, win.id, i);
     ++n_open;
     if (lane == 0) {
@@ -457,21 +514,42 @@ q8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       if (id >= 0 && id < p.num_blocks) {
         uint8_t* dst = ring + slot * 2 * C::TILE;
         tc::mbar_arrive_expect_tx(bar, 2 * C::TILE);
-        load_tile(dst, &tmK, bar, win.at.g * kQ8Block, id);
-        load_tile(dst + C::TILE, &tmV, bar, win.at.g * kQ8Block, id);
+        load_tile(dst, &tmK, bar, win.g * kQ8Block, id);
+        load_tile(dst + C::TILE, &tmV, bar, win.g * kQ8Block, id);
       } else {
         tc::mbar_arrive(bar);  // nothing to wait for: the step is left out
       }
     }
   };
 
-  Window cur, nxt;
-  cur.at = find_step(p, x_begin, qt, n_units, per_group, sm_steps, sm_tiles);
-  ids_of(cur);
-  nxt = window_after(cur);
+  // q of a tile's columns.  Where they are few, the raw loads are made ahead, so that their latency
+  // hides behind the ids'; more would not fit the registers.
+  using Raw = typename Raw4<T>::Type;
+  constexpr bool EARLY = NT * TERMS == 1;
+  const uint32_t inv_rep = (65536u + rep - 1) / rep;  // c / rep = c * inv_rep >> 16 for c < 32, rep <= 16
+  Raw raw[KW];
+  auto load_q = [&](const Place& at, int nt) {
+    const int tok0 = at.j * qt, ncol = min(qt, at.unit.len - tok0) * rep;
+    const int col = nt * 8 + r8, tok = (int)(col * inv_rep >> 16);
+    const bool live = col < ncol;
+    const T* src = reinterpret_cast<const T*>(p.q) + (int64_t)(at.unit.start + tok0 + (live ? tok : 0)) * p.ld_q +
+                   (int64_t)(at.g * rep + (live ? col - tok * rep : 0)) * HD + t4 * (HD / 4);
+#pragma unroll
+    for (int k = 0; k < KW; ++k) raw[k] = reinterpret_cast<const Raw*>(src)[k];
+  };
+
+  Place at = find_step(p, x_begin, qt, n_units, per_group, line);
+  Window cur = take(at), nxt = cur;
+  if (EARLY) load_q(at, 0);
+  nxt.cnt = 0;
+  if (left > 0) {
+    Place to = at;
+    advance(to, cur.cnt);
+    nxt = take(to);
+  }
   int sent = 0, sent_nxt = 0;  // steps of either window whose tiles were asked for
   auto top_up = [&]() {
-    while (n_open < kStages) {
+    while (n_open < STAGES) {
       if (sent < cur.cnt) issue(cur, sent++);
       else if (sent_nxt < nxt.cnt) issue(nxt, sent_nxt++);
       else break;
@@ -480,7 +558,7 @@ q8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   top_up();
   scales_of(cur);
 
-  float colscale[NT][2];
+  float colscale[NT][2], bias[NT][2];
   int lim[NT][2];  // last key of the lane's columns
   float o[2 * VW][NT][4];
   float m[NT][2], m2[NT][2], lift[NT][2], l[NT][2];  // references, 2^(m - m2), sums
@@ -489,49 +567,52 @@ q8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   bool first = true, ok = true;
 
   while (cur.cnt > 0) {
-    const Place& at = cur.at;
     const int tok0 = at.j * qt, ntok = min(qt, at.unit.len - tok0);
     const int ncol = ntok * rep;
     const int pos0 = at.unit.ctx0 + tok0;  // position of the tile's first token
     const int pos_last = pos0 + ntok - 1;
     if (start) {
       start = false;
-      // A (tile, kv head) begins: q of its columns into the warp's shared memory as B fragments.
       i0 = at.block;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const int col = nt * 8 + r8;
-        float q[KW][4];
+        if (!EARLY) load_q(at, nt);
+        const bool live = nt * 8 + r8 < ncol;
         float big = 0.f;
-        const bool live = col < ncol;
-        const T* src = reinterpret_cast<const T*>(p.q) +
-                       (int64_t)(at.unit.start + tok0 + (live ? col / rep : 0)) * p.ld_q +
-                       (int64_t)(at.g * rep + (live ? col % rep : 0)) * HD + t4 * (HD / 4);
-#pragma unroll
-        for (int k = 0; k < KW; ++k) {
-          ld4q(src + k * 4, q[k]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (!live) q[k][e] = 0.f;
-            big = fmaxf(big, fabsf(q[k][e]));
-          }
-        }
-        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-        // a power of two that brings `big` to [2^14, 2^15); in two factors, so that neither overflows
-        const int ex = big > 0.f && big <= 3.402823466e38f ? 14 - ilogbf(big) : 0;
-        const float up = ldexpf(1.f, ex / 2), up2 = ldexpf(1.f, ex - ex / 2);
 #pragma unroll
         for (int k = 0; k < KW; ++k) {
           float v[4];
+          widen4(raw[k], v);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = q[k][e] * up * up2;
+          for (int e = 0; e < 4; ++e) big = fmaxf(big, fabsf(v[e]));
+        }
+        if (!live) big = 0.f;
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+        // 2^ex brings `big` to [2^14, 2^15) (below it, if `big` is not a normal number); in two factors,
+        // so that neither overflows.  Infinite and NaN heads are left as they are.
+        const int field = (int)(__float_as_uint(big) >> 23);
+        const int ex = field == 0 || field == 255 ? (field ? 0 : 140) : 141 - field, ex2nd = ex / 2;
+        const float up = __uint_as_float((uint32_t)(127 + ex2nd) << 23);
+        const float up2 = __uint_as_float((uint32_t)(127 + ex - ex2nd) << 23);
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < KW; ++k) {
+          float v[4];
+          widen4(raw[k], v);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = live ? v[e] * up * up2 : 0.f;
 #pragma unroll
           for (int term = 0; term < TERMS; ++term) {
             uint2 f;
             f.x = pack_f16(v[0], v[1]);
             f.y = pack_f16(v[2], v[3]);
-            sq[((k * NT + nt) * TERMS + term) * 32 + lane] = f;
+            if (C::BIASED) {  // of what the products will see
+              const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&f.x));
+              const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&f.y));
+              sum += (a.x + a.y) + (b.x + b.y);
+            }
+            sq[((k * NT + nt) * TERMS + term) * 32] = f;
             if (TERMS == 2) {
               const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&f.x));
               const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&f.y));
@@ -539,49 +620,62 @@ q8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             }
           }
         }
-        const float back = live ? ldexpf(p.scale_log2, -ex) : 0.f;
+        const float back = live ? p.scale_log2 * __uint_as_float((uint32_t)(127 - ex2nd) << 23) *
+                                      __uint_as_float((uint32_t)(127 - ex + ex2nd) << 23) *
+                                      (C::BIASED ? 0x1p24f : 1.f)
+                                : 0.f;
+        if (C::BIASED) {
+          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int c = nt * 8 + 2 * t4 + e;
           colscale[nt][e] = __shfl_sync(0xffffffffu, back, (2 * t4 + e) * 4);
-          lim[nt][e] = c < ncol ? pos0 + c / rep : -1;
+          if (C::BIASED) bias[nt][e] = __shfl_sync(0xffffffffu, sum, (2 * t4 + e) * 4) * (-128.f * 0x1p-24f);
+          lim[nt][e] = c < ncol ? pos0 + (int)(c * inv_rep >> 16) : -1;
           m[nt][e] = m2[nt][e] = kNoRef;
           lift[nt][e] = l[nt][e] = 0.f;
         }
 #pragma unroll
         for (int d = 0; d < 2 * VW; ++d) o[d][nt][0] = o[d][nt][1] = o[d][nt][2] = o[d][nt][3] = 0.f;
       }
+      asm volatile("" ::: "memory");  // the fragments are read back by lds8
     }
+    const int tail_from = (pos0 + 1) / kQ8Block - at.block;  // steps whose keys some column does not see
 
     for (int i = 0; i < cur.cnt; ++i) {
-      top_up();
-      if (i == 0) scales_of(nxt);  // its ids were asked for a window ago
+      if (i == 0 && nxt.cnt > 0) scales_of(nxt);  // its ids were asked for a window ago
       const int blk = __shfl_sync(0xffffffffu, cur.id, i);
       const float ks = __shfl_sync(0xffffffffu, cur.ks, i), vs = __shfl_sync(0xffffffffu, cur.vs, i);
-      const int slot = n_used % kStages;
-      if (!__all_sync(0xffffffffu, tc::mbar_wait(&full[warp][slot], (uint32_t)(n_used / kStages) & 1u))) {
+      const int slot = at_slot;
+      if (!__all_sync(0xffffffffu, tc::mbar_wait(&full[warp][slot], (uint32_t)at_phase))) {
         ok = false;
         break;
       }
-      ++n_used;
+      at_slot = slot == STAGES - 1 ? 0 : slot + 1;
+      at_phase ^= slot == STAGES - 1;
       --n_open;
-      if (blk < 0) continue;  // a block outside the pool: its keys are left out
-      const uint8_t* kt = ring + slot * 2 * C::TILE;
-      const uint8_t* vt = kt + C::TILE;
-      float s[NT][4];
+      if (blk < 0) {  // a block outside the pool: its keys are left out
+        top_up();
+        continue;
+      }
+      const uint32_t tile = ring_at + slot * (2 * C::TILE);
+      float s[NT][4], s_odd[NT == 1 ? 1 : NT][4];  // two chains of products where there are few columns
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[nt][e] = s_odd[nt][e] = 0.f;
       uint32_t kw[2][KW];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int row = r8 + 8 * h;
+      for (int h = 0; h < 2; ++h) {  // rows eight apart have the same swizzle
         if constexpr (KW == 2) {
-          const uint2 v = *reinterpret_cast<const uint2*>(kt + tile_at<HD>(row, t4 >> 1) + (t4 & 1) * 8);
+          const uint2 v = lds8(tile + k_off[0] + h * 8 * HD);
           kw[h][0] = v.x; kw[h][1] = v.y;
         } else {
 #pragma unroll
           for (int k = 0; k < KW; k += 4) {
-            const uint4 v = *reinterpret_cast<const uint4*>(kt + tile_at<HD>(row, t4 * (KW / 4) + k / 4));
+            const uint4 v = lds16(tile + k_off[k / 4] + h * 8 * HD);
             kw[h][k] = v.x; kw[h][k + 1] = v.y; kw[h][k + 2] = v.z; kw[h][k + 3] = v.w;
           }
         }
@@ -589,34 +683,23 @@ q8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
 #pragma unroll
       for (int k = 0; k < KW; ++k) {
         uint32_t a[4];
-        expand<CODE>(kw[0][k], a[0], a[2]);
-        expand<CODE>(kw[1][k], a[1], a[3]);
+        expand<CODE, C::BIASED>(kw[0][k], a[0], a[2]);
+        expand<CODE, C::BIASED>(kw[1][k], a[1], a[3]);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int term = 0; term < TERMS; ++term) {
-            const uint2 b = sq[((k * NT + nt) * TERMS + term) * 32 + lane];
-            mma_f16(s[nt], a, b.x, b.y);
+            const uint2 b = lds8(sq_at + ((k * NT + nt) * TERMS + term) * 32 * 8);
+            mma_f16(NT == 1 && (k & 1) ? s_odd[nt] : s[nt], a, b.x, b.y);
           }
       }
-      uint32_t vw[4][VW];
+      if constexpr (NT == 1) {
 #pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        const int row = 2 * t4 + (h & 1) + (h >> 1) * 8;
-        if constexpr (VW == 4) {
-          const uint4 v = *reinterpret_cast<const uint4*>(vt + tile_at<HD>(row, r8));
-          vw[h][0] = v.x; vw[h][1] = v.y; vw[h][2] = v.z; vw[h][3] = v.w;
-        } else if constexpr (VW == 2) {
-          const uint2 v = *reinterpret_cast<const uint2*>(vt + tile_at<HD>(row, r8 >> 1) + (r8 & 1) * 8);
-          vw[h][0] = v.x; vw[h][1] = v.y;
-        } else {
-          vw[h][0] = *reinterpret_cast<const uint32_t*>(vt + tile_at<HD>(row, r8 >> 2) + (r8 & 3) * 4);
-        }
+        for (int e = 0; e < 4; ++e) s[0][e] += s_odd[0][e];
       }
-
       // scores; the tail of the tile's keys is masked per column
       const int key0 = (at.block + i) * kQ8Block, key = key0 + r8;
-      const bool tail = key0 + kQ8Block - 1 > pos0;
+      const bool tail = i >= tail_from;
       if (tail) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -634,8 +717,14 @@ q8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         for (int e = 0; e < 2; ++e) {
           // a column that sees none of the block's keys takes nothing from its scales
           const float cs = tail && key0 > lim[nt][e] ? 1.f : colscale[nt][e] * ks;
-          s[nt][e] *= cs;
-          s[nt][2 + e] *= cs;
+          if (C::BIASED) {
+            const float b = bias[nt][e] * cs;
+            s[nt][e] = fmaf(s[nt][e], cs, b);
+            s[nt][2 + e] = fmaf(s[nt][2 + e], cs, b);
+          } else {
+            s[nt][e] *= cs;
+            s[nt][2 + e] *= cs;
+          }
           move |= fmaxf(s[nt][e], s[nt][2 + e]) > fminf(m[nt][e], m2[nt][e] - lv) + kRoom;
         }
       if (__any_sync(0xffffffffu, move)) {  // references move, to 2^8 below their columns' largest
@@ -684,8 +773,22 @@ q8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
           }
         }
       }
+      uint32_t vw[4][VW];
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        const uint32_t a = tile + v_off[h & 1] + (h >> 1) * 8 * HD;
+        if constexpr (VW == 4) {
+          const uint4 v = lds16(a);
+          vw[h][0] = v.x; vw[h][1] = v.y; vw[h][2] = v.z; vw[h][3] = v.w;
+        } else if constexpr (VW == 2) {
+          const uint2 v = lds8(a);
+          vw[h][0] = v.x; vw[h][1] = v.y;
+        } else {
+          vw[h][0] = lds4(a);
+        }
+      }
       // V of keys no column sees counts as 0, whatever its codes (an e4m3 NaN among them)
-      if (key0 + kQ8Block - 1 > pos_last) {
+      if (tail && key0 + kQ8Block - 1 > pos_last) {
         const int k0 = key0 + 2 * t4;
 #pragma unroll
         for (int h = 0; h < 4; ++h)
@@ -710,19 +813,22 @@ q8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         }
       }
       __syncwarp();  // every lane has read the tile: its slot may be asked for again
+      top_up();
     }
     if (!ok) break;
 
     const bool done = at.block + cur.cnt == at.blocks;
+    Place to = at;  // where the next window begins
+    if (nxt.cnt > 0) advance(to, cur.cnt);
     if (done || nxt.cnt == 0) {
       // The lane holds, of columns 2 t4 and 2 t4 + 1 of every n-tile, dims r8 * HD/8 .. + HD/8 - 1.
+      if (EARLY && nxt.cnt > 0) load_q(to, 0);  // (done: the next window begins another tile or head)
       const bool whole = i0 == 0 && done;
       const int64_t slot = 2 * (int64_t)w + (first ? 0 : 1);
       if (i0 == 0 && lane == 0) {
-        const int64_t last = (at.begin + at.blocks - 1) / cut.chunk;
         p.ws_pairs[(int64_t)at.tile * p.nkv + at.g] =
             whole ? make_int4(0, -1, 0, 0)  // nothing to join
-                  : make_int4(w, (int)last, at.u, at.j | (first ? 0x40000000 : 0));
+                  : make_int4(w, at.begin + at.blocks - 1, at.u, at.j | (first ? 0x40000000 : 0));
       }
       const int npad = p.compat_pad ? max(0, cut.max_ctx - (pos0 + 1)) : 0;
 #pragma unroll
@@ -746,8 +852,9 @@ q8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             v[2 * d + 1] = o[d][nt][2 + e] * f;
           }
           if (whole) {
-            T* dst = reinterpret_cast<T*>(p.out) + (int64_t)(at.unit.start + tok0 + c / rep) * p.ld_out +
-                     (int64_t)(at.g * rep + c % rep) * HD + r8 * (4 * VW);
+            const int tok = (int)(c * inv_rep >> 16);
+            T* dst = reinterpret_cast<T*>(p.out) + (int64_t)(at.unit.start + tok0 + tok) * p.ld_out +
+                     (int64_t)(at.g * rep + c - tok * rep) * HD + r8 * (4 * VW);
             if constexpr (sizeof(T) == 4) {
 #pragma unroll
               for (int d = 0; d < VW; ++d)
@@ -771,25 +878,33 @@ q8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       first = false;
       start = true;
     }
+    at = to;
     cur = nxt;
     sent = sent_nxt;
     sent_nxt = 0;
-    nxt = window_after(cur);
+    nxt.cnt = 0;
+    if (left > 0) {
+      advance(to, cur.cnt);
+      nxt = take(to);
+    }
+    top_up();
   }
   if (!ok) {
     // Copies still in flight (only after a wait ran out) land before the CTA exits.
     if (lane == 0) {
       raise_status(p.status, B2_DEV_PIPE_TIMEOUT);
-      for (int i = 0; i < n_open; ++i)
-        tc::mbar_wait(&full[warp][(n_used + i) % kStages], (uint32_t)((n_used + i) / kStages) & 1u, 100000000ull);
+      for (; n_open > 0; --n_open) {
+        tc::mbar_wait(&full[warp][at_slot], (uint32_t)at_phase, 100000000ull);
+        at_slot = at_slot == STAGES - 1 ? 0 : at_slot + 1;
+        at_phase ^= at_slot == 0;
+      }
     }
     __syncwarp();
   }
 }
 
-// Joins the pieces of the tiles that several warps worked on.  One CTA per (tile, kv head);
-// its warps share the columns, and the pieces of a column where there are fewer columns than
-// warps.
+// Joins the pieces of the tiles that several warps worked on.  A CTA takes one (tile, kv head), or
+// one of its columns where those are few; its warps share the pieces of a column.
 constexpr int kJoinWarps = 8;
 
 template <typename T, int HD>
@@ -799,12 +914,12 @@ __global__ void __launch_bounds__(kJoinWarps * 32) q8_join_kernel(Q8AttnParams p
   constexpr int E = HD / 32;  // dims per lane
   __shared__ float part[kJoinWarps][HD];
   __shared__ int most[kJoinWarps];
-  const int rep = p.nq / p.nkv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = blockIdx.y;
-  if ((int)blockIdx.x >= p.ws_tiles[0]) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = blockIdx.y;
   const int4 pair = p.ws_pairs[(int64_t)blockIdx.x * p.nkv + g];
-  if (pair.y < pair.x) return;  // one warp saw the whole tile
+  if ((int)blockIdx.x >= p.ws_tiles[0] || pair.y < 0) return;  // no such tile, or one warp saw all of it
+  const int rep = p.nq / p.nkv;
   const Unit u = unit_of(p, pair.z);
-  const int tok0 = (pair.w & 0x3fffffff) * qt, n = pair.y - pair.x + 1;
+  const int tok0 = (pair.w & 0x3fffffff) * qt, n = pair.y / p.ws_tiles[1] + 1;
   const int64_t slot0 = 2 * (int64_t)pair.x + (pair.w & 0x40000000 ? 0 : 1);
   const int ncol = min(qt, u.len - tok0) * rep;
   int npad = 0;
@@ -817,9 +932,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) q8_join_kernel(Q8AttnParams p
     for (int i = 0; i < kJoinWarps; ++i) mx = max(mx, most[i]);
     npad = max(0, mx - (u.ctx0 + 1));
   }
-  int share = 1;  // warps per column
-  while (share * 2 * ncol <= kJoinWarps) share *= 2;
-  for (int c0 = 0; c0 < ncol; c0 += kJoinWarps / share) {
+  // warps per column: all of them where a column's pieces are many
+  int share = 1;
+  while (share < kJoinWarps && share * 2 <= n) share *= 2;
+  for (int c0 = blockIdx.z * (kJoinWarps / share); c0 < ncol; c0 += gridDim.z * (kJoinWarps / share)) {
     const int c = c0 + warp / share, part_of = warp % share;
     float M = kNoRef, l = 0.f, acc[E];
 #pragma unroll
@@ -836,12 +952,23 @@ __global__ void __launch_bounds__(kJoinWarps * 32) q8_join_kernel(Q8AttnParams p
           f = exp2f(st.z - M);
         }
         const int most_k = min(32, n - k0);
-#pragma unroll 4
-        for (int i = part_of; i < most_k; i += share) {
-          const float fi = __shfl_sync(0xffffffffu, f, i);
-          const float* src = p.ws_o + where(k0 + i) * HD + lane * E;
+        for (int i0 = part_of; i0 < most_k; i0 += 4 * share) {  // four pieces in flight
+          float v[4][E];
 #pragma unroll
-          for (int e = 0; e < E; ++e) acc[e] = fmaf(src[e], fi, acc[e]);
+          for (int q = 0; q < 4; ++q) {
+            const int i = i0 + q * share;
+            const float* src = p.ws_o + where(k0 + min(i, most_k - 1)) * HD + lane * E;
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[q][e] = src[e];
+          }
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int i = i0 + q * share;
+            const float fi = __shfl_sync(0xffffffffu, f, i & 31);
+            if (i < most_k)
+#pragma unroll
+              for (int e = 0; e < E; ++e) acc[e] = fmaf(v[q][e], fi, acc[e]);
+          }
         }
       }
       l = warp_sum(l) + (npad > 0 ? (float)npad * exp2f(-M) : 0.f);
@@ -966,8 +1093,10 @@ int launch_tiles(const Q8AttnParams& p, const AttnPlan& a, cudaStream_t s) {
   if (rc) return rc;
   B2_TRY_CUDA(launch_pdl((q8_attn_kernel<T, HD, CODE, NT>), dim3(a.ctas), dim3(kWarps * 32), C::SMEM, s, mk, mv, p,
                          a.qt, a.units, a.per_group));
-  B2_TRY_CUDA(launch_pdl((q8_join_kernel<T, HD>), dim3((unsigned)a.tiles, p.nkv), dim3(kJoinWarps * 32), 0, s, p, a.qt,
-                         8 * a.nt));
+  // few tiles are cut into many pieces: a CTA per column then
+  const int by_column = a.tiles * p.nkv < sm_count() ? a.qt * (p.nq / p.nkv) : 1;
+  B2_TRY_CUDA(launch_pdl((q8_join_kernel<T, HD>), dim3((unsigned)a.tiles, p.nkv, by_column), dim3(kJoinWarps * 32), 0, s,
+                         p, a.qt, 8 * a.nt));
   return B2_OK;
 }
 
