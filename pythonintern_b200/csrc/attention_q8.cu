@@ -15,8 +15,8 @@
 // One step.  S^T[16 keys x 8 NT] = K Q^T and O^T[head_dim x 8 NT] += V^T P^T on
 // mma.sync.m16n8k16 with float16 operands and float32 sums.  A code of 8 bits is exact in
 // float16, so nothing is rounded on the way in.
-//  * The tiles of K and V (one block and kv head: 16 * head_dim bytes in one run) come by TMA into
-//    a ring of the warp's own, swizzled, two steps ahead and across the ends of tiles.
+//  * The tiles of K and V (one block and kv head: 16 * head_dim bytes in one run) come by cp.async
+//    into a three-stage ring of the warp's own, two steps ahead and across the ends of tiles.
 //  * K: lane (r, t) = (lane / 4, lane % 4) reads head_dim / 4 contiguous codes of keys r and
 //    r + 8.  The order of the head_dim axis inside the product is free, so its codes are taken
 //    as the k indexes of that lane and q is laid out to match.
@@ -32,8 +32,8 @@
 // References move only when a value would pass 2^15 and then to where it is 2^8, so the common
 // step needs no maximum across lanes, only one vote.
 #include "q8.cuh"
-#include "tc_ptx.cuh"
 
+#include <algorithm>
 #include <mutex>
 #include <set>
 #include <type_traits>
@@ -74,16 +74,17 @@ struct Q8AttnParams {
   int64_t ld_out;
   int32_t* status;
   // workspace
-  int* ws_tiles;    // [2]: tiles of the call, steps per warp
-  int4* ws_pairs;   // [tiles * nkv]: first warp, last step from the warp's first on, unit, tile in it
+  int4* ws_open;    // [CTAs]: the (tile, kv head) that begins in a CTA and ends in a later one: that
+                    // CTA (-1: there is none), unit, tile in it, kv head
+  int2* ws_piece;   // [CTAs]: slots of the CTA's piece of one that began before it, and of that one
   float4* ws_stat;  // [slots][columns]: m, l, m2
   float* ws_o;      // [slots][columns][head_dim]
 };
 
 
 // ------------------------------------------------------------------ the cut of the work
-constexpr int kWarps = 4;
 constexpr int kGroups = 256;   // prefix sums kept in shared memory
+constexpr int kMaxWarps = 16;  // of a CTA
 constexpr int kMinChunk = 2;   // steps a warp takes at least
 
 struct Unit {  // a decode row, or a sequence of a prefill
@@ -163,9 +164,9 @@ struct Line {
 
 // Prefix sums over groups of units.  Called by the whole CTA.
 __device__ Cut make_cut(const Q8AttnParams& p, int qt, int n_units, int per_group, Line& line, int warps, bool report) {
-  __shared__ int64_t w_steps[kWarps];
-  __shared__ int w_tiles[kWarps], w_ctx[kWarps];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = kWarps * 32;
+  __shared__ int64_t w_steps[kMaxWarps];
+  __shared__ int w_tiles[kMaxWarps], w_ctx[kMaxWarps];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x;
   const int groups = (n_units + per_group - 1) / per_group;
   const int per_thread = (groups + threads - 1) / threads;
   int64_t steps = 0;
@@ -208,8 +209,7 @@ __device__ Cut make_cut(const Q8AttnParams& p, int qt, int n_units, int per_grou
   Cut c{0, 0, 0, 0};
   int64_t base_s = inc_s - steps;
   int base_t = inc_t - tiles;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
+  for (int w = 0; w < threads / 32; ++w) {
     if (w < warp) {
       base_s += w_steps[w];
       base_t += w_tiles[w];
@@ -340,14 +340,12 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// The 16 rows of one (block, kv head) into shared memory, swizzled by the map.
-__device__ __forceinline__ void load_tile(void* dst, const CUtensorMap* map, uint64_t* bar, int row, int block) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::
-          "r"(tc::smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(tc::smem_u32(bar)), "r"(0), "r"(row), "r"(block)
-      : "memory");
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // Four elements of q, as they are in memory.
 template <typename T>
@@ -366,7 +364,17 @@ constexpr float kRoom = 15.f;       // log2 of the largest P
 constexpr float kLift = 8.f;        // log2 of the largest P when a reference has just moved
 constexpr float kNoRef = -1e30f;    // reference of a column that has seen no key
 
-constexpr int ctas_per_sm(int nt, int terms) { return nt * terms <= 2 ? 3 : 2; }
+// One CTA per SM.  Its warps are as many as their registers allow; a warp with few columns takes
+// two blocks at once.
+struct Shape {
+  int warps, stages, nb;
+};
+constexpr Shape shape_of(int hd, int nt, int terms) {
+  return nt * terms > 2    ? Shape{8, 3, 1}
+         : nt * terms == 2 ? Shape{12, 3, 1}
+         : hd == 128       ? Shape{12, 3, 1}
+                           : Shape{16, 3, 1};
+}
 
 template <typename T, int HD, int CODE, int NT>
 struct AttnCfg {
@@ -380,15 +388,19 @@ struct AttnCfg {
   static constexpr int VW = HD / 32;                     // and of a key's values
   static constexpr int TILE = kQ8Block * HD;             // bytes of codes of one block and head
   static constexpr int Q_BYTES = KW * NT * TERMS * 32 * 8;
-  // Tiles of K and V a warp holds or has in flight, and CTAs per SM that the registers are limited
-  // for and the shared memory holds.
-  static constexpr int STAGES = 3;
-  static constexpr int CTAS = ctas_per_sm(NT, TERMS);
+  static constexpr Shape SHAPE = shape_of(HD, NT, TERMS);
+  static constexpr int WARPS = SHAPE.warps;
+  static constexpr int STAGES = SHAPE.stages;            // tiles of K and V a warp holds or has in flight
+  static constexpr int NB = SHAPE.nb;                    // blocks it takes at once
   static constexpr int WARP_BYTES = STAGES * 2 * TILE;
-  // ring (1024-byte aligned for the swizzle), then the q fragments
-  static constexpr int SMEM = 1024 + kWarps * (WARP_BYTES + Q_BYTES);
+  // rings, then the q fragments
+  static constexpr int SMEM = WARPS * (WARP_BYTES + Q_BYTES);
+  static_assert(SMEM + (int)sizeof(Line) + 512 <= 232448, "shared memory above the 227 KB a CTA may use");
 };
 
+__device__ __forceinline__ uint32_t smem_u32(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
 __device__ __forceinline__ uint4 lds16(uint32_t a) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
@@ -405,13 +417,79 @@ __device__ __forceinline__ uint32_t lds4(uint32_t a) {
   return v;
 }
 
-// Byte offset of 16-byte chunk `chunk` of key row `row` in a tile that TMA has stored with the
-// swizzle as wide as a row (128, 64 or 32 bytes).
+// Byte offset of 16-byte chunk `chunk` of key row `row` in a tile in shared memory: chunks are
+// swapped by the row's place in 128 bytes, so that eight lanes reading a column of chunks, or a
+// row of them, touch different banks.
 template <int HD>
 __device__ __forceinline__ int tile_at(int row, int chunk) {
   constexpr int CHUNKS = HD / 16;
   return row * HD + ((chunk ^ (row * HD / 128 & (CHUNKS - 1))) << 4);
 }
+
+// A softmax in part: l = sum 2^(s - m), o = sum 2^(s - m2) vs v; a lane's HD / 32 dims.
+template <int HD>
+struct Piece {
+  float m, l, m2, o[HD / 32];
+};
+
+// Column c of n pieces in the workspace as one.  The warp's share of o: pieces part_of, part_of +
+// share, ...
+template <int HD, typename SlotOf>
+__device__ __forceinline__ Piece<HD> join_pieces(const Q8AttnParams& p, const SlotOf& slot_of, int n, int columns,
+                                                 int c, int part_of, int share, int lane) {
+  constexpr int E = HD / 32, BATCH = 4;  // pieces in flight
+  Piece<HD> r;
+  float v[BATCH][E], z[BATCH];
+  auto fetch = [&](int k) {
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) {
+      const int64_t at = (int64_t)slot_of(min(k + b * share, n - 1)) * columns + c;
+      z[b] = p.ws_stat[at].z;
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[b][e] = p.ws_o[at * HD + lane * E + e];
+    }
+  };
+  fetch(part_of);
+  float m = kNoRef, l = 0.f, m2 = kNoRef;
+  for (int k = lane; k < n; k += 32) {
+    const float4 st = p.ws_stat[(int64_t)slot_of(k) * columns + c];
+    const float mn = fmaxf(m, st.x);
+    l = l * exp2f(m - mn) + st.y * exp2f(st.x - mn);
+    m = mn;
+    m2 = fmaxf(m2, st.z);
+  }
+  r.m = warp_max(m);
+  r.m2 = warp_max(m2);
+  r.l = warp_sum(l * exp2f(m - r.m));
+#pragma unroll
+  for (int e = 0; e < E; ++e) r.o[e] = 0.f;
+  for (int k = part_of; k < n; k += BATCH * share) {
+    if (k != part_of) fetch(k);
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) {
+      const float f = k + b * share < n ? exp2f(z[b] - r.m2) : 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) r.o[e] = k + b * share < n ? fmaf(v[b][e], f, r.o[e]) : r.o[e];
+    }
+  }
+  return r;
+}
+
+// The result of one row and q head; npad keys of score 0 and value 0 join its denominator.
+template <typename T, int HD>
+__device__ __forceinline__ void write_head(const Q8AttnParams& p, int row, int head, int lane, const Piece<HD>& r,
+                                           int npad) {
+  constexpr int E = HD / 32;
+  const float l = npad > 0 ? r.l + (float)npad * exp2f(-r.m) : r.l;
+  const float f = r.m2 == kNoRef ? (l == l ? 0.f : l) : exp2f(r.m2 - r.m) / l;
+  T* dst = reinterpret_cast<T*>(p.out) + (int64_t)row * p.ld_out + (int64_t)head * HD + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; ++e) dst[e] = from_f32<T>(r.o[e] * f);
+}
+
+struct Join {
+  int warp, slot, pieces, whole, row, g, ncol, npad;
+};
 
 // Up to 32 consecutive steps of one (tile, kv head); lane i holds what step i needs.
 struct Window {
@@ -422,25 +500,23 @@ struct Window {
 };
 
 template <typename T, int HD, int CODE, int NT>
-__global__ void __launch_bounds__(kWarps * 32, (AttnCfg<T, HD, CODE, NT>::CTAS))
-q8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const Q8AttnParams p,
-               int qt, int n_units, int per_group) {
+__global__ void __launch_bounds__(AttnCfg<T, HD, CODE, NT>::WARPS * 32, 1)
+q8_attn_kernel(const Q8AttnParams p, int qt, int n_units, int per_group) {
   pdl_wait();
   pdl_trigger();
   using C = AttnCfg<T, HD, CODE, NT>;
-  constexpr int KW = C::KW, VW = C::VW, TERMS = C::TERMS, N = C::N, STAGES = C::STAGES;
+  constexpr int KW = C::KW, VW = C::VW, TERMS = C::TERMS, N = C::N, STAGES = C::STAGES, NB = C::NB, WARPS = C::WARPS;
   __shared__ Line line;
-  __shared__ __align__(8) uint64_t full[kWarps][STAGES];
-  extern __shared__ uint8_t smem_raw[];
+  __shared__ Join joins[WARPS];
+  __shared__ int n_joins;
+  extern __shared__ __align__(128) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int r8 = lane >> 2, t4 = lane & 3;
-  const int warps = gridDim.x * kWarps, w = blockIdx.x * kWarps + warp;
+  const int warps = gridDim.x * WARPS, w = blockIdx.x * WARPS + warp;
   const int rep = p.nq / p.nkv;
-  uint8_t* smem = smem_raw + ((1024 - (tc::smem_u32(smem_raw) & 1023)) & 1023);
-  uint8_t* ring = smem + warp * C::WARP_BYTES;
-  const uint32_t ring_at = tc::smem_u32(ring);
-  uint2* sq = reinterpret_cast<uint2*>(smem + kWarps * C::WARP_BYTES + warp * C::Q_BYTES) + lane;
-  const uint32_t sq_at = tc::smem_u32(sq);
+  const uint32_t ring_at = smem_u32(smem) + warp * C::WARP_BYTES;
+  uint2* sq = reinterpret_cast<uint2*>(smem + WARPS * C::WARP_BYTES + warp * C::Q_BYTES) + lane;
+  const uint32_t sq_at = smem_u32(sq);
   // what the lane reads of a tile: its codes of keys r8 (and, 8 rows on, r8 + 8), of keys 2 t4 and
   // 2 t4 + 1 (and 8 rows on)
   uint32_t k_off[KW == 8 ? 2 : 1], v_off[2];
@@ -453,18 +529,12 @@ q8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                           : VW == 2 ? tile_at<HD>(2 * t4 + h, r8 >> 1) + (r8 & 1) * 8
                                     : tile_at<HD>(2 * t4 + h, r8 >> 2) + (r8 & 3) * 4);
 
-  if (lane == 0) {
-    for (int i = 0; i < STAGES; ++i) tc::mbar_init(&full[warp][i], 1);
-    tc::fence_mbar_init();
-  }
   const Cut cut = make_cut(p, qt, n_units, per_group, line, warps, blockIdx.x == 0);
-  // a seq_start that goes back may name more tokens than there are rows (and tiles than the
-  // workspace has room for): nothing is computed
+  // a seq_start that goes back may name more tokens than there are rows: nothing is computed
   const bool sane = !p.seq_start || (int64_t)cut.tiles <= (int64_t)(p.n_rows / qt) + n_units;
-  if (w == 0 && lane == 0) {
-    p.ws_tiles[0] = sane ? cut.tiles : 0;
-    p.ws_tiles[1] = (int)cut.chunk;
-    if (!sane) raise_status(p.status, B2_DEV_RANGE);
+  if (threadIdx.x == 0) {
+    p.ws_open[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    if (!sane && blockIdx.x == 0) raise_status(p.status, B2_DEV_RANGE);
   }
   if (!sane) return;
   const int64_t x_begin = w * cut.chunk, x_end = min(cut.total, x_begin + cut.chunk);
@@ -475,9 +545,8 @@ q8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       for (int i = lane; i < p.nq * HD; i += 32) dst[i] = from_f32<T>(0.f);
     }
   }
-  if (x_begin >= x_end) return;
 
-  int left = (int)(x_end - x_begin);  // steps behind the windows taken so far
+  int left = (int)max((int64_t)0, x_end - x_begin);  // steps behind the windows taken so far
   // The window that begins at `from` (cnt 0 at the end of the chunk): starts the loads of its ids.
   auto take = [&](const Place& from) -> Window {
     Window win;
@@ -502,24 +571,29 @@ q8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     win.vs = __ldg(p.v_scale + at);
   };
 
-  int n_open = 0;                             // tiles in the ring or on their way
-  int at_slot = 0, at_phase = 0, to_slot = 0;  // next to consume (and its barrier's phase), next to ask for
+  // The copies of a step's tiles: every lane 16-byte pieces of K and of V, 512 bytes of the run
+  // with each; one commit group per step.  (TMA tile loads cost the warp 500 cycles a step to issue.)
+  int n_open = 0;                // tiles in the ring or on their way
+  int at_slot = 0, to_slot = 0;  // next to consume, next to ask for
+  constexpr int PIECES = HD / 32;
+  uint32_t to_off[PIECES];
+#pragma unroll
+  for (int c = 0; c < PIECES; ++c) to_off[c] = tile_at<HD>((lane + 32 * c) / (HD / 16), lane % (HD / 16));
   auto issue = [&](const Window& win, int i) {
-    const int slot = to_slot;
+    const uint32_t dst = ring_at + to_slot * (2 * C::TILE);
     to_slot = to_slot == STAGES - 1 ? 0 : to_slot + 1;
     const int id = __shfl_sync(0xffffffffu, win.id, i);
     ++n_open;
-    if (lane == 0) {
-      uint64_t* bar = &full[warp][slot];
-      if (id >= 0 && id < p.num_blocks) {
-        uint8_t* dst = ring + slot * 2 * C::TILE;
-        tc::mbar_arrive_expect_tx(bar, 2 * C::TILE);
-        load_tile(dst, &tmK, bar, win.g * kQ8Block, id);
-        load_tile(dst + C::TILE, &tmV, bar, win.g * kQ8Block, id);
-      } else {
-        tc::mbar_arrive(bar);  // nothing to wait for: the step is left out
+    if (id >= 0 && id < p.num_blocks) {  // else the step is left out
+      const int64_t at = ((int64_t)id * p.nkv + win.g) * C::TILE + lane * 16;
+      const uint8_t *ks = p.k_cache + at, *vs = p.v_cache + at;
+#pragma unroll
+      for (int c = 0; c < PIECES; ++c) {
+        cp_async16(dst + to_off[c], ks + c * 512);
+        cp_async16(dst + C::TILE + to_off[c], vs + c * 512);
       }
     }
+    cp_async_commit();
   };
 
   // q of a tile's columns.  Where they are few, the raw loads are made ahead, so that their latency
@@ -538,9 +612,10 @@ q8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     for (int k = 0; k < KW; ++k) raw[k] = reinterpret_cast<const Raw*>(src)[k];
   };
 
-  Place at = find_step(p, x_begin, qt, n_units, per_group, line);
+  Place at{};
+  if (left > 0) at = find_step(p, x_begin, qt, n_units, per_group, line);
   Window cur = take(at), nxt = cur;
-  if (EARLY) load_q(at, 0);
+  if (EARLY && cur.cnt > 0) load_q(at, 0);
   nxt.cnt = 0;
   if (left > 0) {
     Place to = at;
@@ -556,7 +631,7 @@ q8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     }
   };
   top_up();
-  scales_of(cur);
+  if (cur.cnt > 0) scales_of(cur);
 
   float colscale[NT][2], bias[NT][2];
   int lim[NT][2];  // last key of the lane's columns
@@ -564,7 +639,9 @@ q8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   float m[NT][2], m2[NT][2], lift[NT][2], l[NT][2];  // references, 2^(m - m2), sums
   int i0 = 0;          // first block of the current (tile, kv head) that this warp sees
   bool start = true;   // a (tile, kv head) begins with this window
-  bool first = true, ok = true;
+  bool first = true;   // nothing has been written out yet
+  bool open = false;   // the last tile went to the workspace in part
+  bool single = false;  // ... and it was the first
 
   while (cur.cnt > 0) {
     const int tok0 = at.j * qt, ntok = min(qt, at.unit.len - tok0);
@@ -644,98 +721,128 @@ q8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     }
     const int tail_from = (pos0 + 1) / kQ8Block - at.block;  // steps whose keys some column does not see
 
-    for (int i = 0; i < cur.cnt; ++i) {
+    for (int i = 0; i < cur.cnt; i += NB) {
       if (i == 0 && nxt.cnt > 0) scales_of(nxt);  // its ids were asked for a window ago
-      const int blk = __shfl_sync(0xffffffffu, cur.id, i);
-      const float ks = __shfl_sync(0xffffffffu, cur.ks, i), vs = __shfl_sync(0xffffffffu, cur.vs, i);
-      const int slot = at_slot;
-      if (!__all_sync(0xffffffffu, tc::mbar_wait(&full[warp][slot], (uint32_t)at_phase))) {
-        ok = false;
-        break;
+      // NB blocks at once, for the sake of independent work.  One behind the window's last or outside
+      // the pool is computed from what the ring holds and masked whole.
+      const int nb = min(NB, cur.cnt - i);
+      uint32_t tile[NB];
+      float ks[NB], vs[NB];
+      int key0[NB];
+      bool tail = false, any = false;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        tile[b] = ring_at + at_slot * (2 * C::TILE);
+        const bool live = b < nb && __shfl_sync(0xffffffffu, cur.id, (i + b) & 31) >= 0;
+        ks[b] = __shfl_sync(0xffffffffu, cur.ks, (i + b) & 31);
+        vs[b] = live ? __shfl_sync(0xffffffffu, cur.vs, (i + b) & 31) : 0.f;
+        key0[b] = live ? (at.block + i + b) * kQ8Block : 0x40000000;
+        tail |= !live || i + b >= tail_from;
+        any |= live;
+        if (b < nb) at_slot = at_slot == STAGES - 1 ? 0 : at_slot + 1;
       }
-      at_slot = slot == STAGES - 1 ? 0 : slot + 1;
-      at_phase ^= slot == STAGES - 1;
-      --n_open;
-      if (blk < 0) {  // a block outside the pool: its keys are left out
+      n_open -= nb;  // as many groups were committed behind these steps'
+      static_assert(STAGES <= 4, "the waits below");
+      if (n_open >= 3) cp_async_wait<3>();
+      else if (n_open == 2) cp_async_wait<2>();
+      else if (n_open == 1) cp_async_wait<1>();
+      else cp_async_wait<0>();
+      __syncwarp();
+      if (!any) {
         top_up();
         continue;
       }
-      const uint32_t tile = ring_at + slot * (2 * C::TILE);
-      float s[NT][4], s_odd[NT == 1 ? 1 : NT][4];  // two chains of products where there are few columns
+      float s[NB][NT][4], s_odd[NT == 1 ? NB : 1][NT == 1 ? 1 : NT][4];  // two chains of products where columns are few
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[nt][e] = s_odd[nt][e] = 0.f;
-      uint32_t kw[2][KW];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {  // rows eight apart have the same swizzle
-        if constexpr (KW == 2) {
-          const uint2 v = lds8(tile + k_off[0] + h * 8 * HD);
-          kw[h][0] = v.x; kw[h][1] = v.y;
-        } else {
-#pragma unroll
-          for (int k = 0; k < KW; k += 4) {
-            const uint4 v = lds16(tile + k_off[k / 4] + h * 8 * HD);
-            kw[h][k] = v.x; kw[h][k + 1] = v.y; kw[h][k + 2] = v.z; kw[h][k + 3] = v.w;
-          }
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < KW; ++k) {
-        uint32_t a[4];
-        expand<CODE, C::BIASED>(kw[0][k], a[0], a[2]);
-        expand<CODE, C::BIASED>(kw[1][k], a[1], a[3]);
+      for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int term = 0; term < TERMS; ++term) {
-            const uint2 b = lds8(sq_at + ((k * NT + nt) * TERMS + term) * 32 * 8);
-            mma_f16(NT == 1 && (k & 1) ? s_odd[nt] : s[nt], a, b.x, b.y);
+          for (int e = 0; e < 4; ++e) s[b][nt][e] = s_odd[NT == 1 ? b : 0][nt][e] = 0.f;
+      uint32_t kw[NB][2][KW];
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {  // rows eight apart have the same swizzle
+          if constexpr (KW == 2) {
+            const uint2 v = lds8(tile[b] + k_off[0] + h * 8 * HD);
+            kw[b][h][0] = v.x; kw[b][h][1] = v.y;
+          } else {
+#pragma unroll
+            for (int k = 0; k < KW; k += 4) {
+              const uint4 v = lds16(tile[b] + k_off[k / 4] + h * 8 * HD);
+              kw[b][h][k] = v.x; kw[b][h][k + 1] = v.y; kw[b][h][k + 2] = v.z; kw[b][h][k + 3] = v.w;
+            }
           }
+        }
+#pragma unroll
+      for (int k = 0; k < KW; ++k) {
+        uint2 qf[NT][TERMS];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int term = 0; term < TERMS; ++term) qf[nt][term] = lds8(sq_at + ((k * NT + nt) * TERMS + term) * 32 * 8);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          uint32_t a[4];
+          expand<CODE, C::BIASED>(kw[b][0][k], a[0], a[2]);
+          expand<CODE, C::BIASED>(kw[b][1][k], a[1], a[3]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int term = 0; term < TERMS; ++term)
+              mma_f16(NT == 1 && (k & 1) ? s_odd[NT == 1 ? b : 0][nt] : s[b][nt], a, qf[nt][term].x, qf[nt][term].y);
+        }
       }
       if constexpr (NT == 1) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[0][e] += s_odd[0][e];
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[b][0][e] += s_odd[b][0][e];
       }
       // scores; the tail of the tile's keys is masked per column
-      const int key0 = (at.block + i) * kQ8Block, key = key0 + r8;
-      const bool tail = i >= tail_from;
       if (tail) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              if (key0[b] + r8 > lim[nt][e]) s[b][nt][e] = -INFINITY;
+              if (key0[b] + r8 + 8 > lim[nt][e]) s[b][nt][2 + e] = -INFINITY;
+            }
+      }
+      float lv[NB];
+      bool move = false;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        lv[b] = vs[b] == 0.f ? -INFINITY : __log2f(vs[b]);  // only places a reference: approximate
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            if (key > lim[nt][e]) s[nt][e] = -INFINITY;
-            if (key + 8 > lim[nt][e]) s[nt][2 + e] = -INFINITY;
+            // a column that sees none of the block's keys takes nothing from its scales
+            const float cs = tail && key0[b] > lim[nt][e] ? 1.f : colscale[nt][e] * ks[b];
+            const float c0 = C::BIASED ? bias[nt][e] * cs : 0.f;
+            s[b][nt][e] = fmaf(s[b][nt][e], cs, c0);
+            s[b][nt][2 + e] = fmaf(s[b][nt][2 + e], cs, c0);
+            move |= fmaxf(s[b][nt][e], s[b][nt][2 + e]) > fminf(m[nt][e], m2[nt][e] - lv[b]) + kRoom;
           }
       }
-      const float lv = vs == 0.f ? -INFINITY : __log2f(vs);  // only places a reference: approximate
-      bool move = false;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          // a column that sees none of the block's keys takes nothing from its scales
-          const float cs = tail && key0 > lim[nt][e] ? 1.f : colscale[nt][e] * ks;
-          if (C::BIASED) {
-            const float b = bias[nt][e] * cs;
-            s[nt][e] = fmaf(s[nt][e], cs, b);
-            s[nt][2 + e] = fmaf(s[nt][2 + e], cs, b);
-          } else {
-            s[nt][e] *= cs;
-            s[nt][2 + e] *= cs;
-          }
-          move |= fmaxf(s[nt][e], s[nt][2 + e]) > fminf(m[nt][e], m2[nt][e] - lv) + kRoom;
-        }
       if (__any_sync(0xffffffffu, move)) {  // references move, to 2^8 below their columns' largest
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float mx = fmaxf(s[nt][e], s[nt][2 + e]);
+            float mn = m[nt][e], m2n = m2[nt][e];
 #pragma unroll
-            for (int sh = 4; sh < 32; sh <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, sh));
-            const float mn = fmaxf(m[nt][e], mx - kLift), m2n = fmaxf(m2[nt][e], mx - kLift + lv);
+            for (int b = 0; b < NB; ++b) {
+              float mx = fmaxf(s[b][nt][e], s[b][nt][2 + e]);
+#pragma unroll
+              for (int sh = 4; sh < 32; sh <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, sh));
+              mn = fmaxf(mn, mx - kLift);
+              m2n = fmaxf(m2n, mx - kLift + lv[b]);
+            }
             l[nt][e] *= ex2(m[nt][e] - mn);
             const float c = ex2(m2[nt][e] - m2n);
             m[nt][e] = mn;
@@ -748,75 +855,78 @@ q8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             }
           }
       }
-      uint32_t pb[NT][TERMS][2];
+      uint32_t pb[NB][NT][TERMS][2];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float pa[2], pc[2];
+      for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          pa[e] = ex2(s[nt][e] - m[nt][e]);  // -inf gives 0
-          pc[e] = ex2(s[nt][2 + e] - m[nt][e]);
-          l[nt][e] += pa[e] + pc[e];
-          const float f = tail && key0 > lim[nt][e] ? 0.f : vs == 0.f ? 0.f : vs * lift[nt][e];
-          pa[e] *= f;
-          pc[e] *= f;
+        for (int nt = 0; nt < NT; ++nt) {
+          float pa[2], pc[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            pa[e] = ex2(s[b][nt][e] - m[nt][e]);  // -inf gives 0
+            pc[e] = ex2(s[b][nt][2 + e] - m[nt][e]);
+            l[nt][e] += pa[e] + pc[e];
+            const float f = vs[b] == 0.f || (tail && key0[b] > lim[nt][e]) ? 0.f : vs[b] * lift[nt][e];
+            pa[e] *= f;
+            pc[e] *= f;
+          }
+#pragma unroll
+          for (int term = 0; term < TERMS; ++term) {
+            const uint32_t lo = pack_f16(pa[0], pa[1]), hi = pack_f16(pc[0], pc[1]);
+            pb[b][nt][term][0] = transpose8x8(lo);
+            pb[b][nt][term][1] = transpose8x8(hi);
+            if (TERMS == 2) {
+              const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+              const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+              pa[0] -= fa.x; pa[1] -= fa.y; pc[0] -= fb.x; pc[1] -= fb.y;
+            }
+          }
         }
 #pragma unroll
-        for (int term = 0; term < TERMS; ++term) {
-          const uint32_t lo = pack_f16(pa[0], pa[1]), hi = pack_f16(pc[0], pc[1]);
-          pb[nt][term][0] = transpose8x8(lo);
-          pb[nt][term][1] = transpose8x8(hi);
-          if (TERMS == 2) {
-            const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&lo));
-            const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-            pa[0] -= fa.x; pa[1] -= fa.y; pc[0] -= fb.x; pc[1] -= fb.y;
+      for (int b = 0; b < NB; ++b) {
+        uint32_t vw[4][VW];
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const uint32_t a = tile[b] + v_off[h & 1] + (h >> 1) * 8 * HD;
+          if constexpr (VW == 4) {
+            const uint4 v = lds16(a);
+            vw[h][0] = v.x; vw[h][1] = v.y; vw[h][2] = v.z; vw[h][3] = v.w;
+          } else if constexpr (VW == 2) {
+            const uint2 v = lds8(a);
+            vw[h][0] = v.x; vw[h][1] = v.y;
+          } else {
+            vw[h][0] = lds4(a);
+          }
+        }
+        // V of keys no column sees counts as 0, whatever its codes (an e4m3 NaN among them)
+        if (tail && key0[b] + kQ8Block - 1 > pos_last) {
+          const int k0 = key0[b] + 2 * t4;
+#pragma unroll
+          for (int h = 0; h < 4; ++h)
+            if (k0 + (h & 1) + (h >> 1) * 8 > pos_last) {
+#pragma unroll
+              for (int v = 0; v < VW; ++v) vw[h][v] = 0u;
+            }
+        }
+#pragma unroll
+        for (int v = 0; v < VW; ++v) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t sel = half ? 0x7362 : 0x5140;
+            uint32_t a[4];
+            expand<CODE>(prmt(vw[0][v], vw[1][v], sel), a[0], a[1]);
+            expand<CODE>(prmt(vw[2][v], vw[3][v], sel), a[2], a[3]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int term = 0; term < TERMS; ++term)
+                mma_f16(o[2 * v + half][nt], a, pb[b][nt][term][0], pb[b][nt][term][1]);
           }
         }
       }
-      uint32_t vw[4][VW];
-#pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        const uint32_t a = tile + v_off[h & 1] + (h >> 1) * 8 * HD;
-        if constexpr (VW == 4) {
-          const uint4 v = lds16(a);
-          vw[h][0] = v.x; vw[h][1] = v.y; vw[h][2] = v.z; vw[h][3] = v.w;
-        } else if constexpr (VW == 2) {
-          const uint2 v = lds8(a);
-          vw[h][0] = v.x; vw[h][1] = v.y;
-        } else {
-          vw[h][0] = lds4(a);
-        }
-      }
-      // V of keys no column sees counts as 0, whatever its codes (an e4m3 NaN among them)
-      if (tail && key0 + kQ8Block - 1 > pos_last) {
-        const int k0 = key0 + 2 * t4;
-#pragma unroll
-        for (int h = 0; h < 4; ++h)
-          if (k0 + (h & 1) + (h >> 1) * 8 > pos_last) {
-#pragma unroll
-            for (int v = 0; v < VW; ++v) vw[h][v] = 0u;
-          }
-      }
-#pragma unroll
-      for (int v = 0; v < VW; ++v) {
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint32_t sel = half ? 0x7362 : 0x5140;
-          uint32_t a[4];
-          expand<CODE>(prmt(vw[0][v], vw[1][v], sel), a[0], a[1]);
-          expand<CODE>(prmt(vw[2][v], vw[3][v], sel), a[2], a[3]);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int term = 0; term < TERMS; ++term)
-              mma_f16(o[2 * v + half][nt], a, pb[nt][term][0], pb[nt][term][1]);
-        }
-      }
-      __syncwarp();  // every lane has read the tile: its slot may be asked for again
+      __syncwarp();  // every lane has read the tiles: their slots may be asked for again
       top_up();
     }
-    if (!ok) break;
-
     const bool done = at.block + cur.cnt == at.blocks;
     Place to = at;  // where the next window begins
     if (nxt.cnt > 0) advance(to, cur.cnt);
@@ -825,11 +935,9 @@ q8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       if (EARLY && nxt.cnt > 0) load_q(to, 0);  // (done: the next window begins another tile or head)
       const bool whole = i0 == 0 && done;
       const int64_t slot = 2 * (int64_t)w + (first ? 0 : 1);
-      if (i0 == 0 && lane == 0) {
-        p.ws_pairs[(int64_t)at.tile * p.nkv + at.g] =
-            whole ? make_int4(0, -1, 0, 0)  // nothing to join
-                  : make_int4(w, at.begin + at.blocks - 1, at.u, at.j | (first ? 0x40000000 : 0));
-      }
+      if (first && i0 > 0 && warp == 0 && lane == 0) p.ws_piece[blockIdx.x].x = (int)slot;
+      open = !whole && nxt.cnt == 0;
+      single = first;
       const int npad = p.compat_pad ? max(0, cut.max_ctx - (pos0 + 1)) : 0;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -878,6 +986,7 @@ q8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       first = false;
       start = true;
     }
+    if (nxt.cnt == 0) break;  // `at` stays the last tile's
     at = to;
     cur = nxt;
     sent = sent_nxt;
@@ -889,39 +998,70 @@ q8_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     }
     top_up();
   }
-  if (!ok) {
-    // Copies still in flight (only after a wait ran out) land before the CTA exits.
+
+  // Pieces of one (tile, kv head) within the CTA are joined here: into the output, or, where other
+  // CTAs have some too, into the slot of the first.  Every warp whose last tile stays open and
+  // that is the first of the CTA to have a piece of it says so; then the warps share the columns.
+  if (threadIdx.x == 0) n_joins = 0;
+  __syncthreads();
+  if (open && (i0 == 0 || warp == 0)) {
+    const int slot = 2 * w + (single ? 0 : 1);
+    const int last_w = w + (at.begin + at.blocks - 1) / (int)cut.chunk, cta_last = blockIdx.x * WARPS + WARPS - 1;
+    const bool whole = i0 == 0 && last_w <= cta_last;
     if (lane == 0) {
-      raise_status(p.status, B2_DEV_PIPE_TIMEOUT);
-      for (; n_open > 0; --n_open) {
-        tc::mbar_wait(&full[warp][at_slot], (uint32_t)at_phase, 100000000ull);
-        at_slot = at_slot == STAGES - 1 ? 0 : at_slot + 1;
-        at_phase ^= at_slot == 0;
+      if (!whole && i0 == 0) {
+        p.ws_open[blockIdx.x] = make_int4(last_w / WARPS, at.u, at.j, at.g);
+        p.ws_piece[blockIdx.x].y = slot;
+      } else if (!whole) {
+        p.ws_piece[blockIdx.x].x = slot;
+      }
+      const int pieces = min(last_w, cta_last) - w + 1, tok0 = at.j * qt;
+      if (pieces > 1)
+        joins[atomicAdd(&n_joins, 1)] =
+            Join{w, slot, pieces, whole, at.unit.start + tok0, at.g, min(qt, at.unit.len - tok0) * rep,
+                 p.compat_pad ? max(0, cut.max_ctx - (at.unit.ctx0 + tok0 + 1)) : 0};
+    }
+  }
+  __syncthreads();
+  int before = 0;
+  for (int k = 0; k < n_joins; ++k) {
+    const Join jn = joins[k];
+    // columns are dealt to the warps in turn
+    for (int c = (warp + WARPS - before % WARPS) % WARPS; c < jn.ncol; c += WARPS) {
+      const auto slot_of = [&](int q) { return q == 0 ? jn.slot : 2 * (jn.warp + q); };
+      const Piece<HD> r = join_pieces<HD>(p, slot_of, jn.pieces, N, c, 0, 1, lane);
+      if (jn.whole) {
+        const int tok = (int)(c * inv_rep >> 16);
+        write_head<T, HD>(p, jn.row + tok, jn.g * rep + c - tok * rep, lane, r, jn.npad);
+      } else {  // every lane has read what it replaces
+        const int64_t to = (int64_t)jn.slot * N + c;
+        if (lane == 0) p.ws_stat[to] = make_float4(r.m, r.l, r.m2, 0.f);
+        float* dst = p.ws_o + to * HD + lane * (HD / 32);
+#pragma unroll
+        for (int e = 0; e < HD / 32; ++e) dst[e] = r.o[e];
       }
     }
-    __syncwarp();
+    before += jn.ncol;
   }
 }
 
-// Joins the pieces of the tiles that several warps worked on.  A CTA takes one (tile, kv head), or
-// one of its columns where those are few; its warps share the pieces of a column.
+// Joins the pieces of the tiles that reach over several CTAs: block x takes the one that begins in
+// CTA x of the kernel above, its columns z, z + gridDim.z, ...; the warps share columns and pieces.
 constexpr int kJoinWarps = 8;
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(kJoinWarps * 32) q8_join_kernel(Q8AttnParams p, int qt, int columns) {
   pdl_wait();
   pdl_trigger();
-  constexpr int E = HD / 32;  // dims per lane
+  constexpr int E = HD / 32;
   __shared__ float part[kJoinWarps][HD];
   __shared__ int most[kJoinWarps];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = blockIdx.y;
-  const int4 pair = p.ws_pairs[(int64_t)blockIdx.x * p.nkv + g];
-  if ((int)blockIdx.x >= p.ws_tiles[0] || pair.y < 0) return;  // no such tile, or one warp saw all of it
-  const int rep = p.nq / p.nkv;
-  const Unit u = unit_of(p, pair.z);
-  const int tok0 = (pair.w & 0x3fffffff) * qt, n = pair.y / p.ws_tiles[1] + 1;
-  const int64_t slot0 = 2 * (int64_t)pair.x + (pair.w & 0x40000000 ? 0 : 1);
-  const int ncol = min(qt, u.len - tok0) * rep;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cta = blockIdx.x;
+  const int4 open = p.ws_open[cta];
+  if (open.x < 0) return;
+  const int rep = p.nq / p.nkv, n = open.x - cta + 1;
+  const Unit u = unit_of(p, open.y);
+  const int tok0 = open.z * qt, ncol = min(qt, u.len - tok0) * rep;
   int npad = 0;
   if (p.compat_pad) {
     int mx = 0;
@@ -932,63 +1072,27 @@ __global__ void __launch_bounds__(kJoinWarps * 32) q8_join_kernel(Q8AttnParams p
     for (int i = 0; i < kJoinWarps; ++i) mx = max(mx, most[i]);
     npad = max(0, mx - (u.ctx0 + 1));
   }
-  // warps per column: all of them where a column's pieces are many
-  int share = 1;
-  while (share < kJoinWarps && share * 2 <= n) share *= 2;
-  for (int c0 = blockIdx.z * (kJoinWarps / share); c0 < ncol; c0 += gridDim.z * (kJoinWarps / share)) {
-    const int c = c0 + warp / share, part_of = warp % share;
-    float M = kNoRef, l = 0.f, acc[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    auto where = [&](int k) { return (k == 0 ? slot0 : 2 * (int64_t)(pair.x + k)) * columns + c; };
-    if (c < ncol) {
-      for (int k = lane; k < n; k += 32) M = fmaxf(M, p.ws_stat[where(k)].x);
-      M = warp_max(M);
-      for (int k0 = 0; k0 < n; k0 += 32) {
-        float f = 0.f;
-        if (k0 + lane < n) {
-          const float4 st = p.ws_stat[where(k0 + lane)];
-          l = fmaf(st.y, exp2f(st.x - M), l);
-          f = exp2f(st.z - M);
-        }
-        const int most_k = min(32, n - k0);
-        for (int i0 = part_of; i0 < most_k; i0 += 4 * share) {  // four pieces in flight
-          float v[4][E];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int i = i0 + q * share;
-            const float* src = p.ws_o + where(k0 + min(i, most_k - 1)) * HD + lane * E;
-#pragma unroll
-            for (int e = 0; e < E; ++e) v[q][e] = src[e];
-          }
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int i = i0 + q * share;
-            const float fi = __shfl_sync(0xffffffffu, f, i & 31);
-            if (i < most_k)
-#pragma unroll
-              for (int e = 0; e < E; ++e) acc[e] = fmaf(v[q][e], fi, acc[e]);
-          }
-        }
-      }
-      l = warp_sum(l) + (npad > 0 ? (float)npad * exp2f(-M) : 0.f);
-    }
+  const int here = (ncol - (int)blockIdx.z + (int)gridDim.z - 1) / (int)gridDim.z;  // columns of this block
+  int share = 1;                                                                    // warps per column
+  while (share * 2 * here <= kJoinWarps && share < n) share *= 2;
+  const auto slot_of = [&](int q) { return q == 0 ? p.ws_piece[cta].y : p.ws_piece[cta + q].x; };
+  for (int i0 = 0; i0 < here; i0 += kJoinWarps / share) {
+    const int i = i0 + warp / share, c = blockIdx.z + i * gridDim.z, part_of = warp % share;
+    const bool live = i < here;
+    Piece<HD> r;
+    if (live) r = join_pieces<HD>(p, slot_of, n, columns, c, part_of, share, lane);
     if (share > 1) {
       __syncthreads();
+      if (live)
 #pragma unroll
-      for (int e = 0; e < E; ++e) part[warp][lane * E + e] = acc[e];
+        for (int e = 0; e < E; ++e) part[warp][lane * E + e] = r.o[e];
       __syncthreads();
-      if (part_of == 0)
+      if (live && part_of == 0)
         for (int w = 1; w < share; ++w)
 #pragma unroll
-          for (int e = 0; e < E; ++e) acc[e] += part[warp + w][lane * E + e];
+          for (int e = 0; e < E; ++e) r.o[e] += part[warp + w][lane * E + e];
     }
-    if (c < ncol && part_of == 0) {
-      T* dst = reinterpret_cast<T*>(p.out) + (int64_t)(u.start + tok0 + c / rep) * p.ld_out +
-               (int64_t)(g * rep + c % rep) * HD + lane * E;
-#pragma unroll
-      for (int e = 0; e < E; ++e) dst[e] = from_f32<T>(l == 0.f ? 0.f : acc[e] / l);
-    }
+    if (live && part_of == 0) write_head<T, HD>(p, u.start + tok0 + c / rep, open.w * rep + c % rep, lane, r, npad);
   }
 }
 
@@ -1027,8 +1131,7 @@ size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 struct AttnPlan {
   int nt, qt, units, per_group, ctas, slots;
-  int64_t tiles;  // at most
-  size_t pairs, stat, o, total;  // workspace offsets
+  size_t piece, stat, o, total;  // workspace offsets
 };
 
 // Columns of a tile.  A decode row has rep columns.  A sequence of a prefill has tokens * rep;
@@ -1042,32 +1145,13 @@ AttnPlan plan_of(int n_rows, int nq, int nkv, int hd, int n_seqs, bool prefill, 
   a.qt = prefill ? 8 * a.nt / rep : 1;
   a.units = prefill ? n_seqs : n_rows;
   a.per_group = (a.units + kGroups - 1) / kGroups;
-  a.ctas = sm_count() * ctas_per_sm(a.nt, terms);
-  a.slots = 2 * a.ctas * kWarps;
-  a.tiles = prefill ? (int64_t)n_rows / a.qt + n_seqs : n_rows;
-  a.pairs = 256;
-  a.stat = a.pairs + align256((size_t)a.tiles * nkv * sizeof(int4));
+  a.ctas = sm_count();
+  a.slots = 2 * a.ctas * shape_of(hd, a.nt, terms).warps;
+  a.piece = align256((size_t)a.ctas * sizeof(int4));
+  a.stat = a.piece + align256((size_t)a.ctas * sizeof(int2));
   a.o = a.stat + align256((size_t)a.slots * 8 * a.nt * sizeof(float4));
   a.total = a.o + (size_t)a.slots * 8 * a.nt * hd * sizeof(float);
   return a;
-}
-
-// One layer's cache as [blocks][kv heads * 16 tokens][head_dim] bytes, in boxes of one (block, kv
-// head), swizzled as wide as a row.
-int encode_cache(CUtensorMap* m, const void* cache, int num_blocks, int nkv, int hd) {
-  auto fn = tc::encode_fn();
-  if (!fn) return fail(B2_ECUDA, "cuTensorMapEncodeTiled unavailable");
-  const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)nkv * kQ8Block, (cuuint64_t)num_blocks};
-  const cuuint64_t strides[2] = {(cuuint64_t)hd, (cuuint64_t)nkv * kQ8Block * hd};
-  const cuuint32_t box[3] = {(cuuint32_t)hd, kQ8Block, 1}, es[3] = {1, 1, 1};
-  const CUtensorMapSwizzle swizzle = hd == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
-                                     : hd == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
-                                                : CU_TENSOR_MAP_SWIZZLE_32B;
-  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(cache), dims, strides, box, es,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(B2_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
-  return B2_OK;
 }
 
 // Opts a kernel into `bytes` of dynamic shared memory once per (kernel, device).
@@ -1086,17 +1170,12 @@ int allow_smem(const void* fn, size_t bytes) {
 template <typename T, int HD, int CODE, int NT>
 int launch_tiles(const Q8AttnParams& p, const AttnPlan& a, cudaStream_t s) {
   using C = AttnCfg<T, HD, CODE, NT>;
-  CUtensorMap mk, mv;
-  int rc = encode_cache(&mk, p.k_cache, p.num_blocks, p.nkv, HD);
-  if (rc == B2_OK) rc = encode_cache(&mv, p.v_cache, p.num_blocks, p.nkv, HD);
-  if (rc == B2_OK) rc = allow_smem((const void*)q8_attn_kernel<T, HD, CODE, NT>, C::SMEM);
+  const int rc = allow_smem((const void*)q8_attn_kernel<T, HD, CODE, NT>, C::SMEM);
   if (rc) return rc;
-  B2_TRY_CUDA(launch_pdl((q8_attn_kernel<T, HD, CODE, NT>), dim3(a.ctas), dim3(kWarps * 32), C::SMEM, s, mk, mv, p,
-                         a.qt, a.units, a.per_group));
-  // few tiles are cut into many pieces: a CTA per column then
-  const int by_column = a.tiles * p.nkv < sm_count() ? a.qt * (p.nq / p.nkv) : 1;
-  B2_TRY_CUDA(launch_pdl((q8_join_kernel<T, HD>), dim3((unsigned)a.tiles, p.nkv, by_column), dim3(kJoinWarps * 32), 0, s,
-                         p, a.qt, 8 * a.nt));
+  B2_TRY_CUDA(launch_pdl((q8_attn_kernel<T, HD, CODE, NT>), dim3(a.ctas), dim3(C::WARPS * 32), C::SMEM, s, p, a.qt,
+                         a.units, a.per_group));
+  B2_TRY_CUDA(launch_pdl((q8_join_kernel<T, HD>), dim3(a.ctas, 1, std::min(4, a.qt * (p.nq / p.nkv))),
+                         dim3(kJoinWarps * 32), 0, s, p, a.qt, 8 * a.nt));
   return B2_OK;
 }
 
@@ -1123,12 +1202,11 @@ int launch_hd(const Q8AttnParams& p, int hd, int code, const AttnPlan& a, cudaSt
 int launch(const char* name, Q8AttnParams& p, int hd, int cache_dtype, int dtype, void* workspace, size_t bytes,
            cudaStream_t s) {
   const AttnPlan a = plan_of(p.n_rows, p.nq, p.nkv, hd, p.n_seqs, p.seq_start != nullptr, dtype);
-  B2_CHECK_ARG(a.tiles <= 0x7fffffff && p.nkv <= 65535, "%s: too many tiles or kv heads", name);
   B2_CHECK_ARG(workspace && bytes >= a.total, "%s: workspace of %zu bytes needed, %zu given", name, a.total, bytes);
   B2_CHECK_ARG(((uintptr_t)workspace % 16) == 0, "%s: the workspace must be 16-byte aligned", name);
   char* ws = static_cast<char*>(workspace);
-  p.ws_tiles = reinterpret_cast<int*>(ws);
-  p.ws_pairs = reinterpret_cast<int4*>(ws + a.pairs);
+  p.ws_open = reinterpret_cast<int4*>(ws);
+  p.ws_piece = reinterpret_cast<int2*>(ws + a.piece);
   p.ws_stat = reinterpret_cast<float4*>(ws + a.stat);
   p.ws_o = reinterpret_cast<float*>(ws + a.o);
   return dtype == B2_BF16 ? launch_hd<__nv_bfloat16>(p, hd, cache_dtype, a, s)
