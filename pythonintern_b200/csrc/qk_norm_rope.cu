@@ -43,7 +43,9 @@ struct NormRopeParams {
   void* v_cache;
   float* k_scale;
   float* v_scale;
-  int chunk;  // tokens whose runs one block of the tile kernel looks for
+  int heads;        // heads a lane group takes of its token
+  int chunk;        // tokens whose runs a tile block looks for, at most 16
+  int tile_blocks;  // blocks that write tiles, before those of the q heads
   int32_t* status;
 };
 
@@ -69,42 +71,46 @@ __device__ __forceinline__ void st8(__nv_bfloat16* p, const float (&v)[8]) {
   *reinterpret_cast<uint4*>(p) = o;
 }
 
-// Norm (weight not null) and rotation of one head held by a group of LANES lanes.
+// What a lane needs of the tables for one token: cos and sin of its 8 elements of either half.
+struct Angles {
+  float cl[8], sl[8], ch[8], sh[8];
+};
+template <int HD>
+__device__ __forceinline__ void load_angles(const NormRopeParams& p, int64_t rope, int li, Angles& a) {
+  const float *c = p.cos + rope * HD + li * 8, *s = p.sin + rope * HD + li * 8;
+  ld8(c, a.cl);
+  ld8(s, a.sl);
+  ld8(c + HD / 2, a.ch);
+  ld8(s + HD / 2, a.sh);
+}
+
+// Norm (if `norm`; w: the lane's weights) and rotation of one head held by a group of LANES lanes.
 template <int LANES>
-__device__ __forceinline__ void norm_rotate(float (&lo)[8], float (&hi)[8], const float* weight, float eps,
-                                            const float* cos, const float* sin, int li) {
-  constexpr int HALF = LANES * 8;
-  if (weight) {
+__device__ __forceinline__ void norm_rotate(float (&lo)[8], float (&hi)[8], bool norm, const float (&wl)[8],
+                                            const float (&wh)[8], float eps, const Angles& a) {
+  if (norm) {
     // the other groups of the warp may hold value heads, which do not come here
-    const unsigned group = (LANES == 32 ? 0xffffffffu : (1u << LANES) - 1) << (threadIdx.x % 32 / LANES * LANES);
+    const unsigned group = ((1u << LANES) - 1) << (threadIdx.x % 32 / LANES * LANES);
     float ss = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) ss = fmaf(lo[e], lo[e], fmaf(hi[e], hi[e], ss));
 #pragma unroll
     for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(group, ss, o);
-    const float r = rsqrtf(ss * (1.f / (2 * HALF)) + eps);
-    float wl[8], wh[8];
-    ld8(weight + li * 8, wl);
-    ld8(weight + HALF + li * 8, wh);
+    const float r = rsqrtf(ss * (1.f / (16 * LANES)) + eps);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       lo[e] = lo[e] * r * wl[e];
       hi[e] = hi[e] * r * wh[e];
     }
   }
-  float cl[8], sl[8], ch[8], sh[8];
-  ld8(cos + li * 8, cl);
-  ld8(sin + li * 8, sl);
-  ld8(cos + HALF + li * 8, ch);
-  ld8(sin + HALF + li * 8, sh);
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     // two roundings a product, as the separate rotation kernel: without norms and in the
     // model's type the two give the same bits
-    const float a = __fadd_rn(__fmul_rn(lo[e], cl[e]), __fmul_rn(-hi[e], sl[e]));
-    const float b = __fadd_rn(__fmul_rn(hi[e], ch[e]), __fmul_rn(lo[e], sh[e]));
-    lo[e] = a;
-    hi[e] = b;
+    const float x = __fadd_rn(__fmul_rn(lo[e], a.cl[e]), __fmul_rn(-hi[e], a.sl[e]));
+    const float y = __fadd_rn(__fmul_rn(hi[e], a.ch[e]), __fmul_rn(lo[e], a.sh[e]));
+    lo[e] = x;
+    hi[e] = y;
   }
 }
 
@@ -113,110 +119,161 @@ struct Place {
   int64_t rope;  // position in the tables
   int64_t block;
   int64_t pos;  // position in the cache
-  int row;
 };
 
 __device__ __forceinline__ Place place_of(const NormRopeParams& p, int tok) {
   Place r;
   r.rope = p.rope_pos[tok];
   r.pos = p.store_pos ? p.store_pos[tok] : r.rope;
-  r.row = p.table_index ? p.table_index[tok] : tok;
+  const int row = p.table_index ? p.table_index[tok] : tok;
   r.rope_ok = r.rope >= 0 && r.rope < p.max_seq_len;
   r.block = -1;
-  if (r.pos >= 0 && r.pos / p.bs < p.table_stride && r.row >= 0 && r.row < p.table_rows)
-    r.block = p.tables[(int64_t)r.row * p.table_stride + r.pos / p.bs];
+  if (r.pos >= 0 && r.pos / p.bs < p.table_stride && row >= 0 && row < p.table_rows)
+    r.block = p.tables[(int64_t)row * p.table_stride + r.pos / p.bs];
   r.slot_ok = r.block >= 0 && r.block < p.num_blocks;
   return r;
 }
 
-// One (token, head) per lane group: q heads, and with KV the k and v heads of a cache of the
-// model's type.
+// Heads h0 .. h0 + p.heads - 1 of one token per lane group: q heads, and with KV the k and v heads of a
+// cache of the model's type.  The token's angles are read once for all of them, and two heads are
+// on their way while one is worked on.
 template <typename T, int HD, bool KV>
+__device__ __forceinline__ void rope_block(const NormRopeParams& p, int64_t block) {
+  constexpr int LANES = HD / 16, GROUPS = 128 / LANES, HALF = HD / 2;
+  const int li = threadIdx.x % LANES, grp = threadIdx.x / LANES;
+  const int heads = KV ? p.nq + 2 * p.nkv : p.nq, chunks = (heads + p.heads - 1) / p.heads;
+  const int64_t item = block * GROUPS + grp;
+  const int tok = (int)min(item / chunks, (int64_t)p.n_tokens - 1);
+  const bool live = item / chunks < p.n_tokens;
+  const int h0 = (int)(item % chunks) * p.heads, h1 = min(heads, h0 + p.heads);
+  const T* src = reinterpret_cast<const T*>(p.qkv) + (int64_t)tok * p.ld_qkv + li * 8;
+  auto fetch = [&](int h, T (&r)[16]) {
+    const T* at = src + (int64_t)min(h, h1 - 1) * HD;
+#pragma unroll
+    for (int i = 0; i < 8 * (int)sizeof(T) / 16; ++i) {
+      reinterpret_cast<uint4*>(r)[i] = reinterpret_cast<const uint4*>(at)[i];
+      reinterpret_cast<uint4*>(r + 8)[i] = reinterpret_cast<const uint4*>(at + HALF)[i];
+    }
+  };
+  alignas(16) T first[16], second[16];  // the next two heads
+  fetch(h0, first);
+  fetch(h0 + 1, second);
+  const Place at = place_of(p, tok);
+  if (live && h0 == 0 && li == 0 && !(at.rope_ok && at.slot_ok)) raise_status(p.status, B2_DEV_RANGE);
+  Angles a;
+  load_angles<HD>(p, at.rope_ok ? at.rope : 0, li, a);
+  const float* weight = nullptr;
+  float wl[8], wh[8];
+  auto work = [&](int h, T (&r)[16]) {
+    float lo[8], hi[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      lo[e] = to_f32(r[e]);
+      hi[e] = to_f32(r[8 + e]);
+    }
+    fetch(h + 2, r);
+    if (h < p.nq + p.nkv) {
+      const float* w = h < p.nq ? p.q_weight : p.k_weight;
+      if (w && w != weight) {
+        ld8(w + li * 8, wl);
+        ld8(w + HALF + li * 8, wh);
+        weight = w;
+      }
+      norm_rotate<LANES>(lo, hi, w != nullptr, wl, wh, p.eps, a);
+    }
+    if (!live || !at.rope_ok) return;
+    T* dst;
+    if (h < p.nq) {
+      dst = reinterpret_cast<T*>(p.q_out) + ((int64_t)tok * p.nq + h) * HD;
+    } else {
+      if (!at.slot_ok) return;
+      const int g = h < p.nq + p.nkv ? h - p.nq : h - p.nq - p.nkv;
+      T* cache = reinterpret_cast<T*>(h < p.nq + p.nkv ? p.k_cache : p.v_cache);
+      dst = cache + ((at.block * p.bs + at.pos % p.bs) * p.nkv + g) * HD;
+    }
+    st8(dst + li * 8, lo);
+    st8(dst + HALF + li * 8, hi);
+  };
+  for (int h = h0; h < h1; h += 2) {
+    work(h, first);
+    if (h + 1 < h1) work(h + 1, second);
+  }
+}
+
+template <typename T, int HD>
 __global__ void __launch_bounds__(128) qk_norm_rope_kernel(NormRopeParams p) {
   pdl_wait();
   pdl_trigger();
-  constexpr int LANES = HD / 16, GROUPS = 128 / LANES, HALF = HD / 2;
-  const int li = threadIdx.x % LANES, grp = threadIdx.x / LANES;
-  const int heads = KV ? p.nq + 2 * p.nkv : p.nq;
-  const int64_t item = (int64_t)blockIdx.x * GROUPS + grp;
-  const int64_t tok_l = item / heads;
-  const bool live = tok_l < p.n_tokens;
-  const int tok = live ? (int)tok_l : p.n_tokens - 1, h = (int)(item % heads);
-  const Place at = place_of(p, tok);
-  const T* src = reinterpret_cast<const T*>(p.qkv) + (int64_t)tok * p.ld_qkv + (int64_t)h * HD + li * 8;
-  float lo[8], hi[8];
-  ld8(src, lo);
-  ld8(src + HALF, hi);
-  if (live && h == 0 && li == 0 && !(at.rope_ok && at.slot_ok)) raise_status(p.status, B2_DEV_RANGE);
-  if (h < p.nq + p.nkv) {
-    const int64_t rope = at.rope_ok ? at.rope : 0;
-    norm_rotate<LANES>(lo, hi, h < p.nq ? p.q_weight : p.k_weight, p.eps, p.cos + rope * HD, p.sin + rope * HD, li);
-  }
-  if (!live || !at.rope_ok) return;
-  T* dst;
-  if (h < p.nq) {
-    dst = reinterpret_cast<T*>(p.q_out) + ((int64_t)tok * p.nq + h) * HD;
-  } else {
-    if (!at.slot_ok) return;
-    const int g = h < p.nq + p.nkv ? h - p.nq : h - p.nq - p.nkv;
-    T* cache = reinterpret_cast<T*>(h < p.nq + p.nkv ? p.k_cache : p.v_cache);
-    dst = cache + ((at.block * p.bs + at.pos % p.bs) * p.nkv + g) * HD;
-  }
-  st8(dst + li * 8, lo);
-  st8(dst + HALF + li * 8, hi);
+  rope_block<T, HD, true>(p, blockIdx.x);
 }
 
-// Runs and tiles of the 8-bit cache: one warp per (k or v, head), walking the runs that begin
-// among the block's `chunk` tokens.
+// Runs and tiles of the 8-bit cache: one warp per (k or v, head), for the runs that begin among
+// p.chunk tokens.
 template <typename T, int HD, int CODE>
-__global__ void __launch_bounds__(128) kv_write_q8_kernel(NormRopeParams p) {
-  pdl_wait();
-  pdl_trigger();
+__device__ __forceinline__ void tile_block(const NormRopeParams& p, int64_t block) {
   constexpr int LANES = HD / 16, G = 32 / LANES, ITERS = kQ8Block / G, HALF = HD / 2;
   const int lane = threadIdx.x & 31, li = lane % LANES, grp = lane / LANES;
-  const int head = blockIdx.y * 4 + (threadIdx.x >> 5);  // k heads, then v heads
+  const int head_blocks = (2 * p.nkv + 3) / 4;
+  const int head = (int)(block % head_blocks) * 4 + (threadIdx.x >> 5);  // k heads, then v heads
   if (head >= 2 * p.nkv) return;
   const bool is_k = head < p.nkv;
   const int g = is_k ? head : head - p.nkv;
   uint8_t* cache = reinterpret_cast<uint8_t*>(is_k ? p.k_cache : p.v_cache);
   float* scales = is_k ? p.k_scale : p.v_scale;
-  const int t0 = blockIdx.x * p.chunk, t1 = min(p.n_tokens, t0 + p.chunk);
-  for (int t = t0; t < t1; ++t) {
-    const Place at = place_of(p, t);
-    const int off = (int)(at.pos & (kQ8Block - 1));
-    if (!at.slot_ok) continue;
-    if (t > 0 && off > 0) {  // not the first token of its run?
-      const int64_t before = p.store_pos ? p.store_pos[t - 1] : p.rope_pos[t - 1];
-      const int row = p.table_index ? p.table_index[t - 1] : t - 1;
-      if (row == at.row && before + 1 == at.pos) continue;
-    }
-    // Length of the run: lanes 0..15 look at the tokens that could follow.
-    bool in = lane < kQ8Block - off && t + lane < p.n_tokens;
-    if (in) {
-      const int64_t pos = p.store_pos ? p.store_pos[t + lane] : p.rope_pos[t + lane];
-      const int row = p.table_index ? p.table_index[t + lane] : t + lane;
-      in = row == at.row && pos == at.pos + lane;
-    }
-    const int len = __ffs(~__ballot_sync(0xffffffffu, in)) - 1;
-
+  // Lane i looks at token t0 + i: where it goes, and whether it goes on with the run of the token
+  // before.  Sixteen tokens behind the chunk's belong to runs that begin in it.
+  const int t0 = (int)(block / head_blocks) * p.chunk, mine = t0 + lane;
+  const bool there = mine < p.n_tokens;
+  const Place at = place_of(p, there ? mine : t0);
+  const int row = p.table_index ? p.table_index[there ? mine : t0] : mine;
+  const int off = (int)(at.pos & (kQ8Block - 1));
+  int64_t pos_before = __shfl_up_sync(0xffffffffu, at.pos, 1);
+  int row_before = __shfl_up_sync(0xffffffffu, row, 1);
+  if (lane == 0 && t0 > 0) {
+    pos_before = p.store_pos ? p.store_pos[t0 - 1] : p.rope_pos[t0 - 1];
+    row_before = p.table_index ? p.table_index[t0 - 1] : t0 - 1;
+  }
+  const bool goes_on = mine > 0 && off > 0 && row_before == row && pos_before + 1 == at.pos;
+  const unsigned on = __ballot_sync(0xffffffffu, there && goes_on);
+  unsigned begins = __ballot_sync(0xffffffffu, there && lane < p.chunk && at.slot_ok && !goes_on);
+  const bool norm = is_k && p.k_weight != nullptr;
+  float wl[8], wh[8];
+  if (norm) {
+    ld8(p.k_weight + li * 8, wl);
+    ld8(p.k_weight + HALF + li * 8, wh);
+  }
+  for (; begins; begins &= begins - 1) {
+    const int b = __ffs(begins) - 1, t = t0 + b;
+    const int len = b == 31 ? 1 : __ffs(~(on >> (b + 1)));  // the run's tokens: 1 and those that go on
+    const int first = __shfl_sync(0xffffffffu, off, b);
+    const int64_t blk = __shfl_sync(0xffffffffu, at.block, b);
     float lo[ITERS][8], hi[ITERS][8];
     bool have[ITERS];
-    float amax = 0.f;
-    bool bad = false;
+    int64_t rope[ITERS];
 #pragma unroll
     for (int it = 0; it < ITERS; ++it) {
       const int i = it * G + grp;
       have[it] = i < len;
-      const int tok = have[it] ? t + i : t;
-      int64_t rope = p.rope_pos[tok];
-      if (rope < 0 || rope >= p.max_seq_len) {  // reported by the q heads; the token is not stored
-        have[it] = false;
-        rope = 0;
-      }
-      const T* src = reinterpret_cast<const T*>(p.qkv) + (int64_t)tok * p.ld_qkv + (int64_t)(p.nq + head) * HD + li * 8;
+      const T* src = reinterpret_cast<const T*>(p.qkv) + (int64_t)(t + (have[it] ? i : 0)) * p.ld_qkv +
+                     (int64_t)(p.nq + head) * HD + li * 8;
       ld8(src, lo[it]);
       ld8(src + HALF, hi[it]);
-      if (is_k) norm_rotate<LANES>(lo[it], hi[it], p.k_weight, p.eps, p.cos + rope * HD, p.sin + rope * HD, li);
+      const int from = have[it] ? b + i : b;  // below 32: len ends with the lanes
+      rope[it] = __shfl_sync(0xffffffffu, at.rope, from);
+      // a token with a bad position is not stored (it is reported with its q heads)
+      const bool rope_ok = __shfl_sync(0xffffffffu, (int)at.rope_ok, from);  // by every lane
+      have[it] = have[it] && rope_ok;
+      if (!have[it]) rope[it] = 0;
+    }
+    float amax = 0.f;
+    bool bad = false;
+#pragma unroll
+    for (int it = 0; it < ITERS; ++it) {
+      if (is_k) {
+        Angles a;
+        load_angles<HD>(p, rope[it], li, a);
+        norm_rotate<LANES>(lo[it], hi[it], norm, wl, wh, p.eps, a);
+      }
       if (have[it]) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -230,9 +287,9 @@ __global__ void __launch_bounds__(128) kv_write_q8_kernel(NormRopeParams p) {
     float scale = amax / Q8<CODE>::kTop;
     if (!(scale >= kQ8Tiny)) scale = 0.f;
     if (bad) scale = __int_as_float(0x7fffffff);
-    const int64_t si = q8_scale(at.block, p.nkv, g);
-    uint8_t* tile = cache + q8_tile(at.block, p.nkv, g, HD);
-    if (off > 0) {
+    const int64_t si = q8_scale(blk, p.nkv, g);
+    uint8_t* tile = cache + q8_tile(blk, p.nkv, g, HD);
+    if (first > 0) {
       const float old = scales[si];
       if (old >= scale || old != old) {
         scale = old;
@@ -241,7 +298,7 @@ __global__ void __launch_bounds__(128) kv_write_q8_kernel(NormRopeParams p) {
 #pragma unroll
         for (int it = 0; it < ITERS; ++it) {
           const int slot = it * G + grp;
-          if (slot < off) {
+          if (slot < first) {
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
               uint2* w = reinterpret_cast<uint2*>(tile + slot * HD + half * HALF + li * 8);
@@ -266,7 +323,7 @@ __global__ void __launch_bounds__(128) kv_write_q8_kernel(NormRopeParams p) {
 #pragma unroll
     for (int it = 0; it < ITERS; ++it) {
       if (!have[it]) continue;
-      const int slot = off + it * G + grp;
+      const int slot = first + it * G + grp;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const float(&y)[8] = half ? hi[it] : lo[it];
@@ -284,6 +341,16 @@ __global__ void __launch_bounds__(128) kv_write_q8_kernel(NormRopeParams p) {
     if (lane == 0) scales[si] = scale;
     __syncwarp();  // a token given twice finds the tile as this run left it
   }
+}
+
+// Tiles and q heads in one launch: they have nothing to do with each other, and the tiles' chains of
+// loads hide behind the q heads' traffic.
+template <typename T, int HD, int CODE>
+__global__ void __launch_bounds__(128, 4) qk_norm_rope_q8_kernel(NormRopeParams p) {
+  pdl_wait();
+  pdl_trigger();
+  if ((int)blockIdx.x < p.tile_blocks) tile_block<T, HD, CODE>(p, blockIdx.x);
+  else rope_block<T, HD, false>(p, blockIdx.x - p.tile_blocks);
 }
 
 // out[i, token, head, :] = code * scale of block ids[i], [n, 16, nkv, head_dim].
@@ -341,28 +408,43 @@ int check_norm_rope(const char* name, const NormRopeParams& p, int hd, int layer
   return B2_OK;
 }
 
-template <typename T, int HD, bool KV>
-int launch_rope(const NormRopeParams& p, cudaStream_t s) {
+// Heads per lane group.  More of them share one reading of the token's angles (16 384 tokens of 48
+// heads: %MEAS%); fewer fill the GPU when tokens are few.
+int heads_per_group(int n_tokens, int heads) {
+  int h = 1;
+  while (h < 8 && (int64_t)n_tokens * heads / (2 * h) >= 64 * (int64_t)sm_count()) h *= 2;
+  return h;
+}
+
+template <int HD>
+int64_t rope_blocks(const NormRopeParams& p, int heads) {
   constexpr int GROUPS = 128 / (HD / 16);
-  const int64_t items = (int64_t)p.n_tokens * (KV ? p.nq + 2 * p.nkv : p.nq);
-  const int64_t grid = (items + GROUPS - 1) / GROUPS;
+  return ((int64_t)p.n_tokens * ((heads + p.heads - 1) / p.heads) + GROUPS - 1) / GROUPS;
+}
+
+template <typename T, int HD>
+int launch_rope(NormRopeParams& p, cudaStream_t s) {
+  const int heads = p.nq + 2 * p.nkv;
+  p.heads = heads_per_group(p.n_tokens, heads);
+  const int64_t grid = rope_blocks<HD>(p, heads);
   B2_CHECK_ARG(grid <= 0x7fffffff, "qk_norm_rope: %d tokens are too many for one call", p.n_tokens);
-  B2_TRY_CUDA(launch_pdl((qk_norm_rope_kernel<T, HD, KV>), dim3((unsigned)grid), dim3(128), 0, s, p));
+  B2_TRY_CUDA(launch_pdl((qk_norm_rope_kernel<T, HD>), dim3((unsigned)grid), dim3(128), 0, s, p));
   return B2_OK;
 }
 
 template <typename T, int HD>
-int launch_q8(const NormRopeParams& p0, int cache_dtype, cudaStream_t s) {
-  NormRopeParams p = p0;
-  int rc = launch_rope<T, HD, false>(p, s);
-  if (rc) return rc;
-  p.chunk = p.n_tokens >= 2048 ? 16 : 1;
-  const dim3 grid((p.n_tokens + p.chunk - 1) / p.chunk, (2 * p.nkv + 3) / 4);
-  B2_CHECK_ARG(grid.y <= 65535, "qk_norm_rope: %d kv heads are too many", p.nkv);
+int launch_q8(NormRopeParams& p, int cache_dtype, cudaStream_t s) {
+  p.heads = heads_per_group(p.n_tokens, p.nq);
+  // one token's runs per block while that fills the GPU; a long prefill has one run in sixteen tokens
+  p.chunk = p.n_tokens >= 2048 ? 16 : p.n_tokens >= 512 ? 4 : 1;
+  const int64_t tiles = (int64_t)((p.n_tokens + p.chunk - 1) / p.chunk) * ((2 * p.nkv + 3) / 4);
+  const int64_t grid = tiles + rope_blocks<HD>(p, p.nq);
+  B2_CHECK_ARG(grid <= 0x7fffffff, "qk_norm_rope: %d tokens are too many for one call", p.n_tokens);
+  p.tile_blocks = (int)tiles;
   if (cache_dtype == B2_I8)
-    B2_TRY_CUDA(launch_pdl((kv_write_q8_kernel<T, HD, B2_I8>), grid, dim3(128), 0, s, p));
+    B2_TRY_CUDA(launch_pdl((qk_norm_rope_q8_kernel<T, HD, B2_I8>), dim3((unsigned)grid), dim3(128), 0, s, p));
   else
-    B2_TRY_CUDA(launch_pdl((kv_write_q8_kernel<T, HD, B2_E4M3>), grid, dim3(128), 0, s, p));
+    B2_TRY_CUDA(launch_pdl((qk_norm_rope_q8_kernel<T, HD, B2_E4M3>), dim3((unsigned)grid), dim3(128), 0, s, p));
   return B2_OK;
 }
 
@@ -380,13 +462,13 @@ int b2_qk_norm_rope_kv_write(const void* qkv, int64_t ld_qkv, int n_tokens, int 
   using namespace b2;
   NormRopeParams p{qkv, ld_qkv, n_tokens, nq, nkv, q_weight, k_weight, eps, rope_pos, store_pos, table_index,
                    block_tables, table_rows, table_stride, num_blocks, block_size, cos, sin, max_seq_len, q_out,
-                   k_cache, v_cache, nullptr, nullptr, 0, status};
+                   k_cache, v_cache, nullptr, nullptr, 0, 0, 0, status};
   const int rc = check_norm_rope("b2_qk_norm_rope_kv_write", p, head_dim, layer, dtype);
   if (rc || n_tokens == 0) return rc;
   const size_t off = (size_t)layer * num_blocks * block_size * nkv * head_dim * dtype_bytes(dtype);
   p.k_cache = static_cast<char*>(k_cache) + off;
   p.v_cache = static_cast<char*>(v_cache) + off;
-#define B2_ROPE_CASE(T, HD) return launch_rope<T, HD, true>(p, stream)
+#define B2_ROPE_CASE(T, HD) return launch_rope<T, HD>(p, stream)
   if (dtype == B2_BF16) {
     if (head_dim == 32) B2_ROPE_CASE(__nv_bfloat16, 32);
     if (head_dim == 64) B2_ROPE_CASE(__nv_bfloat16, 64);
@@ -408,7 +490,7 @@ int b2_qk_norm_rope_kv_write_q8(const void* qkv, int64_t ld_qkv, int n_tokens, i
   using namespace b2;
   NormRopeParams p{qkv, ld_qkv, n_tokens, nq, nkv, q_weight, k_weight, eps, rope_pos, store_pos, table_index,
                    block_tables, table_rows, table_stride, num_blocks, block_size, cos, sin, max_seq_len, q_out,
-                   k_cache, v_cache, k_scale, v_scale, 0, status};
+                   k_cache, v_cache, k_scale, v_scale, 0, 0, 0, status};
   B2_CHECK_ARG(valid_q8_dtype(cache_dtype), "b2_qk_norm_rope_kv_write_q8: bad cache dtype");
   if (block_size != kQ8Block)
     return fail(B2_ENOTSUP, "b2_qk_norm_rope_kv_write_q8: block_size %d (16 only)", block_size);
