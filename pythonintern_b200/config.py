@@ -10,6 +10,11 @@ reference constructs them unchanged.  Two behaviours are worth stating:
   This package reproduces that by default; ``ModelConfig.honor_rope_theta = True``
   opts into the configured base.
 * ``KVCacheConfig.device`` defaults to ``"cuda"`` here: the pool lives in HBM.
+
+Two fields have no counterpart there.  ``KVCacheConfig.kv_dtype`` keeps the KV pool in 8 bits
+(``"int8"`` or ``"fp8_e4m3"``, one float32 scale per block and kv head) instead of the model's
+type, and ``ModelConfig.qk_norm`` gives each attention layer an RMS norm over every q and k head
+ahead of the rotation (``self_attn.q_norm.weight``, ``self_attn.k_norm.weight``, [head_dim]).
 """
 
 from dataclasses import dataclass, field
@@ -31,6 +36,7 @@ class ModelConfig:
     # Behaviour switches (defaults reproduce the reference exactly).
     honor_rope_theta: bool = False      # reference ignores rope_theta (attention.py:129)
     masked_decode_padding: bool = False  # reference pads decode K/V with zeros and no mask
+    qk_norm: bool = False               # RMS norm per q and k head before RoPE; not in the reference
 
     @property
     def head_dim(self) -> int:
@@ -68,6 +74,7 @@ class KVCacheConfig:
     block_size: int = 16
     num_blocks: int = 256
     device: str = "cuda"
+    kv_dtype: str = "model"  # "model" (the model's dtype), "int8" or "fp8_e4m3"
 
     @property
     def total_token_capacity(self) -> int:

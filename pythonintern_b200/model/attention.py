@@ -16,6 +16,9 @@ loops and dense gather/pad/repeat copies:
      sequence of the call in one causal launch that shares each K/V block across a tile
      of tokens (attention.py:166-174,211-228);
 then the row-parallel out_proj with its all-reduce (attention.py:231-232).
+
+With ``ModelConfig.qk_norm`` or an 8-bit KV pool step 2 is ``b2_qk_norm_rope_kv_write`` or its
+``_q8`` form, and an 8-bit pool is read by ``b2_prefill_attention_q8`` and ``b2_paged_attention_q8``.
 """
 
 from __future__ import annotations
@@ -31,7 +34,7 @@ from pythonintern_b200.config import ModelConfig
 from pythonintern_b200.model.kv_cache import PhysicalKVCachePool
 from pythonintern_b200.model.metadata import TokenMetadata, build_metadata
 from pythonintern_b200.tensor_parallel.comm import DistributedCommunicator
-from pythonintern_b200.tensor_parallel.layers import ColumnParallelLinear, RowParallelLinear
+from pythonintern_b200.tensor_parallel.layers import ColumnParallelLinear, RMSNorm, RowParallelLinear
 from pythonintern_b200._lib import torch_dtype
 
 
@@ -110,6 +113,9 @@ class DistributedAttention(nn.Module):
         self.v_proj = ColumnParallelLinear(H, config.num_kv_heads * hd, False, rank, world_size, dtype=dt, device=dev)
         self.out_proj = RowParallelLinear(config.num_heads * hd, H, False, rank, world_size, communicator,
                                           dtype=dt, device=dev)
+        # per-head norms, the same weights on every rank
+        self.q_norm = RMSNorm(hd, eps=config.rms_norm_eps, device=dev) if config.qk_norm else None
+        self.k_norm = RMSNorm(hd, eps=config.rms_norm_eps, device=dev) if config.qk_norm else None
         self.rope = rope_for(hd, config.max_seq_len, config.rope_base, dev)
 
     def set_communicator(self, communicator: DistributedCommunicator):
@@ -131,9 +137,20 @@ class DistributedAttention(nn.Module):
             x2d = x2d.to(wdt)
         wq, wk, wv = self.q_proj.packed_weight(), self.k_proj.packed_weight(), self.v_proj.packed_weight()
         q = torch.empty(md.n_tokens, nq * hd, dtype=wdt, device=x2d.device)
+        if pool.quantised or self.q_norm is not None:
+            qkv = (kernels.linear_qkv(x2d, wq, wk, wv) if row_ss is None
+                   else kernels.linear_qkv_rownorm(x2d, wq, wk, wv, row_ss, eps))
+            write = (qkv, nq, nkv, hd, None if self.q_norm is None else self.q_norm.weight,
+                     None if self.k_norm is None else self.k_norm.weight, self.config.rms_norm_eps, md.rope_pos,
+                     md.store_pos, md.table_index, md.tables, self.rope.cos_cached, self.rope.sin_cached, q,
+                     pool.k_cache, pool.v_cache)
+            if pool.quantised:
+                kernels.qk_norm_rope_kv_write_q8(*write, pool.k_scale, pool.v_scale, self.layer_idx)
+            else:
+                kernels.qk_norm_rope_kv_write(*write, self.layer_idx)
         # q|k|v GEMM with RoPE and the KV write in its epilogue where the shape allows it
         # (bit-identical to the GEMM + rope_kv_write pair below)
-        if not kernels.linear_qkv_rope_kv(x2d, wq, wk, wv, nq, nkv, hd, md.rope_pos, md.store_pos, md.table_index,
+        elif not kernels.linear_qkv_rope_kv(x2d, wq, wk, wv, nq, nkv, hd, md.rope_pos, md.store_pos, md.table_index,
                                           md.tables, self.rope.cos_cached, self.rope.sin_cached, q, pool.k_cache,
                                           pool.v_cache, self.layer_idx, row_ss=row_ss, eps=eps):
             if row_ss is not None:
@@ -143,6 +160,13 @@ class DistributedAttention(nn.Module):
             kernels.rope_kv_write(qkv, nq, nkv, hd, md.rope_pos, md.store_pos, md.table_index, md.tables,
                                   self.rope.cos_cached, self.rope.sin_cached, q, pool.k_cache, pool.v_cache,
                                   self.layer_idx)
+        if pool.quantised:
+            cache = (q, nq, nkv, hd, pool.k_cache, pool.v_cache, pool.k_scale, pool.v_scale, self.layer_idx, md.tables)
+            if md.is_prefill and md.seq_start is not None:
+                return kernels.prefill_attention_q8(*cache, md.seq_start, md.n_seqs, 1.0 / math.sqrt(hd),
+                                                    seq_ctx0=md.seq_ctx0, out=out)
+            return kernels.paged_attention_q8(*cache, md.table_index, md.ctx_lens, md.compat_pad, 1.0 / math.sqrt(hd),
+                                              out=out)
         if (md.is_prefill and md.seq_start is not None
                 and kernels.prefill_supported(wdt, nq, nkv, hd, pool.block_size)):
             # every prompt token of every sequence in one causal launch

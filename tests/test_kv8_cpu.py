@@ -1,5 +1,7 @@
 """Refusals of the 8-bit KV cache entry points that need no GPU: the C ABI's argument checks."""
 
+import pytest
+
 from pythonintern_b200 import _lib
 
 A = 1 << 20  # an aligned address that no rejected call dereferences
@@ -95,3 +97,40 @@ def test_block_tables_refusals():
     refused(extend(state=None), _lib.B2_EINVAL, "together")
     rc = L.b2_block_tables_truncate(A, 2, 4, A, A, 16, None, 8, A, None, None)
     refused(rc, _lib.B2_EINVAL, "null")
+
+
+def test_pool_types_and_refusals():
+    import torch
+    from pythonintern_b200._lib import B2Error
+    from pythonintern_b200.config import KVCacheConfig, ModelConfig
+    from pythonintern_b200.model.kv_cache import KVCacheManager, PhysicalKVCachePool
+    assert KVCacheConfig().kv_dtype == "model" and ModelConfig().qk_norm is False
+    m = KVCacheManager(KVCacheConfig(16, 4, "meta", kv_dtype="int8"), ModelConfig(dtype="bfloat16"), 1)
+    p = m.pool
+    assert p.k_cache.shape == (8, 4, 4, 16, 64) and p.k_cache.dtype is torch.int8 and p.dtype is torch.bfloat16
+    assert p.k_scale.shape == (8, 4, 4) and p.k_scale.dtype is torch.float32
+    assert KVCacheManager(KVCacheConfig(16, 4, "meta", kv_dtype="fp8_e4m3"), ModelConfig(),
+                          1).pool.v_cache.dtype is torch.float8_e4m3fn
+    assert not KVCacheManager(KVCacheConfig(16, 4, "meta"), ModelConfig(), 1).pool.quantised
+    with pytest.raises(ValueError, match="kernels only"):
+        p.store_kv(0, 0, 0, torch.zeros(4, 64), torch.zeros(4, 64))
+    with pytest.raises(ValueError, match="kernels only"):
+        p.store_kv_batch(0, [0], [0], torch.zeros(1, 4, 64), torch.zeros(1, 4, 64))
+    for bs, hd in ((8, 64), (16, 96)):
+        with pytest.raises(ValueError, match="blocks of 16"):
+            PhysicalKVCachePool(4, bs, 4, hd, 1, device="meta", dtype="bfloat16", kv_dtype="int8")
+    with pytest.raises(B2Error, match="unsupported KV cache dtype"):
+        PhysicalKVCachePool(4, 16, 4, 64, 1, device="meta", kv_dtype="int4")
+
+
+def test_device_block_tables_refusals():
+    import torch
+    from pythonintern_b200.model.kv_cache import DeviceBlockTables
+    bt = DeviceBlockTables(3, 4, 8, device="cpu")
+    with pytest.raises(ValueError, match="n_tokens"):
+        bt.extend(torch.ones(3, dtype=torch.int32))
+    with pytest.raises(ValueError, match="at least one"):
+        bt.extend([0, 0, 0])
+    for bad in ([1, 2], torch.ones(3, dtype=torch.int64), torch.ones(2, dtype=torch.int32)):
+        with pytest.raises(ValueError, match="per sequence slot"):
+            bt.truncate(bad)
