@@ -368,6 +368,8 @@ __device__ __forceinline__ void tile_block(const NormRopeParams& p, int64_t bloc
       __syncwarp();  // every lane has read the old scale
     }
     const float inv = scale > 0.f ? 1.f / scale : 0.f;  // 0 for a tile of zeros and for NaN
+    // A poisoned run's codes are 0: no NaN code is stored, since a product with it would also reach rows that do
+    // not see its tile.
 #pragma unroll
     for (int it = 0; it < ITERS; ++it) {
       if (!have[it]) continue;
@@ -378,10 +380,10 @@ __device__ __forceinline__ void tile_block(const NormRopeParams& p, int64_t bloc
         float v[4];
         uint2 c;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = y[e] * inv;
+        for (int e = 0; e < 4; ++e) v[e] = bad ? 0.f : y[e] * inv;
         c.x = Q8<CODE>::encode4(v);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = y[4 + e] * inv;
+        for (int e = 0; e < 4; ++e) v[e] = bad ? 0.f : y[4 + e] * inv;
         c.y = Q8<CODE>::encode4(v);
         *reinterpret_cast<uint2*>(tile + slot * HD + half * HALF + li * 8) = c;
       }
