@@ -364,16 +364,11 @@ constexpr float kRoom = 15.f;       // log2 of the largest P
 constexpr float kLift = 8.f;        // log2 of the largest P when a reference has just moved
 constexpr float kNoRef = -1e30f;    // reference of a column that has seen no key
 
-// One CTA per SM.  Its warps are as many as their registers allow; a warp with few columns takes
-// two blocks at once.
-struct Shape {
-  int warps, stages, nb;
-};
-constexpr Shape shape_of(int hd, int nt, int terms) {
-  return nt * terms > 2    ? Shape{8, 3, 1}
-         : nt * terms == 2 ? Shape{12, 3, 1}
-         : hd == 128       ? Shape{12, 3, 1}
-                           : Shape{16, 3, 1};
+// One CTA per SM, of as many warps as its registers allow (decode of 128 rows over 2 048 keys, 8 heads of 128: 100 us
+// with 12 warps; 16 of them spill), each with a ring of three tiles of K and V: a fourth is no faster, nor
+// are two blocks at a time.
+constexpr int warps_of(int hd, int nt, int terms) {
+  return nt * terms > 2 ? 8 : nt * terms == 2 || hd == 128 ? 12 : 16;
 }
 
 template <typename T, int HD, int CODE, int NT>
@@ -388,10 +383,8 @@ struct AttnCfg {
   static constexpr int VW = HD / 32;                     // and of a key's values
   static constexpr int TILE = kQ8Block * HD;             // bytes of codes of one block and head
   static constexpr int Q_BYTES = KW * NT * TERMS * 32 * 8;
-  static constexpr Shape SHAPE = shape_of(HD, NT, TERMS);
-  static constexpr int WARPS = SHAPE.warps;
-  static constexpr int STAGES = SHAPE.stages;            // tiles of K and V a warp holds or has in flight
-  static constexpr int NB = SHAPE.nb;                    // blocks it takes at once
+  static constexpr int WARPS = warps_of(HD, NT, TERMS);
+  static constexpr int STAGES = 3;                       // tiles of K and V a warp holds or has in flight
   static constexpr int WARP_BYTES = STAGES * 2 * TILE;
   // rings, then the q fragments
   static constexpr int SMEM = WARPS * (WARP_BYTES + Q_BYTES);
@@ -505,7 +498,7 @@ q8_attn_kernel(const Q8AttnParams p, int qt, int n_units, int per_group) {
   pdl_wait();
   pdl_trigger();
   using C = AttnCfg<T, HD, CODE, NT>;
-  constexpr int KW = C::KW, VW = C::VW, TERMS = C::TERMS, N = C::N, STAGES = C::STAGES, NB = C::NB, WARPS = C::WARPS;
+  constexpr int KW = C::KW, VW = C::VW, TERMS = C::TERMS, N = C::N, STAGES = C::STAGES, WARPS = C::WARPS;
   __shared__ Line line;
   __shared__ Join joins[WARPS];
   __shared__ int n_joins;
@@ -721,60 +714,43 @@ q8_attn_kernel(const Q8AttnParams p, int qt, int n_units, int per_group) {
     }
     const int tail_from = (pos0 + 1) / kQ8Block - at.block;  // steps whose keys some column does not see
 
-    for (int i = 0; i < cur.cnt; i += NB) {
+    for (int i = 0; i < cur.cnt; ++i) {
       if (i == 0 && nxt.cnt > 0) scales_of(nxt);  // its ids were asked for a window ago
-      // NB blocks at once, for the sake of independent work.  One behind the window's last or outside
-      // the pool is computed from what the ring holds and masked whole.
-      const int nb = min(NB, cur.cnt - i);
-      uint32_t tile[NB];
-      float ks[NB], vs[NB];
-      int key0[NB];
-      bool tail = false, any = false;
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        tile[b] = ring_at + at_slot * (2 * C::TILE);
-        const bool live = b < nb && __shfl_sync(0xffffffffu, cur.id, (i + b) & 31) >= 0;
-        ks[b] = __shfl_sync(0xffffffffu, cur.ks, (i + b) & 31);
-        vs[b] = live ? __shfl_sync(0xffffffffu, cur.vs, (i + b) & 31) : 0.f;
-        key0[b] = live ? (at.block + i + b) * kQ8Block : 0x40000000;
-        tail |= !live || i + b >= tail_from;
-        any |= live;
-        if (b < nb) at_slot = at_slot == STAGES - 1 ? 0 : at_slot + 1;
-      }
-      n_open -= nb;  // as many groups were committed behind these steps'
-      static_assert(STAGES <= 4, "the waits below");
-      if (n_open >= 3) cp_async_wait<3>();
-      else if (n_open == 2) cp_async_wait<2>();
+      const uint32_t tile = ring_at + at_slot * (2 * C::TILE);
+      const bool live = __shfl_sync(0xffffffffu, cur.id, i) >= 0;  // a block outside the pool is passed over
+      const float ks = __shfl_sync(0xffffffffu, cur.ks, i), vs = __shfl_sync(0xffffffffu, cur.vs, i);
+      const int key0 = (at.block + i) * kQ8Block;
+      const bool tail = i >= tail_from;
+      at_slot = at_slot == STAGES - 1 ? 0 : at_slot + 1;
+      --n_open;  // as many groups were committed behind this step's
+      static_assert(STAGES == 3, "the waits below");
+      if (n_open >= 2) cp_async_wait<2>();
       else if (n_open == 1) cp_async_wait<1>();
       else cp_async_wait<0>();
       __syncwarp();
-      if (!any) {
+      if (!live) {
         top_up();
         continue;
       }
-      float s[NB][NT][4], s_odd[NT == 1 ? NB : 1][NT == 1 ? 1 : NT][4];  // two chains of products where columns are few
+      float s[NT][4], s_odd[NT][4];  // two chains of products where columns are few
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int e = 0; e < 4; ++e) s[nt][e] = s_odd[nt][e] = 0.f;
+      uint32_t kw[2][KW];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[b][nt][e] = s_odd[NT == 1 ? b : 0][nt][e] = 0.f;
-      uint32_t kw[NB][2][KW];
+      for (int h = 0; h < 2; ++h) {  // rows eight apart have the same swizzle
+        if constexpr (KW == 2) {
+          const uint2 v = lds8(tile + k_off[0] + h * 8 * HD);
+          kw[h][0] = v.x; kw[h][1] = v.y;
+        } else {
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {  // rows eight apart have the same swizzle
-          if constexpr (KW == 2) {
-            const uint2 v = lds8(tile[b] + k_off[0] + h * 8 * HD);
-            kw[b][h][0] = v.x; kw[b][h][1] = v.y;
-          } else {
-#pragma unroll
-            for (int k = 0; k < KW; k += 4) {
-              const uint4 v = lds16(tile[b] + k_off[k / 4] + h * 8 * HD);
-              kw[b][h][k] = v.x; kw[b][h][k + 1] = v.y; kw[b][h][k + 2] = v.z; kw[b][h][k + 3] = v.w;
-            }
+          for (int k = 0; k < KW; k += 4) {
+            const uint4 v = lds16(tile + k_off[k / 4] + h * 8 * HD);
+            kw[h][k] = v.x; kw[h][k + 1] = v.y; kw[h][k + 2] = v.z; kw[h][k + 3] = v.w;
           }
         }
+      }
 #pragma unroll
       for (int k = 0; k < KW; ++k) {
         uint2 qf[NT][TERMS];
@@ -782,67 +758,51 @@ q8_attn_kernel(const Q8AttnParams p, int qt, int n_units, int per_group) {
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int term = 0; term < TERMS; ++term) qf[nt][term] = lds8(sq_at + ((k * NT + nt) * TERMS + term) * 32 * 8);
+        uint32_t a[4];
+        expand<CODE, C::BIASED>(kw[0][k], a[0], a[2]);
+        expand<CODE, C::BIASED>(kw[1][k], a[1], a[3]);
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          uint32_t a[4];
-          expand<CODE, C::BIASED>(kw[b][0][k], a[0], a[2]);
-          expand<CODE, C::BIASED>(kw[b][1][k], a[1], a[3]);
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int term = 0; term < TERMS; ++term)
-              mma_f16(NT == 1 && (k & 1) ? s_odd[NT == 1 ? b : 0][nt] : s[b][nt], a, qf[nt][term].x, qf[nt][term].y);
-        }
+          for (int term = 0; term < TERMS; ++term)
+            mma_f16(NT == 1 && (k & 1) ? s_odd[nt] : s[nt], a, qf[nt][term].x, qf[nt][term].y);
       }
       if constexpr (NT == 1) {
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[b][0][e] += s_odd[b][0][e];
+        for (int e = 0; e < 4; ++e) s[0][e] += s_odd[0][e];
       }
       // scores; the tail of the tile's keys is masked per column
       if (tail) {
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              if (key0[b] + r8 > lim[nt][e]) s[b][nt][e] = -INFINITY;
-              if (key0[b] + r8 + 8 > lim[nt][e]) s[b][nt][2 + e] = -INFINITY;
-            }
-      }
-      float lv[NB];
-      bool move = false;
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        lv[b] = vs[b] == 0.f ? -INFINITY : __log2f(vs[b]);  // only places a reference: approximate
-#pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            // a column that sees none of the block's keys takes nothing from its scales
-            const float cs = tail && key0[b] > lim[nt][e] ? 1.f : colscale[nt][e] * ks[b];
-            const float c0 = C::BIASED ? bias[nt][e] * cs : 0.f;
-            s[b][nt][e] = fmaf(s[b][nt][e], cs, c0);
-            s[b][nt][2 + e] = fmaf(s[b][nt][2 + e], cs, c0);
-            move |= fmaxf(s[b][nt][e], s[b][nt][2 + e]) > fminf(m[nt][e], m2[nt][e] - lv[b]) + kRoom;
+            if (key0 + r8 > lim[nt][e]) s[nt][e] = -INFINITY;
+            if (key0 + r8 + 8 > lim[nt][e]) s[nt][2 + e] = -INFINITY;
           }
       }
+      const float lv = vs == 0.f ? -INFINITY : __log2f(vs);  // only places a reference: approximate
+      bool move = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          // a column that sees none of the block's keys takes nothing from its scales
+          const float cs = tail && key0 > lim[nt][e] ? 1.f : colscale[nt][e] * ks;
+          const float c0 = C::BIASED ? bias[nt][e] * cs : 0.f;
+          s[nt][e] = fmaf(s[nt][e], cs, c0);
+          s[nt][2 + e] = fmaf(s[nt][2 + e], cs, c0);
+          move |= fmaxf(s[nt][e], s[nt][2 + e]) > fminf(m[nt][e], m2[nt][e] - lv) + kRoom;
+        }
       if (__any_sync(0xffffffffu, move)) {  // references move, to 2^8 below their columns' largest
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float mn = m[nt][e], m2n = m2[nt][e];
+            float mx = fmaxf(s[nt][e], s[nt][2 + e]);
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-              float mx = fmaxf(s[b][nt][e], s[b][nt][2 + e]);
-#pragma unroll
-              for (int sh = 4; sh < 32; sh <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, sh));
-              mn = fmaxf(mn, mx - kLift);
-              m2n = fmaxf(m2n, mx - kLift + lv[b]);
-            }
+            for (int sh = 4; sh < 32; sh <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, sh));
+            const float mn = fmaxf(m[nt][e], mx - kLift), m2n = fmaxf(m2[nt][e], mx - kLift + lv);
             l[nt][e] *= ex2(m[nt][e] - mn);
             const float c = ex2(m2[nt][e] - m2n);
             m[nt][e] = mn;
@@ -855,39 +815,36 @@ q8_attn_kernel(const Q8AttnParams p, int qt, int n_units, int per_group) {
             }
           }
       }
-      uint32_t pb[NB][NT][TERMS][2];
+      uint32_t pb[NT][TERMS][2];
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
+      for (int nt = 0; nt < NT; ++nt) {
+        float pa[2], pc[2];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float pa[2], pc[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            pa[e] = ex2(s[b][nt][e] - m[nt][e]);  // -inf gives 0
-            pc[e] = ex2(s[b][nt][2 + e] - m[nt][e]);
-            l[nt][e] += pa[e] + pc[e];
-            const float f = vs[b] == 0.f || (tail && key0[b] > lim[nt][e]) ? 0.f : vs[b] * lift[nt][e];
-            pa[e] *= f;
-            pc[e] *= f;
-          }
-#pragma unroll
-          for (int term = 0; term < TERMS; ++term) {
-            const uint32_t lo = pack_f16(pa[0], pa[1]), hi = pack_f16(pc[0], pc[1]);
-            pb[b][nt][term][0] = transpose8x8(lo);
-            pb[b][nt][term][1] = transpose8x8(hi);
-            if (TERMS == 2) {
-              const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&lo));
-              const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-              pa[0] -= fa.x; pa[1] -= fa.y; pc[0] -= fb.x; pc[1] -= fb.y;
-            }
-          }
+        for (int e = 0; e < 2; ++e) {
+          pa[e] = ex2(s[nt][e] - m[nt][e]);  // -inf gives 0
+          pc[e] = ex2(s[nt][2 + e] - m[nt][e]);
+          l[nt][e] += pa[e] + pc[e];
+          const float f = vs == 0.f || (tail && key0 > lim[nt][e]) ? 0.f : vs * lift[nt][e];
+          pa[e] *= f;
+          pc[e] *= f;
         }
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
+        for (int term = 0; term < TERMS; ++term) {
+          const uint32_t lo = pack_f16(pa[0], pa[1]), hi = pack_f16(pc[0], pc[1]);
+          pb[nt][term][0] = transpose8x8(lo);
+          pb[nt][term][1] = transpose8x8(hi);
+          if (TERMS == 2) {
+            const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+            const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+            pa[0] -= fa.x; pa[1] -= fa.y; pc[0] -= fb.x; pc[1] -= fb.y;
+          }
+        }
+      }
+      {
         uint32_t vw[4][VW];
 #pragma unroll
         for (int h = 0; h < 4; ++h) {
-          const uint32_t a = tile[b] + v_off[h & 1] + (h >> 1) * 8 * HD;
+          const uint32_t a = tile + v_off[h & 1] + (h >> 1) * 8 * HD;
           if constexpr (VW == 4) {
             const uint4 v = lds16(a);
             vw[h][0] = v.x; vw[h][1] = v.y; vw[h][2] = v.z; vw[h][3] = v.w;
@@ -899,8 +856,8 @@ q8_attn_kernel(const Q8AttnParams p, int qt, int n_units, int per_group) {
           }
         }
         // V of keys no column sees counts as 0, whatever its codes (an e4m3 NaN among them)
-        if (tail && key0[b] + kQ8Block - 1 > pos_last) {
-          const int k0 = key0[b] + 2 * t4;
+        if (tail && key0 + kQ8Block - 1 > pos_last) {
+          const int k0 = key0 + 2 * t4;
 #pragma unroll
           for (int h = 0; h < 4; ++h)
             if (k0 + (h & 1) + (h >> 1) * 8 > pos_last) {
@@ -920,7 +877,7 @@ q8_attn_kernel(const Q8AttnParams p, int qt, int n_units, int per_group) {
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int term = 0; term < TERMS; ++term)
-                mma_f16(o[2 * v + half][nt], a, pb[b][nt][term][0], pb[b][nt][term][1]);
+                mma_f16(o[2 * v + half][nt], a, pb[nt][term][0], pb[nt][term][1]);
           }
         }
       }
@@ -1120,11 +1077,21 @@ int check_q8_pointers(const char* name, const Q8AttnParams& p, int dtype) {
 
 
 // ------------------------------------------------------------------ host side
-// Prefills of long enough pieces run on tcgen05 (prefill_q8_tc.cu).
+// Which prefills run on tcgen05 (prefill_q8_tc.cu).  Its items are two tiles of 128 columns of a sequence and
+// head, one per SM at a time, 22 ns per key; this file's kernel cuts all tiles of 32 columns evenly over
+// the SMs, 13 ns per key and tile of an SM.  Both are proportional to the context, which only the
+// device knows, so the rule compares tiles with rounds of items.  Both sides measured (us, here / tcgen05):
+//   heads 32/8, 1 sequence, 32 000 keys:    64 tokens  220 / 722,  128  395 / 723,  256  746 / 726
+//   heads 32/8, 8 sequences, 4 000 keys:    16 tokens   86 /  94,   32  137 /  76,  256  796 / 203
+//   heads  8/8, 64 sequences, 1 000 keys:   16 tokens   58 / 107,   64  165 / 110,  256  507 / 139
+//   heads  8/1, 64 sequences, 1 000 keys:    8 tokens   45 /  29,   16   65 /  26,   64  153 /  35
 bool tensor_prefill(int n_rows, int n_seqs, int nq, int nkv, int hd, float scale, int dtype) {
   const int rep = nq / nkv;
-  return dtype == B2_BF16 && hd == 128 && (rep == 1 || rep == 2 || rep == 4 || rep == 8) && scale > 0.f &&
-         n_rows >= 16 * n_seqs;
+  if (dtype != B2_BF16 || hd != 128 || !(rep == 1 || rep == 2 || rep == 4 || rep == 8) || !(scale > 0.f)) return false;
+  const int64_t columns = ((int64_t)n_rows + n_seqs - 1) / n_seqs * rep;
+  const int64_t tiles = (columns + 31) / 32 * n_seqs * nkv, items = (columns + 255) / 256 * n_seqs * nkv;
+  const int64_t sms = sm_count(), rounds = (items + sms - 1) / sms;
+  return 3 * tiles >= 4 * sms * rounds;
 }
 
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
@@ -1136,17 +1103,18 @@ struct AttnPlan {
 
 // Columns of a tile.  A decode row has rep columns.  A sequence of a prefill has tokens * rep;
 // wide tiles read the cache once for more of them, narrow ones keep more warps resident and
-// waste fewer columns of the products, so the width follows the mean length.
+// waste fewer columns of the products, so the width follows the mean length (48 drafts of 5 tokens, 4 heads
+// to a kv head: 96 us in 24 columns, 129 in 32).
 AttnPlan plan_of(int n_rows, int nq, int nkv, int hd, int n_seqs, bool prefill, int dtype) {
   AttnPlan a{};
   const int rep = nq / nkv, terms = dtype == B2_F32 ? 2 : 1;
   const int64_t columns = prefill ? (int64_t)((n_rows + n_seqs - 1) / n_seqs) * rep : rep;
-  a.nt = columns <= 8 && rep <= 8 ? 1 : columns <= 16 || terms == 2 ? 2 : 4;
+  a.nt = columns <= 8 && rep <= 8 ? 1 : columns <= 16 || terms == 2 ? 2 : columns <= 24 ? 3 : 4;
   a.qt = prefill ? 8 * a.nt / rep : 1;
   a.units = prefill ? n_seqs : n_rows;
   a.per_group = (a.units + kGroups - 1) / kGroups;
   a.ctas = sm_count();
-  a.slots = 2 * a.ctas * shape_of(hd, a.nt, terms).warps;
+  a.slots = 2 * a.ctas * warps_of(hd, a.nt, terms);
   a.piece = align256((size_t)a.ctas * sizeof(int4));
   a.stat = a.piece + align256((size_t)a.ctas * sizeof(int2));
   a.o = a.stat + align256((size_t)a.slots * 8 * a.nt * sizeof(float4));
@@ -1183,7 +1151,8 @@ template <typename T, int HD, int CODE>
 int launch_nt(const Q8AttnParams& p, const AttnPlan& a, cudaStream_t s) {
   if (a.nt == 1) return launch_tiles<T, HD, CODE, 1>(p, a, s);
   if (a.nt == 2) return launch_tiles<T, HD, CODE, 2>(p, a, s);
-  if constexpr (sizeof(T) == 2) return launch_tiles<T, HD, CODE, 4>(p, a, s);
+  if constexpr (sizeof(T) == 2)
+    return a.nt == 3 ? launch_tiles<T, HD, CODE, 3>(p, a, s) : launch_tiles<T, HD, CODE, 4>(p, a, s);
   return fail(B2_ENOTSUP, "attention over the 8-bit cache: no tile of %d columns", 8 * a.nt);
 }
 

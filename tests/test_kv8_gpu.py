@@ -735,6 +735,68 @@ def test_prefill_attention_q8_long(code, nq, nkv, lens, ctx0):
             _close(out[r], want, size, torch.bfloat16)
 
 
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("nq,nkv", [(16, 16), (16, 8), (16, 4), (16, 2)])
+def test_prefill_attention_q8_many_rows(code, nq, nkv):
+    """Enough rows for the tcgen05 kernel at every number of heads to a kv head, with what may go wrong in it: an
+    empty sequence, scales that differ by 2^40 and are 0, pages outside the pool, NaN codes behind the context,
+    padded q rows, and rows behind the last sequence."""
+    hd, lens, ctx0 = 128, [200, 0, 250], [40, 0, 7]
+    tab, NB = _tables_for([-(-(c + n) // 16) for c, n in zip(ctx0, lens)], 2, 1)
+    cache = _stored(code, NB, nkv, hd, seed=4)
+    cache[3] *= torch.exp2(torch.randint(-20, 20, cache[3].shape, generator=gen(5)).float()).to(DEV)
+    for j in (0, 1):
+        cache[3][0, tab[0, j]] = 0
+    cache[2][0, tab[0, 2]] = 0
+    for s in (0, 2):
+        last = ctx0[s] + lens[s] - 1
+        for x in (cache[0], cache[1]):
+            x[0, int(tab[s, last // 16])].view(torch.uint8)[:, last % 16 + 1:] = 0x7f  # e4m3: NaN
+    T = sum(lens)
+    q = torch.randn(T + 3, nq * hd + 8, generator=gen(6))
+    q[::3] *= 6
+    q[1::5] *= 2.0 ** -60
+    q = q.to(DEV, torch.bfloat16)[:, : nq * hd]
+    start = np.concatenate([[0], np.cumsum(lens)])
+    bad = tab.copy()
+    bad[0, 5], bad[2, 1], bad[2, 9] = NB, -1, 1 << 30
+    clean = np.where((bad < 0) | (bad >= NB), -1, bad)
+    for t, pages in ((tab, tab), (bad, clean)):
+        out = torch.full((T + 3, nq * hd), 7.0, dtype=torch.bfloat16, device=DEV)
+        kernels.prefill_attention_q8(q, nq, nkv, hd, *cache, 0, torch.from_numpy(t).to(DEV), i32(start.tolist()), 3,
+                                     1 / math.sqrt(hd), seq_ctx0=i32(ctx0), out=out)
+        if t is bad:
+            with pytest.raises(IndexError):
+                _lib.check_device_status(DEV, "prefill")
+        _lib.check_device_status(DEV, "prefill")
+        assert (out[T:] == 7.0).all()
+        for s, n in enumerate(lens):
+            for i in sorted({0, 15, 16, 31, 63, 64, 127, 128, n // 2, n - 1} & set(range(n))):
+                r = int(start[s]) + i
+                want, size = _attend64(q[r], cache, 0, pages[s].tolist(), ctx0[s] + i + 1, 1 / math.sqrt(hd))
+                _close(out[r], want, size, torch.bfloat16)
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("nkv,n", [(16, 400), (2, 60)])
+def test_a_value_that_is_not_finite_reaches_no_row_before_its_block(code, nkv, n):
+    """Written and read in one call: tcgen05 tiles (400 tokens, 16 heads) and mma tiles hold rows of several
+    blocks, of which those before the poisoned one keep their bits."""
+    hd, at = 128, 37
+    rope = RotaryEmbedding(hd, 512, 10000.0, DEV)
+    outs = []
+    for x in (1.0, float("inf"), float("nan")):
+        qkv, pos, row, tab, NB = _step([n], [0], nkv, nkv, hd, torch.bfloat16, 2)
+        qkv.view(n, 3 * nkv, hd)[at, nkv:, 5] = x
+        cache = _caches(code, NB, nkv, hd, seed=3)
+        q = _write(qkv, nkv, nkv, hd, None, pos, row, tab, rope, cache)
+        outs.append(kernels.prefill_attention_q8(q, nkv, nkv, hd, *cache, 0, tab, i32([0, n]), 1, 0.1))
+        _lib.check_device_status(DEV, "poison")
+    assert torch.isfinite(outs[0]).all()
+    for out in outs[1:]:
+        assert torch.equal(out[:32], outs[0][:32]) and torch.isnan(out[32:]).all()
+
+
 def test_attention_q8_refusals():
     nq, nkv, hd = 4, 2, 64
     cache = _stored("int8", 4, nkv, hd)
