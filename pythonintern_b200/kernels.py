@@ -355,7 +355,7 @@ class SlotMap(NamedTuple):
 
 def _check(t: torch.Tensor, name: str, dtype: torch.dtype, numel: int, device: torch.device):
     """A contiguous CUDA tensor of at least ``numel`` elements of ``dtype`` on ``device``."""
-    if t.dtype is not dtype or t.get_device() != device.index or not t.is_contiguous() or t.numel() < numel:
+    if t.dtype is not dtype or t.get_device() != device.index or t.numel() < numel or not t.is_contiguous():
         raise _lib.B2Error(f"{name} must be a contiguous {dtype} tensor of at least {numel} elements on {device}; "
                            f"got {t.dtype} {tuple(t.shape)} on {t.device}")
 
@@ -413,8 +413,8 @@ def block_tables_extend(tables: torch.Tensor, lens: torch.Tensor, new_lens: torc
     if out is None:
         i64 = torch.empty(2 * max_tokens + n, dtype=torch.int64, device=dev)
         i32 = torch.empty(2 * max_tokens + n + 1, dtype=torch.int32, device=dev)
-        positions, slots, last_rows = i64.split_with_sizes((max_tokens, max_tokens, n))
-        table_index, ctx_lens, seq_start = i32.split_with_sizes((max_tokens, max_tokens, n + 1))
+        positions, slots, last_rows = i64.unsafe_split_with_sizes((max_tokens, max_tokens, n))
+        table_index, ctx_lens, seq_start = i32.unsafe_split_with_sizes((max_tokens, max_tokens, n + 1))
         out = SlotMap(seq_start, positions, table_index, slots, ctx_lens, last_rows)
     else:
         _check(out.seq_start, "seq_start", torch.int32, n + 1, dev)
@@ -478,34 +478,38 @@ def qk_norm_rope_kv_write(qkv: torch.Tensor, nq: int, nkv: int, head_dim: int, q
     norm) before the rotation, in the same pass (engine/model/attention.py:46-63, :166-184)."""
     args = _norm_rope_args(qkv, nq, nkv, head_dim, q_weight, k_weight, eps, rope_pos, store_pos, table_index,
                            block_tables, cos, sin, q_out)
-    _check_cache(k_cache, v_cache, layer, (nkv, head_dim), qkv.dtype, qkv.device, 2)
-    _, NB, bs, _, _ = k_cache.shape
+    _, NB, bs, _, _ = _check_cache(k_cache, v_cache, layer, qkv.dtype, qkv.device, (None, nkv, head_dim))
     _call("b2_qk_norm_rope_kv_write", qkv.device, *args, NB, bs, ptr(cos), ptr(sin), cos.shape[0], ptr(q_out),
           ptr(k_cache), ptr(v_cache), layer, dtype_code(qkv.dtype))
 
 
-def _check_cache(k_cache, v_cache, layer, tail, dtype, device, at):
-    """Both caches: contiguous, 5 dimensions, of ``dtype``, with ``tail`` as their dimensions from ``at + 1``."""
+def _check_cache(k_cache, v_cache, layer, dtype, device, tail):
+    """Both caches: contiguous, [layers, blocks, *tail] of ``dtype`` (None in ``tail``: any size)."""
+    shape = k_cache.shape
+    ok = len(shape) == 5 and v_cache.shape == shape
+    if ok:
+        for have, want in zip(shape[2:], tail):
+            ok = ok and (want is None or have == want)
+    at = device.index
     for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        if (t.dim() != 5 or t.dtype != dtype or t.device != device or not t.is_contiguous()
-                or t.shape != k_cache.shape or tuple(t.shape[at + 1:at + 1 + len(tail)]) != tail):
-            raise _lib.B2Error(f"{name} must be a contiguous {dtype} cache of {tail} on {device}; got {t.dtype} "
-                               f"{tuple(t.shape)} on {t.device}")
-    if not 0 <= layer < k_cache.shape[0]:
-        raise IndexError(f"layer {layer} of a cache with {k_cache.shape[0]}")
+        if not ok or t.dtype is not dtype or t.get_device() != at or not t.is_contiguous():
+            raise _lib.B2Error(f"{name} must be a contiguous {dtype} cache [layers, blocks, {', '.join(map(str, tail))}] "
+                               f"on {device}; got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if not 0 <= layer < shape[0]:
+        raise IndexError(f"layer {layer} of a cache with {shape[0]}")
+    return shape
 
 
 def _q8_cache(k_cache, v_cache, k_scale, v_scale, layer, nkv, hd, device):
     """Checks an 8-bit cache [L, blocks, nkv, 16, hd] and its scales [L, blocks, nkv]; returns (type code, blocks, 16)."""
     code = _lib.cache_dtype_code(k_cache.dtype)
-    _check_cache(k_cache, v_cache, layer, (nkv,), k_cache.dtype, device, 1)
-    if k_cache.shape[4] != hd:
-        raise _lib.B2Error(f"the cache holds heads of {k_cache.shape[4]}, not {hd}")
+    shape = _check_cache(k_cache, v_cache, layer, k_cache.dtype, device, (nkv, None, hd))
+    scales = shape[:3]
     for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
         _check(t, name, torch.float32, 1, device)
-        if t.shape != k_cache.shape[:3]:
-            raise _lib.B2Error(f"{name} must be {tuple(k_cache.shape[:3])}, got {tuple(t.shape)}")
-    return code, k_cache.shape[1], k_cache.shape[3]
+        if t.shape != scales:
+            raise _lib.B2Error(f"{name} must be {tuple(scales)}, got {tuple(t.shape)}")
+    return code, shape[1], shape[3]
 
 
 def qk_norm_rope_kv_write_q8(qkv: torch.Tensor, nq: int, nkv: int, head_dim: int, q_weight: Optional[torch.Tensor],
