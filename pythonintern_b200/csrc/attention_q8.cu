@@ -9,8 +9,15 @@
 // blocks; the blocks of all tiles and heads in a row form one line of steps, cut into equal
 // chunks, one per resident warp, so ragged contexts cost no more than even ones.  A warp works
 // alone (no barrier in the loop).  A tile that lies in one chunk is finished there; the pieces of
-// others go to the workspace as softmax states and are joined by a second kernel.  Every CTA
-// finds the cut by itself from the lengths, so nothing waits on the host.
+// others go to the workspace as softmax states.  Those of one CTA are joined by its own warps after its
+// loop; only a tile that reaches over CTAs, at most one begins in each, is left to a second kernel.
+// Every CTA finds the cut by itself from the lengths, so nothing waits on the host.
+//
+// What bounds it (heads 32/8 of 128, measured in a graph): int8 decode of 128 rows over 2 048 keys reads 540 MB in
+// 100-107 us, 5.0-5.4 TB/s of 6.55 measured (its loop runs at the copy's rate; 4.5 us go to finding the cut and
+// the first tiles, some 8 to filling and draining and the join); one row over 8 192 keys 17 us, of which
+// 2.6 are reading; drafts of 5 tokens for 48 sequences 96 us, bound by the work on a step (expanding
+// codes, products, softmax), not by its bytes.
 //
 // One step.  S^T[16 keys x 8 NT] = K Q^T and O^T[head_dim x 8 NT] += V^T P^T on
 // mma.sync.m16n8k16 with float16 operands and float32 sums.  A code of 8 bits is exact in

@@ -10,13 +10,17 @@
 // order and writes the maps of the new tokens; truncate() gives the blocks behind the kept
 // tokens back to the ring's tail, in sequence and then table order, as the host list would.
 //
-// Every CTA scans all n_seqs lengths by itself (two prefix sums kept in shared memory), which
-// costs less than a second launch or a grid barrier would; the items (groups of tokens, or
+// Every CTA scans all n_seqs lengths by itself (lengths and two prefix sums kept in shared memory),
+// which costs less than a second launch or a grid barrier would; the items (groups of tokens, or
 // blocks to give back) are then spread over the grid, each finding its sequence by bisection
 // of the prefix.  Nothing that a CTA reads is written before every CTA has read it: the last
 // CTA to finish (a ticket in free_state[2], put back to 0) updates lens and the ring's state.
 // A call that cannot be served whole (a bad length, a row past the table, too few free blocks,
 // more tokens than the maps hold) raises its bit in *status and changes nothing.
+//
+// Bound by latency: one extend and one truncate of 128 sequences with 5 new tokens each take 11.2 us in a graph, 16 new
+// prompts of 1 024 tokens 8.6, 2 048 ragged sequences 18.6 (5.2 MB: 0.8 us of reading and writing); a chain of
+// loads, scan, bisection, dependent loads and stores, and the ticket, twice.
 #include <algorithm>
 #include <mutex>
 #include <set>

@@ -13,6 +13,11 @@
 // and written in 16-byte pieces, the rotation stays within a lane and the mean takes
 // log2(head_dim / 16) shuffles.
 //
+// Measured (heads 32/8 of 128, in a graph): bf16 cache, 16 384 tokens: 95 us, 404 MB at 4.3 TB/s (bound by
+// the issue of instructions, 0.65 of the copy's rate); 8 tokens: 2.5 us.  int8 cache and the read-back of 128 blocks:
+// 128 tokens 10.9 us, two launches and their chains of loads.  e4m3 cache, 3 815 ragged tokens of heads 32/4 of 64, with
+// the read-back: 32 us.
+//
 // 8-bit tiles.  The tokens of a call that fall into one block form a run; one warp per (run,
 // head) holds the run's values in registers, takes their largest magnitude and writes codes
 // and scale.  Where the run begins inside a block, the slots before it are history: the tile
