@@ -12,9 +12,8 @@
 // follows the largest s + log2(vs), so f16 keeps its precision however the scales of blocks differ.
 //
 // 16 prompts of 1 024 tokens, heads 32/8, int8: 266 us, 517 TFLOP/s (prefill_tc.cu on a bf16 cache: 262).  As there, the
-// issue of the MMAs and the hand-offs between the roles bound it, not the conversion: four converter
-// warps for two took 334 to 307 us with the scales fetched a tile ahead, one election per batch of MMAs
-// instead of per MMA 307 to 269.
+// issue of the MMAs and the hand-offs between the roles bound it: four converter warps and the register split
+// 368 -> 334 us, scales fetched a tile ahead 307, one election per batch of MMAs instead of per MMA 269.
 #include "prefill_tc.cuh"
 #include "q8.cuh"
 

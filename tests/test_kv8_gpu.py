@@ -777,6 +777,29 @@ def test_prefill_attention_q8_many_rows(code, nq, nkv):
                 _close(out[r], want, size, torch.bfloat16)
 
 
+@pytest.mark.parametrize("nq,nkv,n,longest", [(8, 1, 300, 32), (4, 2, 700, 6)])
+def test_prefill_attention_q8_many_sequences(nq, nkv, n, longest):
+    """More sequences than a CTA keeps the lengths of (192 in the tcgen05 kernel, 256 groups in the mma one), many of
+    them empty."""
+    hd = 128
+    lens = torch.randint(0, longest, (n,), generator=gen(1)).tolist()
+    ctx0 = torch.randint(0, 40, (n,), generator=gen(2)).tolist()
+    lens[0] = lens[-1] = 0
+    tab, NB = _tables_for([-(-(c + m) // 16) for c, m in zip(ctx0, lens)], 3, nq)
+    cache = _stored("int8", NB, nkv, hd, seed=nq)
+    T = sum(lens)
+    q = torch.randn(T, nq * hd, generator=gen(9)).to(DEV, torch.bfloat16)
+    start = np.concatenate([[0], np.cumsum(lens)])
+    out = kernels.prefill_attention_q8(q, nq, nkv, hd, *cache, 0, torch.from_numpy(tab).to(DEV), i32(start.tolist()),
+                                       n, 1 / math.sqrt(hd), seq_ctx0=i32(ctx0))
+    _lib.check_device_status(DEV, "prefill")
+    for s in list(range(0, n, 37)) + [n - 2, n - 1]:
+        for i in sorted({0, lens[s] - 1} & set(range(lens[s]))):
+            r = int(start[s]) + i
+            want, size = _attend64(q[r], cache, 0, tab[s].tolist(), ctx0[s] + i + 1, 1 / math.sqrt(hd))
+            _close(out[r], want, size, torch.bfloat16)
+
+
 @pytest.mark.parametrize("code", ["int8", "e4m3"])
 @pytest.mark.parametrize("nkv,n", [(16, 400), (2, 60)])
 def test_a_value_that_is_not_finite_reaches_no_row_before_its_block(code, nkv, n):

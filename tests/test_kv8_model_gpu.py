@@ -191,6 +191,55 @@ def test_a_step_that_cannot_be_served_is_empty():
     assert torch.equal(pool.k_cache, before[0]) and torch.equal(bt.tables, before[1]) and torch.equal(bt.lens, before[2])
 
 
+@pytest.mark.parametrize("kv_dtype", ["model", "fp8_e4m3"])
+def test_idle_slots_and_captured_steps_over_device_tables(kv_dtype):
+    """Slots without new tokens, and a step of drafts (extend, forward, truncate) captured once and replayed with
+    other lengths on the device: the same as eager steps over a second set of tables and pool."""
+    from pythonintern_b200.model.kv_cache import DeviceBlockTables
+    cfg = _config()
+    model = _model(cfg, 6)
+    sides = [(DeviceBlockTables(4, 8, 32, device=DEV), _pool(cfg, kv_dtype)) for _ in range(2)]
+    g = torch.Generator(device="cpu").manual_seed(3)
+    prompt = torch.randint(0, 128, (1, 41), generator=g).to(DEV)
+    for bt, pool in sides:
+        model.greedy(prompt, None, pool, [], True, 0, metadata=bt.extend([30, 0, 11, 0]))
+    _lib.check_device_status(DEV, "prompts")
+    new = torch.zeros(4, dtype=torch.int32, device=DEV)
+    keep = torch.zeros(4, dtype=torch.int32, device=DEV)
+    ids = torch.zeros(1, 8, dtype=torch.int64, device=DEV)
+
+    def step(bt, pool):
+        out = model.greedy(ids, None, pool, [], True, 0, metadata=bt.extend(new, 8))
+        bt.truncate(keep)
+        return out
+
+    plan = [([5, 0, 3, 0], [33, 0, 14, 0]), ([2, 5, 0, 1], [35, 2, 14, 1]), ([0, 4, 2, 2], [17, 6, 16, 0])]
+    (bt, pool), (bt2, pool2) = sides
+    want = []
+    for k, (n, c) in enumerate(plan):
+        ids.copy_(torch.randint(0, 128, (1, 8), generator=torch.Generator().manual_seed(k)))
+        new.copy_(torch.tensor(n, dtype=torch.int32))
+        keep.copy_(torch.tensor(c, dtype=torch.int32))
+        tok, top = step(bt, pool)
+        active = torch.tensor(n) > 0
+        want.append((tok.cpu()[active], top.cpu()[active], bt.tables.clone(), bt.lens.clone(), bt.free_state.clone()))
+    _lib.check_device_status(DEV, "eager")
+    new.zero_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        tok, top = step(bt2, pool2)
+    for k, (n, c) in enumerate(plan):
+        ids.copy_(torch.randint(0, 128, (1, 8), generator=torch.Generator().manual_seed(k)))
+        new.copy_(torch.tensor(n, dtype=torch.int32))
+        keep.copy_(torch.tensor(c, dtype=torch.int32))
+        graph.replay()
+        active = torch.tensor(n) > 0
+        got = (tok.cpu()[active], top.cpu()[active], bt2.tables, bt2.lens, bt2.free_state)
+        assert all(torch.equal(a, b) for a, b in zip(got, want[k])), k
+    _lib.check_device_status(DEV, "replays")
+    assert torch.equal(pool.k_cache.view(torch.uint8), pool2.k_cache.view(torch.uint8))
+
+
 def test_qk_norm_adds_two_keys_to_a_layer_and_none_without():
     plain, normed = _model(_config()).state_dict(), _model(_config(qk_norm=True)).state_dict()
     extra = set(normed) - set(plain)
