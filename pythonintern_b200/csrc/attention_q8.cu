@@ -91,7 +91,6 @@ struct Q8AttnParams {
 
 // ------------------------------------------------------------------ the cut of the work
 constexpr int kGroups = 256;   // prefix sums kept in shared memory
-constexpr int kMaxWarps = 16;  // of a CTA
 constexpr int kMinChunk = 2;   // steps a warp takes at least
 
 struct Unit {  // a decode row, or a sequence of a prefill
@@ -170,10 +169,13 @@ struct Line {
 };
 
 // Prefix sums over groups of units.  Called by the whole CTA.
-__device__ Cut make_cut(const Q8AttnParams& p, int qt, int n_units, int per_group, Line& line, int warps, bool report) {
-  __shared__ int64_t w_steps[kMaxWarps];
-  __shared__ int w_tiles[kMaxWarps], w_ctx[kMaxWarps];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x;
+template <int WARPS>
+__device__ __forceinline__ Cut make_cut(const Q8AttnParams& p, int qt, int n_units, int per_group, Line& line,
+                                        int warps, bool report) {
+  __shared__ int64_t w_steps[WARPS];
+  __shared__ int w_tiles[WARPS], w_ctx[WARPS];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  constexpr int threads = 32 * WARPS;
   const int groups = (n_units + per_group - 1) / per_group;
   const int per_thread = (groups + threads - 1) / threads;
   int64_t steps = 0;
@@ -216,7 +218,8 @@ __device__ Cut make_cut(const Q8AttnParams& p, int qt, int n_units, int per_grou
   Cut c{0, 0, 0, 0};
   int64_t base_s = inc_s - steps;
   int base_t = inc_t - tiles;
-  for (int w = 0; w < threads / 32; ++w) {
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
     if (w < warp) {
       base_s += w_steps[w];
       base_t += w_tiles[w];
@@ -231,7 +234,8 @@ __device__ Cut make_cut(const Q8AttnParams& p, int qt, int n_units, int per_grou
   }
   __syncthreads();
   c.total *= p.nkv;
-  const int64_t even = c.total >> 32 ? (c.total + warps - 1) / warps : ((uint32_t)c.total + warps - 1) / (uint32_t)warps;
+  const int64_t even =
+      c.total >> 32 ? (c.total + warps - 1) / warps : ((uint32_t)c.total + warps - 1) / (uint32_t)warps;
   c.chunk = max((int64_t)kMinChunk, even);
   return c;
 }
@@ -250,11 +254,13 @@ struct Place {  // where a step lies
 __device__ __forceinline__ Place find_step(const Q8AttnParams& p, int64_t x, int qt, int n_units, int per_group,
                                            const Line& line) {
   const int groups = (n_units + per_group - 1) / per_group;
-  int lo = 0, hi = groups - 1;
-  while (lo < hi) {  // the last group that begins at or before x (empty ones share their successor's begin)
-    const int mid = (lo + hi + 1) >> 1;
-    if (line.steps[mid] * p.nkv <= x) lo = mid; else hi = mid - 1;
-  }
+  // the last group that begins at or before x (empty ones share their successor's begin): every lane looks at
+  // some, which waits for shared memory once where a bisection would eight times
+  int lo = 0;
+#pragma unroll
+  for (int g = 0; g < kGroups; g += 32)
+    if (g + (int)(threadIdx.x & 31) < groups && line.steps[g + (threadIdx.x & 31)] * p.nkv <= x) ++lo;
+  lo = __reduce_add_sync(0xffffffffu, lo) - 1;
   Place r;
   r.u = lo * per_group;
   r.tile = line.tiles[lo];
@@ -314,7 +320,8 @@ __device__ __forceinline__ void expand(uint32_t x, uint32_t& lo, uint32_t& hi) {
     const uint32_t u = x ^ 0x80808080u;
     const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));  // 1152
     uint32_t a = prmt(u, 0x64646464u, 0x4140), b = prmt(u, 0x64646464u, 0x4342);
-    const __half2 ha = __hsub2(*reinterpret_cast<__half2*>(&a), bias), hb = __hsub2(*reinterpret_cast<__half2*>(&b), bias);
+    const __half2 ha = __hsub2(*reinterpret_cast<__half2*>(&a), bias);
+    const __half2 hb = __hsub2(*reinterpret_cast<__half2*>(&b), bias);
     lo = *reinterpret_cast<const uint32_t*>(&ha);
     hi = *reinterpret_cast<const uint32_t*>(&hb);
   } else {
@@ -529,7 +536,7 @@ q8_attn_kernel(const Q8AttnParams p, int qt, int n_units, int per_group) {
                           : VW == 2 ? tile_at<HD>(2 * t4 + h, r8 >> 1) + (r8 & 1) * 8
                                     : tile_at<HD>(2 * t4 + h, r8 >> 2) + (r8 & 3) * 4);
 
-  const Cut cut = make_cut(p, qt, n_units, per_group, line, warps, blockIdx.x == 0);
+  const Cut cut = make_cut<WARPS>(p, qt, n_units, per_group, line, warps, blockIdx.x == 0);
   // a seq_start that goes back may name more tokens than there are rows: nothing is computed
   const bool sane = !p.seq_start || (int64_t)cut.tiles <= (int64_t)(p.n_rows / qt) + n_units;
   if (threadIdx.x == 0) {
@@ -1064,10 +1071,12 @@ int check_q8_attention(const char* name, const Q8AttnParams& p, int hd, int cach
   B2_CHECK_ARG(p.n_rows >= 0 && p.nq > 0 && p.nkv > 0 && p.nq % p.nkv == 0, "%s: bad head counts", name);
   B2_CHECK_ARG(valid_dtype(dtype), "%s: bad dtype", name);
   B2_CHECK_ARG(valid_q8_dtype(cache_dtype), "%s: bad cache dtype", name);
-  B2_CHECK_ARG(p.num_blocks > 0 && p.table_stride > 0 && p.table_rows > 0 && layer >= 0, "%s: bad cache geometry", name);
+  B2_CHECK_ARG(p.num_blocks > 0 && p.table_stride > 0 && p.table_rows > 0 && layer >= 0, "%s: bad cache geometry",
+               name);
   B2_CHECK_ARG(p.table_stride <= 0x7fffffff / kQ8Block, "%s: table_stride %d too large", name, p.table_stride);
   if (bs != kQ8Block) return fail(B2_ENOTSUP, "%s: block_size %d (16 only)", name, bs);
-  if (hd != 32 && hd != 64 && hd != 128) return fail(B2_ENOTSUP, "%s: head_dim %d not supported (32, 64, 128)", name, hd);
+  if (hd != 32 && hd != 64 && hd != 128)
+    return fail(B2_ENOTSUP, "%s: head_dim %d not supported (32, 64, 128)", name, hd);
   if (p.nq / p.nkv > 16) return fail(B2_ENOTSUP, "%s: nq/nkv = %d not supported (1..16)", name, p.nq / p.nkv);
   B2_CHECK_ARG(p.ld_q >= (int64_t)p.nq * hd && p.ld_out >= (int64_t)p.nq * hd, "%s: row strides too small", name);
   return B2_OK;

@@ -112,7 +112,8 @@ __device__ __forceinline__ void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
     const uint32_t u = w ^ 0x80808080u;
     uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
     const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));  // 1152
-    const __half2 ha = __hsub2(*reinterpret_cast<__half2*>(&a), bias), hb = __hsub2(*reinterpret_cast<__half2*>(&b), bias);
+    const __half2 ha = __hsub2(*reinterpret_cast<__half2*>(&a), bias);
+    const __half2 hb = __hsub2(*reinterpret_cast<__half2*>(&b), bias);
     lo = *reinterpret_cast<const uint32_t*>(&ha);
     hi = *reinterpret_cast<const uint32_t*>(&hb);
   } else {

@@ -15,8 +15,8 @@
 //
 // Measured (heads 32/8 of 128, in a graph): bf16 cache, 16 384 tokens: 95 us, 404 MB at 4.3 TB/s (bound by
 // the issue of instructions, 0.65 of the copy's rate); 8 tokens: 2.5 us.  int8 cache and the read-back of 128 blocks:
-// 128 tokens 10.9 us, two launches and their chains of loads.  e4m3 cache, 3 815 ragged tokens of heads 32/4 of 64, with
-// the read-back: 32 us.
+// 128 tokens 10.9 us, two launches and their chains of loads.  e4m3 cache, 3 815 ragged tokens of heads 32/4
+// of 64, with the read-back: 32 us.
 //
 // 8-bit tiles.  The tokens of a call that fall into one block form a run; one warp per (run,
 // head) holds the run's values in registers, takes their largest magnitude and writes codes
@@ -80,12 +80,16 @@ __device__ __forceinline__ void st8(__nv_bfloat16* p, const float (&v)[8]) {
 // product with a packed sum in spite of their .rn.)
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   float2 d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(d)) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
   return d;
 }
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   float2 d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(d)) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
   return d;
 }
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -329,7 +333,8 @@ __device__ __forceinline__ void tile_block(const NormRopeParams& p, int64_t bloc
       if (have[it]) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float x = reinterpret_cast<const float(&)[8]>(lo[it])[e], y = reinterpret_cast<const float(&)[8]>(hi[it])[e];
+          const float x = reinterpret_cast<const float(&)[8]>(lo[it])[e];
+          const float y = reinterpret_cast<const float(&)[8]>(hi[it])[e];
           amax = fmaxf(amax, fmaxf(fabsf(x), fabsf(y)));
           bad |= !(fabsf(x) <= 3.402823466e38f) || !(fabsf(y) <= 3.402823466e38f);
         }
@@ -373,8 +378,8 @@ __device__ __forceinline__ void tile_block(const NormRopeParams& p, int64_t bloc
       __syncwarp();  // every lane has read the old scale
     }
     const float inv = scale > 0.f ? 1.f / scale : 0.f;  // 0 for a tile of zeros and for NaN
-    // A poisoned run's codes are 0: no NaN code is stored, since a product with it would also reach rows that do
-    // not see its tile.
+    // A poisoned run's codes are 0: no NaN code is stored, since a product with it would also reach
+    // rows that do not see its tile.
 #pragma unroll
     for (int it = 0; it < ITERS; ++it) {
       if (!have[it]) continue;
@@ -429,7 +434,8 @@ __global__ void __launch_bounds__(128) kv_read_q8_kernel(const uint8_t* k_cache,
   for (int kv = 0; kv < 2; ++kv) {
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (ok) {
-      const uint2 c = *reinterpret_cast<const uint2*>((kv ? v_cache : k_cache) + q8_tile(blk, nkv, g, hd) + slot * hd + d);
+      const uint8_t* tile = (kv ? v_cache : k_cache) + q8_tile(blk, nkv, g, hd);
+      const uint2 c = *reinterpret_cast<const uint2*>(tile + slot * hd + d);
       const float s = (kv ? v_scale : k_scale)[q8_scale(blk, nkv, g)];
       float a[4];
       Q8<CODE>::decode4(c.x, a);
@@ -446,7 +452,8 @@ __global__ void __launch_bounds__(128) kv_read_q8_kernel(const uint8_t* k_cache,
 int check_norm_rope(const char* name, const NormRopeParams& p, int hd, int layer, int dtype) {
   B2_CHECK_ARG(p.n_tokens >= 0 && p.nq > 0 && p.nkv > 0, "%s: bad head counts", name);
   B2_CHECK_ARG(valid_dtype(dtype), "%s: bad dtype", name);
-  if (hd != 32 && hd != 64 && hd != 128) return fail(B2_ENOTSUP, "%s: head_dim %d not supported (32, 64, 128)", name, hd);
+  if (hd != 32 && hd != 64 && hd != 128)
+    return fail(B2_ENOTSUP, "%s: head_dim %d not supported (32, 64, 128)", name, hd);
   B2_CHECK_ARG(p.ld_qkv >= ((int64_t)p.nq + 2 * (int64_t)p.nkv) * hd, "%s: ld_qkv too small", name);
   B2_CHECK_ARG(p.num_blocks > 0 && p.bs > 0 && p.table_stride > 0 && p.table_rows > 0 && layer >= 0 &&
                    p.max_seq_len > 0, "%s: bad cache geometry", name);
