@@ -48,6 +48,7 @@
 
 namespace b2 {
 
+bool prefill_q8_tc_serves(int rep);
 int prefill_attention_q8_tc(const void* q, int64_t ld_q, int n_rows, int nq, int nkv, const uint8_t* k_cache,
                             const uint8_t* v_cache, const float* k_scale, const float* v_scale, int cache_dtype,
                             int num_blocks, const int32_t* tables, int table_stride, const int32_t* seq_start,
@@ -1103,9 +1104,10 @@ int check_q8_pointers(const char* name, const Q8AttnParams& p, int dtype) {
 //   heads  8/1, 64 sequences, 1 000 keys:    8 tokens   45 /  29,   16   65 /  26,   64  153 /  35
 bool tensor_prefill(int n_rows, int n_seqs, int nq, int nkv, int hd, float scale, int dtype) {
   const int rep = nq / nkv;
-  if (dtype != B2_BF16 || hd != 128 || !(rep == 1 || rep == 2 || rep == 4 || rep == 8) || !(scale > 0.f)) return false;
-  const int64_t columns = ((int64_t)n_rows + n_seqs - 1) / n_seqs * rep;
-  const int64_t tiles = (columns + 31) / 32 * n_seqs * nkv, items = (columns + 255) / 256 * n_seqs * nkv;
+  if (dtype != B2_BF16 || hd != 128 || !prefill_q8_tc_serves(rep) || !(scale > 0.f)) return false;
+  const int64_t tokens = ((int64_t)n_rows + n_seqs - 1) / n_seqs, narrow = 32 / rep, wide = 2 * (128 / rep);
+  const int64_t tiles = (tokens + narrow - 1) / narrow * n_seqs * nkv;
+  const int64_t items = (tokens + wide - 1) / wide * n_seqs * nkv;
   const int64_t sms = sm_count(), rounds = (items + sms - 1) / sms;
   return 3 * tiles >= 4 * sms * rounds;
 }

@@ -225,7 +225,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             continue;
           }
           uint8_t* qs = smem + OFF_Q + (g * 2 + qb) * Q_BYTES;
-          mbar_arrive_expect_tx(&q_full[g][qb], Q_BYTES);
+          // rows behind QT * REP hold what they held: they belong to no token, and a row of Q reaches
+          // only its own row of S and O
+          mbar_arrive_expect_tx(&q_full[g][qb], QT * REP * HD * 2);
           tma_load_3d(qs, &tmQ, &q_full[g][qb], 0, it.g * REP, it.rs + it.t0[g], pol_q);
           tma_load_3d(qs + Q_HALF, &tmQ, &q_full[g][qb], 64, it.g * REP, it.rs + it.t0[g], pol_q);
           ++iq[g];
@@ -672,6 +674,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Launches the tensor-core prefill attention over the 8-bit cache (bf16 q, head_dim 128).
 // k_cache ... v_scale are those of the layer.  Returns B2_ENOTSUP, launching nothing, for shapes
 // it does not serve.
+// Heads to a kv head that the kernel is compiled for.
+bool prefill_q8_tc_serves(int rep) { return (rep >= 1 && rep <= 8) || rep == 12 || rep == 16; }
+
 int prefill_attention_q8_tc(const void* q, int64_t ld_q, int n_rows, int nq, int nkv, const uint8_t* k_cache,
                             const uint8_t* v_cache, const float* k_scale, const float* v_scale, int cache_dtype,
                             int num_blocks, const int32_t* tables, int table_stride, const int32_t* seq_start,
@@ -679,7 +684,7 @@ int prefill_attention_q8_tc(const void* q, int64_t ld_q, int n_rows, int nq, int
                             int32_t* status, cudaStream_t stream) {
   using namespace pftc;
   const int rep = nq / nkv;
-  if (!(rep == 1 || rep == 2 || rep == 4 || rep == 8)) return fail(B2_ENOTSUP, "prefill q8 tc: nq/nkv = %d", rep);
+  if (!prefill_q8_tc_serves(rep)) return fail(B2_ENOTSUP, "prefill q8 tc: nq/nkv = %d", rep);
   if (!(scale > 0.f)) return fail(B2_ENOTSUP, "prefill q8 tc: scale %g", (double)scale);
   ParamsQ8 p{};
   p.n_rows = n_rows;
@@ -714,20 +719,22 @@ int prefill_attention_q8_tc(const void* q, int64_t ld_q, int n_rows, int nq, int
     B2_TRY_CUDA(launch_pdl(k, grid, dim3(kThreads), SMEM, stream, mq, p));
     return B2_OK;
   };
-  if (cache_dtype == B2_I8) {
-    switch (rep) {
-      case 1: return go(prefill_q8_tc_kernel<1, B2_I8>);
-      case 2: return go(prefill_q8_tc_kernel<2, B2_I8>);
-      case 4: return go(prefill_q8_tc_kernel<4, B2_I8>);
-      default: return go(prefill_q8_tc_kernel<8, B2_I8>);
-    }
-  }
+  const bool i8 = cache_dtype == B2_I8;
+#define B2_CASE(REP) \
+  case REP: return go(i8 ? prefill_q8_tc_kernel<REP, B2_I8> : prefill_q8_tc_kernel<REP, B2_E4M3>)
   switch (rep) {
-    case 1: return go(prefill_q8_tc_kernel<1, B2_E4M3>);
-    case 2: return go(prefill_q8_tc_kernel<2, B2_E4M3>);
-    case 4: return go(prefill_q8_tc_kernel<4, B2_E4M3>);
-    default: return go(prefill_q8_tc_kernel<8, B2_E4M3>);
+    B2_CASE(1);
+    B2_CASE(2);
+    B2_CASE(3);
+    B2_CASE(4);
+    B2_CASE(5);
+    B2_CASE(6);
+    B2_CASE(7);
+    B2_CASE(8);
+    B2_CASE(12);
+    default: return go(i8 ? prefill_q8_tc_kernel<16, B2_I8> : prefill_q8_tc_kernel<16, B2_E4M3>);
   }
+#undef B2_CASE
 }
 
 }  // namespace b2

@@ -736,7 +736,8 @@ def test_prefill_attention_q8_long(code, nq, nkv, lens, ctx0):
 
 
 @pytest.mark.parametrize("code", ["int8", "e4m3"])
-@pytest.mark.parametrize("nq,nkv", [(16, 16), (16, 8), (16, 4), (16, 2)])
+@pytest.mark.parametrize("nq,nkv", [(16, 16), (16, 8), (16, 4), (16, 2), (15, 5), (20, 4), (18, 3), (14, 2), (24, 2),
+                                    (32, 2)])
 def test_prefill_attention_q8_many_rows(code, nq, nkv):
     """Enough rows for the tcgen05 kernel at every number of heads to a kv head, with what may go wrong in it: an
     empty sequence, scales that differ by 2^40 and are 0, pages outside the pool, NaN codes behind the context,

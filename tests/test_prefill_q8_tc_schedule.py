@@ -138,7 +138,7 @@ def simulate(work, seed):
     return False
 
 
-@pytest.mark.parametrize("qt", [16, 32, 128])
+@pytest.mark.parametrize("qt", [16, 18, 32, 128])
 @pytest.mark.parametrize("lens,ctx0", [([1], [0]), ([5, 130, 77], [0, 17, 0]), ([300, 1, 64, 65], [200, 0, 0, 9])])
 def test_protocol_finishes_without_early_reuse(qt, lens, ctx0):
     work = [tiles for _, _, tiles in items(lens, ctx0, qt, 1)]
