@@ -15,7 +15,7 @@
 //
 // Measured (heads 32/8 of 128, in a graph): bf16 cache, 16 384 tokens: 95 us, 404 MB at 4.3 TB/s (bound by
 // the issue of instructions, 0.65 of the copy's rate); 8 tokens: 2.5 us.  int8 cache and the read-back of 128 blocks:
-// 128 tokens 10.9 us, two launches and their chains of loads.  e4m3 cache, 3 815 ragged tokens of heads 32/4
+// 128 tokens 10.9 us, two launches and their chains of loads.  e4m3 cache, 7 947 ragged tokens of heads 32/4
 // of 64, with the read-back: 32 us.
 //
 // 8-bit tiles.  The tokens of a call that fall into one block form a run; one warp per (run,
@@ -24,6 +24,8 @@
 // keeps its old scale if that is larger, else the old codes are rounded again under the new
 // one (code * old / new, to nearest), which a tile's growing maximum makes ever rarer.
 #include "q8.cuh"
+
+#include <algorithm>
 
 namespace b2 {
 namespace {
@@ -404,7 +406,7 @@ __device__ __forceinline__ void tile_block(const NormRopeParams& p, int64_t bloc
 }
 
 // Tiles and q heads in one launch: they have nothing to do with each other, and the tiles' chains of
-// loads hide behind the q heads' traffic (bf16 ragged prefill of 3 815 tokens, 32 and 8 heads of 128: 32 us,
+// loads hide behind the q heads' traffic (bf16 ragged prefill of 7 947 tokens, heads 32/4 of 64: 32 us,
 // in two launches 52; 3 CTAs per SM 38, 5 spill and take 36).
 template <typename T, int HD, int CODE>
 __global__ void __launch_bounds__(128, 4) qk_norm_rope_q8_kernel(NormRopeParams p) {
@@ -472,7 +474,7 @@ int check_norm_rope(const char* name, const NormRopeParams& p, int hd, int layer
 }
 
 // Heads per lane group.  More of them share one reading of the token's angles (16 384 tokens of 48
-// heads: 214 us with 1, 139 with 2, 120 with 4, 119 with 8; 16 no faster); fewer keep 64 or more lane
+// heads, 4 CTAs per SM: 123 us with 2, 109 with 4, 106 with 8, 107 with 16); fewer keep 64 or more lane
 // groups per SM when tokens are few.
 int heads_per_group(int n_tokens, int heads) {
   int h = 1;
@@ -500,9 +502,12 @@ int launch_rope(NormRopeParams& p, cudaStream_t s) {
 template <typename T, int HD>
 int launch_q8(NormRopeParams& p, int cache_dtype, cudaStream_t s) {
   p.heads = heads_per_group(p.n_tokens, p.nq);
-  // One token's runs per block while that fills the GPU.  A long prefill has one run in sixteen tokens:
-  // 3 815 tokens take 33 us in chunks of 16, 35 in chunks of 8, 41 in chunks of 4.
-  p.chunk = p.n_tokens >= 2048 ? 16 : p.n_tokens >= 512 ? 4 : 1;
+  // A warp looks for the runs of `chunk` tokens with one load and works them off in turn, so a chunk should hold
+  // about one run: the mean length of a table row's tokens, and more where there are chunks enough.  In us, heads
+  // 32/8 of 128, in chunks of 1 / 4 / 16: 4 prompts of 64 tokens 7.2 / 6.3 / 7.1, of 512 28 / 16 / 13, of 2 048
+  // 131 / 73 / 57; one token each for 256 rows 11 / 20 / 51, 1 024 rows 34 / 32 / 66, 4 096 rows 133 / 107 / 114
+  // (8: 101).
+  p.chunk = std::min(16, std::max({1, p.n_tokens / p.table_rows, std::min(8, p.n_tokens / 512)}));
   const int64_t tiles = (int64_t)((p.n_tokens + p.chunk - 1) / p.chunk) * ((2 * p.nkv + 3) / 4);
   const int64_t grid = tiles + rope_blocks<HD>(p, p.nq);
   B2_CHECK_ARG(grid <= 0x7fffffff, "qk_norm_rope: %d tokens are too many for one call", p.n_tokens);
