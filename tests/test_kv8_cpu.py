@@ -134,3 +134,16 @@ def test_device_block_tables_refusals():
     for bad in ([1, 2], torch.ones(3, dtype=torch.int64), torch.ones(2, dtype=torch.int32)):
         with pytest.raises(ValueError, match="per sequence slot"):
             bt.truncate(bad)
+
+
+def test_norms_of_q_and_k_are_the_same_on_every_rank():
+    import torch
+    from pythonintern_b200.tensor_parallel.sharding import WeightSharder
+    state = {"layers.0.self_attn.q_norm.weight": torch.arange(8.0), "layers.0.self_attn.k_norm.weight": torch.ones(8),
+             "layers.0.self_attn.q_proj.weight": torch.zeros(16, 32)}
+    for rank in range(2):
+        shard = WeightSharder(2).shard_full_model_state_dict(state, rank)
+        for n in "qk":
+            key = f"layers.0.self_attn.{n}_norm.weight"
+            assert torch.equal(shard[key], state[key])
+        assert shard["layers.0.self_attn.q_proj.weight"].shape == (16, 16)
