@@ -138,11 +138,12 @@ def test_device_block_tables_refusals():
 
 def test_norms_of_q_and_k_are_the_same_on_every_rank():
     import torch
+    from pythonintern_b200.config import ModelConfig
     from pythonintern_b200.tensor_parallel.sharding import WeightSharder
     state = {"layers.0.self_attn.q_norm.weight": torch.arange(8.0), "layers.0.self_attn.k_norm.weight": torch.ones(8),
              "layers.0.self_attn.q_proj.weight": torch.zeros(16, 32)}
     for rank in range(2):
-        shard = WeightSharder(2).shard_full_model_state_dict(state, rank)
+        shard = WeightSharder(ModelConfig(hidden_dim=32, num_heads=4, num_kv_heads=2), 2).shard_full_model_state_dict(state, rank)
         for n in "qk":
             key = f"layers.0.self_attn.{n}_norm.weight"
             assert torch.equal(shard[key], state[key])
