@@ -786,7 +786,17 @@ q8_attn_kernel(const Q8AttnParams p, int qt, int n_units, int per_group) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[0][e] += s_odd[0][e];
       }
-      // scores; the tail of the tile's keys is masked per column
+      const float lv = vs == 0.f ? -INFINITY : __log2f(vs);  // only places a reference: approximate
+      // scores; the tail of the tile's keys is masked per column, after the scaling: a factor that is 0
+      // (a tile of zeros, a head next to zeros), negative or NaN would not leave a masked score at -inf
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float cs = colscale[nt][e] * ks, c0 = C::BIASED ? bias[nt][e] * cs : 0.f;
+          s[nt][e] = fmaf(s[nt][e], cs, c0);
+          s[nt][2 + e] = fmaf(s[nt][2 + e], cs, c0);
+        }
       if (tail) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -796,19 +806,12 @@ q8_attn_kernel(const Q8AttnParams p, int qt, int n_units, int per_group) {
             if (key0 + r8 + 8 > lim[nt][e]) s[nt][2 + e] = -INFINITY;
           }
       }
-      const float lv = vs == 0.f ? -INFINITY : __log2f(vs);  // only places a reference: approximate
       bool move = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          // a column that sees none of the block's keys takes nothing from its scales
-          const float cs = tail && key0 > lim[nt][e] ? 1.f : colscale[nt][e] * ks;
-          const float c0 = C::BIASED ? bias[nt][e] * cs : 0.f;
-          s[nt][e] = fmaf(s[nt][e], cs, c0);
-          s[nt][2 + e] = fmaf(s[nt][2 + e], cs, c0);
+        for (int e = 0; e < 2; ++e)
           move |= fmaxf(s[nt][e], s[nt][2 + e]) > fminf(m[nt][e], m2[nt][e] - lv) + kRoom;
-        }
       if (__any_sync(0xffffffffu, move)) {  // references move, to 2^8 below their columns' largest
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -839,6 +842,7 @@ q8_attn_kernel(const Q8AttnParams p, int qt, int n_units, int per_group) {
           pa[e] = ex2(s[nt][e] - m[nt][e]);  // -inf gives 0
           pc[e] = ex2(s[nt][2 + e] - m[nt][e]);
           l[nt][e] += pa[e] + pc[e];
+          // a column that sees none of the block's keys takes nothing from its scale
           const float f = vs == 0.f || (tail && key0 > lim[nt][e]) ? 0.f : vs * lift[nt][e];
           pa[e] *= f;
           pc[e] *= f;
