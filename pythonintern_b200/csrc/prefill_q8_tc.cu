@@ -37,7 +37,9 @@ static_assert(SMEM + 8 * kSeqCache + 512 <= 232448, "shared memory above the 227
 constexpr float kRoom = 15.f;  // log2 of the largest P
 constexpr float kLift = 8.f;   // log2 of P's largest value when a reference has just moved
 
-constexpr float kTiny = 1e-37f;  // stands for a K scale of 0: -inf * 0 is not -inf
+// Stands for a factor of the scores that is 0 (a K scale of 0, or one whose product with the call's scale rounds to
+// 0): -inf * 0 is not -inf.  The smallest number, so that no sum of codes it multiplies becomes a score to speak of.
+constexpr float kTiny = 0x1p-149f;
 
 struct ParamsQ8 : Params {
   const uint8_t* k_cache;
@@ -411,7 +413,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int b = js & 1;
         const int k0 = j * KT;
         // the scales were fetched a tile ago: their latency is behind the last tile's work
-        const float kc_own = id_raw < 0 ? -1.f : ks_raw == 0.f ? kTiny : ks_raw * p.scale_log2;
+        const float factor = ks_raw * p.scale_log2;
+        const float kc_own = id_raw < 0 ? -1.f : factor == 0.f ? kTiny : factor;
         float kc[KT / 16], vs[KT / 16];
         bool gap = false;  // a block of the tile is outside the pool
 #pragma unroll

@@ -105,3 +105,15 @@ def test_masked_keys_of_many_prefill_rows_stay_masked(what, code):
     tab, cache, q, scale = _masked_inputs(what, code, torch.bfloat16, nq, nkv, hd, sum(lens), seen, 5)
     out, rows = _prefill(q, nq, nkv, hd, cache, tab, lens, ctx0, scale)
     _check_rows(out, q, cache, tab, rows[::23] + rows[190:202] + rows[-12:], scale, torch.bfloat16)
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_a_scale_next_to_0_weighs_all_keys_alike(code):
+    """scale * K scale rounds to 0: every visible key has the same score, the masked ones none."""
+    nq, nkv, hd, scale = 32, 16, 128, 1e-44
+    for lens, ctx0 in (([200, 250], [33, 7]), ([3, 2], [30, 7])):
+        tab, NB = _tables_for([-(-(c + n) // 16) for c, n in zip(ctx0, lens)], 2, 1)
+        cache = _stored(code, NB, nkv, hd, seed=2)
+        q = torch.randn(sum(lens), nq * hd, generator=gen(3)).to(DEV, torch.bfloat16)
+        out, rows = _prefill(q, nq, nkv, hd, cache, tab, lens, ctx0, scale)
+        _check_rows(out, q, cache, tab, rows[::23] + rows[-5:], scale, torch.bfloat16)
