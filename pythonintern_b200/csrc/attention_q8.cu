@@ -378,6 +378,9 @@ __device__ __forceinline__ void widen4(const uint2& a, float (&v)[4]) {
 constexpr float kRoom = 15.f;       // log2 of the largest P
 constexpr float kLift = 8.f;        // log2 of the largest P when a reference has just moved
 constexpr float kNoRef = -1e30f;    // reference of a column that has seen no key
+// m2 is held within 2^kGap of m, which runs ahead of it where V tiles of scale 0 hold the loudest keys: 2^(m - m2)
+// stays finite, and what float16 cuts off P (2^-25) is 2^-133 of a code, since l is 2^8 or more.
+constexpr float kGap = 100.f;
 
 // One CTA per SM, of as many warps as its registers allow (decode of 128 rows over 2 048 keys, 8 heads of 128: 100 us
 // with 12 warps; 16 of them spill), each with a ring of three tiles of K and V: a fourth is no faster, nor
@@ -820,7 +823,9 @@ q8_attn_kernel(const Q8AttnParams p, int qt, int n_units, int per_group) {
             float mx = fmaxf(s[nt][e], s[nt][2 + e]);
 #pragma unroll
             for (int sh = 4; sh < 32; sh <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, sh));
-            const float mn = fmaxf(m[nt][e], mx - kLift), m2n = fmaxf(m2[nt][e], mx - kLift + lv);
+            const float mn = fmaxf(m[nt][e], mx - kLift);
+            float m2n = fmaxf(m2[nt][e], mx - kLift + lv);
+            if (m2n != kNoRef) m2n = fmaxf(m2n, mn - kGap);
             l[nt][e] *= ex2(m[nt][e] - mn);
             const float c = ex2(m2[nt][e] - m2n);
             m[nt][e] = mn;
@@ -842,8 +847,9 @@ q8_attn_kernel(const Q8AttnParams p, int qt, int n_units, int per_group) {
           pa[e] = ex2(s[nt][e] - m[nt][e]);  // -inf gives 0
           pc[e] = ex2(s[nt][2 + e] - m[nt][e]);
           l[nt][e] += pa[e] + pc[e];
-          // a column that sees none of the block's keys takes nothing from its scale
-          const float f = vs == 0.f || (tail && key0 > lim[nt][e]) ? 0.f : vs * lift[nt][e];
+          // a column that sees none of the block's keys takes nothing from its scale.  Where the product would
+          // overflow, the exponentials it meets are 2^-112 or less: keys of less than 2^-120 of the softmax.
+          const float f = vs == 0.f || (tail && key0 > lim[nt][e]) ? 0.f : q8_finite(vs * lift[nt][e]);
           pa[e] *= f;
           pc[e] *= f;
         }

@@ -36,6 +36,9 @@ constexpr size_t SMEM = OFF_Q + NG * 2 * Q_BYTES + 1024;
 static_assert(SMEM + 8 * kSeqCache + 512 <= 232448, "shared memory above the 227 KB a CTA may use");
 constexpr float kRoom = 15.f;  // log2 of the largest P
 constexpr float kLift = 8.f;   // log2 of P's largest value when a reference has just moved
+// m2 is held within 2^kGap of m, which runs ahead of it where V tiles of scale 0 hold the loudest keys: 2^(m - m2)
+// stays finite, and what f16 cuts off P (2^-25) is 2^-133 of a code, since l is 2^8 or more.
+constexpr float kGap = 100.f;
 
 // Stands for a factor of the scores that is 0 (a K scale of 0, or one whose product with the call's scale rounds to
 // 0): -inf * 0 is not -inf.  The smallest number, so that no sum of codes it multiplies becomes a score to speak of.
@@ -466,7 +469,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool need = false;
         float corr = 1.f;
         if (mx > m_ref + kRoom || mx2 > m2_ref + kRoom) {
-          const float mn = fmaxf(m_ref, mx - kLift), m2n = fmaxf(m2_ref, mx2 - kLift);
+          const float mn = fmaxf(m_ref, mx - kLift);
+          float m2n = fmaxf(m2_ref, mx2 - kLift);
+          if (m2n != -INFINITY) m2n = fmaxf(m2n, mn - kGap);
           l_run *= exp2f(m_ref - mn);  // from -inf: times 0, and l_run is 0
           if (m2_ref != -INFINITY) {   // else the row's O is empty
             need = m2n != m2_ref;
@@ -504,7 +509,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           // the next S tile this group consumes (in this item or the next): ask now, so that the
           // answer has arrived when this tile is done
           if (u == 1) peek(pk_s, &s_full[grp][(js + 1) & 1], (uint32_t)((js + 1) >> 1) & 1u);
-          const float f = vs[u] == 0.f ? 0.f : vs[u] * lift;
+          // where the product would overflow, the exponentials it meets are 2^-112 or less (2^-120 of the softmax)
+          const float f = vs[u] == 0.f ? 0.f : q8_finite(vs[u] * lift);
           const uint64_t k2 = pack2(kc[u], kc[u]), f2 = pack2(f, f);
           uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll

@@ -70,4 +70,11 @@ __device__ __forceinline__ int64_t q8_tile(int64_t block, int nkv, int head, int
 }
 __device__ __forceinline__ int64_t q8_scale(int64_t block, int nkv, int head) { return block * nkv + head; }
 
+// x, or the largest number where x is infinite; a NaN stays one.
+__device__ __forceinline__ float q8_finite(float x) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(3.402823466e38f));
+  return y;
+}
+
 }  // namespace b2

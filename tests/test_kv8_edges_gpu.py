@@ -117,3 +117,70 @@ def test_a_scale_next_to_0_weighs_all_keys_alike(code):
         q = torch.randn(sum(lens), nq * hd, generator=gen(3)).to(DEV, torch.bfloat16)
         out, rows = _prefill(q, nq, nkv, hd, cache, tab, lens, ctx0, scale)
         _check_rows(out, q, cache, tab, rows[::23] + rows[-5:], scale, torch.bfloat16)
+
+
+# ------------------------------------------------------------------ value tiles of scale 0 under the loudest keys
+def _loud_zero_values(code, nkv, hd, blocks, loud, gap, seed):
+    """One sequence of `blocks` full blocks whose keys score -gap / 2 bits, but for block `loud`: +gap / 2, and a
+    value tile of zeros.  Queries of all ones score so with scale 1."""
+    tab, NB = _tables_for([blocks], 2, seed)
+    cache = _stored(code, NB, nkv, hd, seed=seed)
+    cache[0].zero_()
+    one = 64 if code == "int8" else 0x38  # e4m3: 1.0
+    cache[0].view(torch.uint8)[...] = (256 - one) if code == "int8" else one | 0x80
+    cache[2].fill_(gap / 2 * math.log(2) / hd / (64 if code == "int8" else 1))
+    b = int(tab[0, loud])
+    cache[0].view(torch.uint8)[0, b] = one
+    cache[1].view(torch.uint8)[0, b] = 0
+    cache[3][0, b] = 0
+    return tab, cache
+
+
+def _close_to_next_to_nothing(got, want, size, cache, dtype):
+    """As _close, for weights far below 1.  Scores of up to 2^7 bits err by 2^-14 of a weight.  The value reference
+    is held within 2^100 of the score reference, where the loudest key weighs 2^8 or more: float16's half step of
+    2^-25 leaves 2^-133 of a code, and a weight whose exponential is below 2^-126 counts as 0 (2^-134 of a value).
+    The output's own half step below its normal numbers is 2^-134 (bf16) or 2^-150."""
+    size, small = size
+    out = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24
+    prob = 2.0 ** -11 if dtype == torch.bfloat16 else 2.0 ** -22
+    code = cache[1].double().abs().sum((2, 3, 4)).max().item()
+    value = code * cache[3].double().max().item()
+    assert torch.isfinite(got).all()
+    limit = (out * want.abs() + (prob + 2.0 ** -14) * size + 2.0 ** -33 * small + 2.0 ** -133 * code
+             + 2.0 ** -134 * value + 2.0 ** -134)
+    err = (got.double().cpu() - want).abs()
+    assert (err <= limit * 1.01).all(), float((err / limit).max())
+
+
+@pytest.mark.parametrize("gap", [40, 110, 131, 150, 260])
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_zero_values_under_the_loudest_keys(code, dtype, gap):
+    nq, nkv, hd = 4, 2, 64
+    for blocks, loud in ((2, 0), (2, 1), (10, 0), (10, 5), (10, 9), (300, 7)):
+        tab, cache = _loud_zero_values(code, nkv, hd, blocks, loud, gap, blocks)
+        ctx = 16 * blocks
+        q = torch.ones(3, nq * hd, dtype=dtype, device=DEV)
+        want, size = _attend64(q[0], cache, 0, tab[0].tolist(), ctx, 1.0)
+        out = kernels.paged_attention_q8(q, nq, nkv, hd, *cache, 0, torch.from_numpy(tab).to(DEV), i32([0, 0, 0]),
+                                         i32([ctx] * 3), False, 1.0)
+        _lib.check_device_status(DEV, "decode")
+        _close_to_next_to_nothing(out[1], want, size, cache, dtype)
+        out, rows = _prefill(q, nq, nkv, hd, cache, tab, [3], [ctx - 3], 1.0)
+        _close_to_next_to_nothing(out[2], want, size, cache, dtype)
+
+
+@pytest.mark.parametrize("gap", [40, 110, 131, 150, 260])
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_zero_values_under_the_loudest_keys_of_many_rows(code, gap):
+    """Enough rows for the tcgen05 kernel; the loud block in the first tile, within it behind others, and later."""
+    nq, nkv, hd, blocks = 32, 16, 128, 25
+    for loud in (0, 2, 3, 9, 24):
+        tab, cache = _loud_zero_values(code, nkv, hd, blocks, loud, gap, blocks)
+        n = 16 * blocks
+        q = torch.ones(n, nq * hd, dtype=torch.bfloat16, device=DEV)
+        out, rows = _prefill(q, nq, nkv, hd, cache, tab, [n], [0], 1.0)
+        for r in (0, 15, 16, 63, 64, 200, n - 1):
+            want, size = _attend64(q[r], cache, 0, tab[0].tolist(), r + 1, 1.0)
+            _close_to_next_to_nothing(out[r], want, size, cache, torch.bfloat16)
