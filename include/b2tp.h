@@ -258,6 +258,14 @@ int b2_block_tables_extend(int32_t* block_tables, int n_seqs, int table_stride, 
                            int32_t* free_state, int max_tokens, int32_t* seq_start, int64_t* positions,
                            int32_t* table_index, int64_t* slots, int32_t* ctx_lens, int64_t* last_rows,
                            int32_t* status, b2_stream_t stream);
+/* extend that writes all max_tokens entries of the maps: those behind the total, and all of a call that cannot be
+ * served, name no token (positions, slots and last_rows -1, table_index, ctx_lens and seq_start 0), so kernels that
+ * run on the maps before *status is read find nothing to do there. */
+int b2_block_tables_extend_filled(int32_t* block_tables, int n_seqs, int table_stride, int32_t* lens,
+                                  const int32_t* new_lens, int block_size, int32_t* free_ring, int num_blocks,
+                                  int32_t* free_state, int max_tokens, int32_t* seq_start, int64_t* positions,
+                                  int32_t* table_index, int64_t* slots, int32_t* ctx_lens, int64_t* last_rows,
+                                  int32_t* status, b2_stream_t stream);
 int b2_block_tables_truncate(int32_t* block_tables, int n_seqs, int table_stride, int32_t* lens,
                              const int32_t* keep_lens, int block_size, int32_t* free_ring, int num_blocks,
                              int32_t* free_state, int32_t* status, b2_stream_t stream);

@@ -95,6 +95,9 @@ _SIGS = {
     "b2_block_tables_extend": (_c_int, [_c_void_p, _c_int, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p,
                                         _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
                                         _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
+    "b2_block_tables_extend_filled": (_c_int, [_c_void_p, _c_int, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p,
+                                               _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
+                                               _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
     "b2_block_tables_truncate": (_c_int, [_c_void_p, _c_int, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p,
                                           _c_int, _c_void_p, _c_void_p, _c_void_p]),
     "b2_qk_norm_rope_kv_write": (_c_int, [_c_void_p, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_void_p,
@@ -165,8 +168,8 @@ _LAUNCHING = {"b2_embedding", "b2_rmsnorm", "b2_linear", "b2_linear_qkv", "b2_li
               "b2_row_parallel_linear", "b2_allreduce_rmsnorm_sharded", "b2_paged_attention_noalloc",
               "b2_argmax_allgather", "b2_linear_residual_norm", "b2_linear_qkv_rownorm", "b2_linear_swiglu_rownorm",
               "b2_linear_qkv_rope_kv", "b2_prefill_attention", "b2_prefill_attention_tc", "b2_block_tables_extend",
-              "b2_block_tables_truncate", "b2_qk_norm_rope_kv_write", "b2_qk_norm_rope_kv_write_q8", "b2_kv_read_q8",
-              "b2_paged_attention_q8", "b2_prefill_attention_q8"}
+              "b2_block_tables_extend_filled", "b2_block_tables_truncate", "b2_qk_norm_rope_kv_write",
+              "b2_qk_norm_rope_kv_write_q8", "b2_kv_read_q8", "b2_paged_attention_q8", "b2_prefill_attention_q8"}
 
 
 def check(rc: int, what: str = ""):

@@ -50,6 +50,7 @@ struct TablesParams {
   int64_t* slots;
   int32_t* ctx_lens;
   int64_t* last_rows;
+  bool fill;  // extend: entries of no token are written too
   int32_t* status;
 };
 
@@ -95,6 +96,16 @@ __device__ __forceinline__ int find_seq(const int* prefix, int n, int x) {
 __device__ __forceinline__ int64_t ring_slot(const TablesParams& p, int64_t head, int64_t x) {
   const int64_t at = head + x;
   return at >= p.num_blocks ? at - p.num_blocks : at;
+}
+
+// Map entries i and on, as those of no token.
+__device__ __forceinline__ void fill_from(const TablesParams& p, int64_t i) {
+  for (i += (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < p.max_tokens; i += (int64_t)gridDim.x * blockDim.x) {
+    p.positions[i] = -1;
+    p.table_index[i] = 0;
+    p.slots[i] = -1;
+    p.ctx_lens[i] = 0;
+  }
 }
 
 template <bool EXTEND>
@@ -165,6 +176,14 @@ __global__ void __launch_bounds__(kMaxThreads) block_tables_kernel(TablesParams 
   }
   if (error) {  // every CTA finds the same: nothing is changed
     if (blockIdx.x == 0 && tid == 0) raise_status(p.status, error);
+    if (EXTEND && p.fill) {  // the maps of a step without tokens
+      if (blockIdx.x == 0)
+        for (int s = tid; s <= p.n_seqs; s += threads) {
+          p.seq_start[s] = 0;
+          if (s < p.n_seqs) p.last_rows[s] = -1;
+        }
+      fill_from(p, 0);
+    }
     return;
   }
   for (int s = s0; s < s1; ++s) {
@@ -182,6 +201,7 @@ __global__ void __launch_bounds__(kMaxThreads) block_tables_kernel(TablesParams 
     base_i += n;
   }
   if (EXTEND && blockIdx.x == 0 && tid == 0) p.seq_start[p.n_seqs] = (int)total;
+  if (EXTEND && p.fill) fill_from(p, total);
   __syncthreads();
 
   const int64_t step = (int64_t)gridDim.x * threads * kPerThread;
@@ -273,27 +293,19 @@ int launch(const TablesParams& p, int64_t items_bound, cudaStream_t stream) {
   return B2_OK;
 }
 
-}  // namespace
-}  // namespace b2
-
-extern "C" {
-
-int b2_block_tables_extend(int32_t* block_tables, int n_seqs, int table_stride, int32_t* lens,
-                           const int32_t* new_lens, int block_size, int32_t* free_ring, int num_blocks,
-                           int32_t* free_state, int max_tokens, int32_t* seq_start, int64_t* positions,
-                           int32_t* table_index, int64_t* slots, int32_t* ctx_lens, int64_t* last_rows,
-                           int32_t* status, b2_stream_t stream) {
+int extend(const char* name, bool fill, int32_t* block_tables, int n_seqs, int table_stride, int32_t* lens,
+           const int32_t* new_lens, int block_size, int32_t* free_ring, int num_blocks, int32_t* free_state,
+           int max_tokens, int32_t* seq_start, int64_t* positions, int32_t* table_index, int64_t* slots,
+           int32_t* ctx_lens, int64_t* last_rows, int32_t* status, cudaStream_t stream) {
   B2_CHECK_ARG(n_seqs > 0 && table_stride > 0 && block_size > 0 && num_blocks > 0 && max_tokens >= 0,
-               "b2_block_tables_extend: bad sizes");
-  if (n_seqs > b2::kMaxSeqs)
-    return b2::fail(B2_ENOTSUP, "b2_block_tables_extend: %d sequences (at most %d)", n_seqs, b2::kMaxSeqs);
-  B2_CHECK_ARG(block_tables && lens && new_lens && seq_start && last_rows,
-               "b2_block_tables_extend: null pointer");
-  B2_CHECK_ARG(max_tokens == 0 || (positions && table_index && slots && ctx_lens),
-               "b2_block_tables_extend: null map");
+               "%s: bad sizes", name);
+  if (n_seqs > kMaxSeqs)
+    return fail(B2_ENOTSUP, "%s: %d sequences (at most %d)", name, n_seqs, kMaxSeqs);
+  B2_CHECK_ARG(block_tables && lens && new_lens && seq_start && last_rows, "%s: null pointer", name);
+  B2_CHECK_ARG(max_tokens == 0 || (positions && table_index && slots && ctx_lens), "%s: null map", name);
   B2_CHECK_ARG((free_ring == nullptr) == (free_state == nullptr),
-               "b2_block_tables_extend: the free ring and its state come together");
-  b2::TablesParams p{};
+               "%s: the free ring and its state come together", name);
+  TablesParams p{};
   p.tables = block_tables;
   p.n_seqs = n_seqs;
   p.stride = table_stride;
@@ -310,8 +322,34 @@ int b2_block_tables_extend(int32_t* block_tables, int n_seqs, int table_stride, 
   p.slots = slots;
   p.ctx_lens = ctx_lens;
   p.last_rows = last_rows;
+  p.fill = fill;
   p.status = status;
-  return b2::launch<true>(p, max_tokens, stream);
+  return launch<true>(p, max_tokens, stream);
+}
+
+}  // namespace
+}  // namespace b2
+
+extern "C" {
+
+int b2_block_tables_extend(int32_t* block_tables, int n_seqs, int table_stride, int32_t* lens,
+                           const int32_t* new_lens, int block_size, int32_t* free_ring, int num_blocks,
+                           int32_t* free_state, int max_tokens, int32_t* seq_start, int64_t* positions,
+                           int32_t* table_index, int64_t* slots, int32_t* ctx_lens, int64_t* last_rows,
+                           int32_t* status, b2_stream_t stream) {
+  return b2::extend("b2_block_tables_extend", false, block_tables, n_seqs, table_stride, lens, new_lens, block_size,
+                    free_ring, num_blocks, free_state, max_tokens, seq_start, positions, table_index, slots, ctx_lens,
+                    last_rows, status, stream);
+}
+
+int b2_block_tables_extend_filled(int32_t* block_tables, int n_seqs, int table_stride, int32_t* lens,
+                                  const int32_t* new_lens, int block_size, int32_t* free_ring, int num_blocks,
+                                  int32_t* free_state, int max_tokens, int32_t* seq_start, int64_t* positions,
+                                  int32_t* table_index, int64_t* slots, int32_t* ctx_lens, int64_t* last_rows,
+                                  int32_t* status, b2_stream_t stream) {
+  return b2::extend("b2_block_tables_extend_filled", true, block_tables, n_seqs, table_stride, lens, new_lens,
+                    block_size, free_ring, num_blocks, free_state, max_tokens, seq_start, positions, table_index,
+                    slots, ctx_lens, last_rows, status, stream);
 }
 
 int b2_block_tables_truncate(int32_t* block_tables, int n_seqs, int table_stride, int32_t* lens,

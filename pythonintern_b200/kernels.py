@@ -395,9 +395,11 @@ def block_tables_extend(tables: torch.Tensor, lens: torch.Tensor, new_lens: torc
     [n_seqs].  With a free ring (int32 [num_blocks] ids, state int32 [4] = head, count, 0, 0) every
     sequence takes the blocks its new tokens need, FIFO like the host's free list
     (engine/model/kv_cache.py:172-227), and ``lens`` grows; without one (give ``num_blocks``) the
-    tables are taken as they are and only the maps are built.  Map entries behind the step's last
-    token are left as they were.  Too few free blocks (``MemoryError``) or a length out of range
-    (``IndexError``) are reported by ``_lib.check_device_status`` and change nothing.
+    tables are taken as they are and only the maps are built.  Too few free blocks (``MemoryError``)
+    or a length out of range (``IndexError``) are reported by ``_lib.check_device_status`` and
+    change nothing.  Map entries behind the step's last token, and all of a refused call, name no
+    token (positions, slots and last_rows -1, the others 0); in maps given as ``out`` they are left
+    as they were, so what runs before the status is read would take those of an earlier step.
     """
     _check_tables(tables)
     dev = tables.device
@@ -411,19 +413,21 @@ def block_tables_extend(tables: torch.Tensor, lens: torch.Tensor, new_lens: torc
     elif num_blocks is None:
         raise _lib.B2Error("num_blocks is needed without a free ring")
     if out is None:
+        fn = "b2_block_tables_extend_filled"
         i64 = torch.empty(2 * max_tokens + n, dtype=torch.int64, device=dev)
         i32 = torch.empty(2 * max_tokens + n + 1, dtype=torch.int32, device=dev)
         positions, slots, last_rows = i64.unsafe_split_with_sizes((max_tokens, max_tokens, n))
         table_index, ctx_lens, seq_start = i32.unsafe_split_with_sizes((max_tokens, max_tokens, n + 1))
         out = SlotMap(seq_start, positions, table_index, slots, ctx_lens, last_rows)
     else:
+        fn = "b2_block_tables_extend"
         _check(out.seq_start, "seq_start", torch.int32, n + 1, dev)
         _check(out.positions, "positions", torch.int64, max_tokens, dev)
         _check(out.table_index, "table_index", torch.int32, max_tokens, dev)
         _check(out.slots, "slots", torch.int64, max_tokens, dev)
         _check(out.ctx_lens, "ctx_lens", torch.int32, max_tokens, dev)
         _check(out.last_rows, "last_rows", torch.int64, n, dev)
-    _call("b2_block_tables_extend", dev, ptr(tables), n, width, ptr(lens), ptr(new_lens), block_size, ptr(free_ring),
+    _call(fn, dev, ptr(tables), n, width, ptr(lens), ptr(new_lens), block_size, ptr(free_ring),
           num_blocks, ptr(free_state), max_tokens, ptr(out.seq_start), ptr(out.positions), ptr(out.table_index),
           ptr(out.slots), ptr(out.ctx_lens), ptr(out.last_rows))
     return out

@@ -236,16 +236,10 @@ class DeviceBlockTables:
         if n_tokens < 1:
             raise ValueError("a step needs at least one new token")
         new = self._lengths(new_lens)
-        n, dev = self.n_seqs, self.device
-        # maps of a step without tokens, which they stay if it cannot be served
-        i64 = torch.full((2 * n_tokens + n,), -1, dtype=torch.int64, device=dev)
-        i32 = torch.zeros(2 * n_tokens + n + 1, dtype=torch.int32, device=dev)
-        positions, slots, last_rows = i64.split_with_sizes((n_tokens, n_tokens, n))
-        table_index, ctx_lens, seq_start = i32.split_with_sizes((n_tokens, n_tokens, n + 1))
+        n = self.n_seqs
         ctx0 = self.lens.clone()
-        m = kernels.block_tables_extend(
-            self.tables, self.lens, new, n_tokens, self.block_size, self.free_ring, self.free_state,
-            out=kernels.SlotMap(seq_start, positions, table_index, slots, ctx_lens, last_rows))
+        m = kernels.block_tables_extend(self.tables, self.lens, new, n_tokens, self.block_size, self.free_ring,
+                                        self.free_state)
         return TokenMetadata(n_tokens=n_tokens, is_prefill=True, rope_pos=m.positions, store_pos=m.positions,
                              table_index=m.table_index, tables=self.tables, ctx_lens=m.ctx_lens,
                              max_ctx=self.tables.shape[1] * self.block_size, compat_pad=False,

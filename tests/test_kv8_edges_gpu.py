@@ -184,3 +184,40 @@ def test_zero_values_under_the_loudest_keys_of_many_rows(code, gap):
         for r in (0, 15, 16, 63, 64, 200, n - 1):
             want, size = _attend64(q[r], cache, 0, tab[0].tolist(), r + 1, 1.0)
             _close_to_next_to_nothing(out[r], want, size, cache, torch.bfloat16)
+
+
+# ------------------------------------------------------------------ maps that hold more than the step's tokens
+@pytest.mark.parametrize("T", [96, 30001])
+@pytest.mark.parametrize("refused", [False, True])
+def test_map_entries_of_no_token_are_written_by_none(refused, T):
+    """Without maps given, entries behind the step's tokens, and all of a refused call, name no token: a write that
+    runs on them before the status is read leaves the cache as it was."""
+    nq, nkv, hd, bs = 4, 2, 64, 16
+    tables = torch.full((3, 4), -1, dtype=torch.int32, device=DEV)
+    lens, ring, state = i32([0, 0, 0]), i32(list(range(12))), i32([0, 12, 0, 0])
+    # the memory that the next maps get holds those of an earlier step
+    m = kernels.block_tables_extend(tables, lens, i32([40, 16, 40]), T, bs, ring, state)
+    del m
+    new = [40, 0, 100] if refused else [1, 0, 2]
+    m = kernels.block_tables_extend(tables, lens, i32(new), T, bs, ring, state)
+    n = 0 if refused else 3
+    assert (m.positions[n:] == -1).all() and (m.slots[n:] == -1).all()
+    assert (m.table_index[n:] == 0).all() and (m.ctx_lens[n:] == 0).all()
+    if refused:
+        assert (m.seq_start == 0).all() and (m.last_rows == -1).all()
+    else:
+        assert m.positions[:3].tolist() == [40, 40, 41] and m.seq_start.tolist() == [0, 1, 1, 3]
+    qkv = torch.randn(T, (nq + 2 * nkv) * hd, device=DEV).to(torch.bfloat16)
+    cos = sin = torch.ones(64, hd, device=DEV)
+    q = torch.empty(T, nq * hd, dtype=torch.bfloat16, device=DEV)
+    cache = _stored("int8", 12, nkv, hd)
+    before = [t.clone() for t in cache]
+    kernels.qk_norm_rope_kv_write_q8(qkv, nq, nkv, hd, None, None, 1e-5, m.positions, None, m.table_index, tables, cos,
+                                     sin, q, *cache, 0)
+    touched = torch.zeros(12, dtype=torch.bool, device=DEV)
+    if not refused:
+        touched[tables[0, 2]] = touched[tables[2, 2]] = True
+    for t, b in zip(cache, before):
+        assert torch.equal(t[0][~touched], b[0][~touched])
+    with pytest.raises((IndexError, MemoryError)):
+        _lib.check_device_status(DEV, "write")
