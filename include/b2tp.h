@@ -252,7 +252,9 @@ int b2_prefill_attention_tc(const void* q, int64_t ld_q, int n_rows, int nq, int
  *
  * A call that cannot be served whole (a negative length, a sequence past its table row, more
  * than max_tokens tokens, a ring that would overflow: B2_DEV_RANGE; too few free blocks:
- * B2_DEV_NO_BLOCKS) raises its bit in *status and changes nothing, maps included. */
+ * B2_DEV_NO_BLOCKS) raises its bit in *status and changes nothing, maps included.  An id outside
+ * [0, num_blocks) in the ring or among the blocks that a table row holds does not stop a call: it moves as -1, its
+ * tokens get slot -1, and B2_DEV_RANGE is raised. */
 int b2_block_tables_extend(int32_t* block_tables, int n_seqs, int table_stride, int32_t* lens,
                            const int32_t* new_lens, int block_size, int32_t* free_ring, int num_blocks,
                            int32_t* free_state, int max_tokens, int32_t* seq_start, int64_t* positions,

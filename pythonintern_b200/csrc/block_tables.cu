@@ -16,7 +16,8 @@
 // of the prefix.  Nothing that a CTA reads is written before every CTA has read it: the last
 // CTA to finish (a ticket in free_state[2], put back to 0) updates lens and the ring's state.
 // A call that cannot be served whole (a bad length, a row past the table, too few free blocks,
-// more tokens than the maps hold) raises its bit in *status and changes nothing.
+// more tokens than the maps hold) raises its bit in *status and changes nothing.  A block id outside the pool, in
+// the ring or in a table, is found only when its block is moved: it is moved as -1, and reported.
 //
 // Bound by latency: one extend and one truncate of 128 sequences with 5 new tokens each take 11.2 us in a graph, 16 new
 // prompts of 1 024 tokens 8.6, 2 048 ragged sequences 18.6 (5.2 MB: 0.8 us of reading and writing); a chain of
@@ -222,22 +223,25 @@ __global__ void __launch_bounds__(kMaxThreads) block_tables_kernel(TablesParams 
         const int held = blocks_of(p, len);
         const int pos = len + (i - item0[s]);
         const int j = pos / p.bs, off = pos - j * p.bs;
-        int blk;
-        if (alloc && j >= held) {
-          blk = p.ring[ring_slot(p, head, (int64_t)third[s] + (j - held))];
-          if (off == 0) p.tables[(int64_t)s * p.stride + j] = blk;  // a taken block's first token is new
-        } else {
-          blk = p.tables[(int64_t)s * p.stride + j];
+        const bool take = alloc && j >= held;
+        int blk = take ? p.ring[ring_slot(p, head, (int64_t)third[s] + (j - held))] : p.tables[(int64_t)s * p.stride + j];
+        if (blk < 0 || blk >= p.num_blocks) {
+          blk = -1;
+          raise_status(p.status, B2_DEV_RANGE);
         }
-        const bool ok = blk >= 0 && blk < p.num_blocks;
-        if (!ok) raise_status(p.status, B2_DEV_RANGE);
+        if (take && off == 0) p.tables[(int64_t)s * p.stride + j] = blk;  // a taken block's first token is new
         p.positions[i] = pos;
         p.table_index[i] = s;
-        p.slots[i] = ok ? (int64_t)blk * p.bs + off : -1;
+        p.slots[i] = blk >= 0 ? (int64_t)blk * p.bs + off : -1;
         p.ctx_lens[i] = pos + 1;
       } else {
         int32_t* entry = p.tables + (int64_t)s * p.stride + blocks_of(p, third[s]) + (i - item0[s]);
-        p.ring[ring_slot(p, head, (int64_t)count + i)] = *entry;
+        int blk = *entry;
+        if (blk < 0 || blk >= p.num_blocks) {  // a hole in what the sequence should hold: it stays one
+          blk = -1;
+          raise_status(p.status, B2_DEV_RANGE);
+        }
+        p.ring[ring_slot(p, head, (int64_t)count + i)] = blk;
         *entry = -1;
       }
     }

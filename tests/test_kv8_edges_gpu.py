@@ -221,3 +221,28 @@ def test_map_entries_of_no_token_are_written_by_none(refused, T):
         assert torch.equal(t[0][~touched], b[0][~touched])
     with pytest.raises((IndexError, MemoryError)):
         _lib.check_device_status(DEV, "write")
+
+
+# ------------------------------------------------------------------ ids outside the pool in tables and ring
+@pytest.mark.parametrize("bad", [-1, 12, 1 << 30])
+def test_block_ids_outside_the_pool_are_reported(bad):
+    """truncate over a table with a hole, and extend from a ring with one: the call reports it."""
+    tables, lens = i32([[4, bad, 2], [7, 8, -1]]), i32([40, 32])
+    ring, state = i32([0] * 12), i32([0, 0, 0, 0])
+    kernels.block_tables_truncate(tables, lens, i32([0, 32]), 16, ring, state)
+    with pytest.raises(IndexError):
+        _lib.check_device_status(DEV, "truncate")
+    assert lens.tolist() == [0, 32] and tables.tolist() == [[-1] * 3, [7, 8, -1]]
+    # the hole takes its place in the ring as -1 ...
+    assert state[:2].tolist() == [0, 3] and ring[:3].tolist() == [4, -1, 2]
+    # ... and the sequence that draws it holds no block there
+    m = kernels.block_tables_extend(tables, lens, i32([33, 0]), 33, 16, ring, state)
+    with pytest.raises(IndexError):
+        _lib.check_device_status(DEV, "extend")
+    assert tables[0].tolist() == [4, -1, 2] and (m.slots[16:32] == -1).all() and m.slots[32] == 32
+    ring2 = i32([bad] * 12)
+    tables = i32([[-1, -1]])
+    m = kernels.block_tables_extend(tables, i32([0]), i32([17]), 17, 16, ring2, i32([3, 12, 0, 0]))
+    with pytest.raises(IndexError):
+        _lib.check_device_status(DEV, "extend")
+    assert (tables == -1).all() and (m.slots == -1).all()
