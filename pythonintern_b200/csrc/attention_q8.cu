@@ -566,7 +566,7 @@ q8_attn_kernel(const Q8AttnParams p, int qt, int n_units, int per_group) {
     win.g = from.g;
     win.id = -1;
     if (lane < win.cnt)
-      win.id = __ldg(p.tables + (int64_t)table_row(p, from.u) * p.table_stride + from.block + lane);
+      win.id = p.tables[(int64_t)table_row(p, from.u) * p.table_stride + from.block + lane];
     return win;
   };
   auto advance = [&](Place& pl, int cnt) {
@@ -578,8 +578,8 @@ q8_attn_kernel(const Q8AttnParams p, int qt, int n_units, int per_group) {
     if (lane < win.cnt && !in_pool) raise_status(p.status, B2_DEV_RANGE);
     if (!in_pool) win.id = -1;
     const int64_t at = in_pool ? q8_scale(win.id, p.nkv, win.g) : 0;
-    win.ks = __ldg(p.k_scale + at);
-    win.vs = __ldg(p.v_scale + at);
+    win.ks = p.k_scale[at];
+    win.vs = p.v_scale[at];
   };
 
   // The copies of a step's tiles: every lane 16-byte pieces of K and of V, 512 bytes of the run

@@ -406,8 +406,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       int id_raw;
       auto fetch = [&](int id) {
         id_raw = id;
-        ks_raw = id >= 0 ? __ldg(p.k_scale + (int64_t)id * p.nkv + it.g) : 0.f;
-        vs_raw = id >= 0 ? __ldg(p.v_scale + (int64_t)id * p.nkv + it.g) : 1.f;
+        ks_raw = id >= 0 ? p.k_scale[(int64_t)id * p.nkv + it.g] : 0.f;
+        vs_raw = id >= 0 ? p.v_scale[(int64_t)id * p.nkv + it.g] : 1.f;
       };
       int id_next = id_of(0);
       fetch(id_next);
@@ -617,7 +617,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int64_t tile = (int64_t)max(0, __shfl_sync(0xffffffffu, ids, u)) * p.nkv * (16 * HD) + at;
 #pragma unroll
           for (int i = 0; i < 16 / KEYS; ++i)
-            code[u * (16 / KEYS) + i] = __ldg(reinterpret_cast<const uint4*>(cache + tile + i * KEYS * HD));
+            code[u * (16 / KEYS) + i] = *reinterpret_cast<const uint4*>(cache + tile + i * KEYS * HD);
         }
       };
       int ids = id_of(0), ids_next = id_of(1);

@@ -17,3 +17,13 @@ def test_both_forms_of_extend_refuse_the_same(fn):
                            (dict(state=None), _lib.B2_EINVAL, "together")):
         refused(extend(**kw), code, text)
         assert _lib.last_error().startswith(fn + ":")
+
+
+@pytest.mark.parametrize("source", ["attention_q8.cu", "prefill_q8_tc.cu", "qk_norm_rope.cu", "block_tables.cu", "q8.cuh"])
+def test_kernels_that_begin_early_do_not_load_through_the_read_only_path(source):
+    """Tables, scales and codes may be written by the kernel before, which need not have ended when these begin:
+    ld.global.nc wants memory that nobody writes for as long as the kernel lives."""
+    import os
+    text = open(os.path.join(os.path.dirname(_lib.LIB_PATH), "csrc", source)).read()
+    for word in ("__ldg", "global.nc", "__restrict__"):
+        assert word not in text, word
