@@ -466,7 +466,10 @@ def _norm_rope_args(qkv, nq, nkv, hd, q_weight, k_weight, eps, rope_pos, store_p
         _check(table_index, "table_index", torch.int32, n, dev)
     _check_tables(block_tables)
     _check(cos, "cos", torch.float32, hd, dev)
-    _check(sin, "sin", torch.float32, cos.numel(), dev)
+    _check(sin, "sin", torch.float32, hd, dev)
+    angles = cos.shape
+    if len(angles) != 2 or angles[1] != hd or sin.shape != angles:
+        raise _lib.B2Error(f"cos and sin must be [positions, {hd}], got {tuple(angles)} and {tuple(sin.shape)}")
     _check(q_out, "q_out", qkv.dtype, n * nq * hd, dev)
     return (ptr(qkv), qkv.stride(0) if n > 1 else max(qkv.stride(0), qkv.shape[1]), n, nq, nkv, hd, ptr(q_weight),
             ptr(k_weight), float(eps), ptr(rope_pos), ptr(store_pos), ptr(table_index), ptr(block_tables),

@@ -246,3 +246,40 @@ def test_block_ids_outside_the_pool_are_reported(bad):
     with pytest.raises(IndexError):
         _lib.check_device_status(DEV, "extend")
     assert (tables == -1).all() and (m.slots == -1).all()
+
+
+# ------------------------------------------------------------------ arguments that the wrappers refuse or take
+def _write_args(n=3, nq=4, nkv=2, hd=64, positions=32):
+    qkv = torch.randn(n, (nq + 2 * nkv) * hd, generator=gen(1)).to(DEV, torch.bfloat16)
+    pos = torch.arange(n, dtype=torch.int64, device=DEV)
+    angle = torch.arange(positions)[:, None] / 10000.0 ** (torch.arange(hd // 2) * 2 / hd)
+    cos, sin = (torch.cat([f, f], 1).to(DEV) for f in (angle.cos(), angle.sin()))
+    return dict(qkv=qkv, nq=nq, nkv=nkv, hd=hd, pos=pos, store=None, row=i32([0] * n), tab=i32([[1, 2]]), cos=cos, sin=sin)
+
+
+def _run_write(a, q8, cache=None):
+    """One write into a fresh cache (or the given one): q, and what it wrote."""
+    q = torch.zeros(a["qkv"].shape[0], a["nq"] * a["hd"], dtype=a["qkv"].dtype, device=DEV)
+    head = (a["qkv"], a["nq"], a["nkv"], a["hd"], None, None, 1e-5, a["pos"], a["store"], a["row"], a["tab"], a["cos"],
+            a["sin"], q)
+    if q8:
+        cache = _stored("int8", 4, a["nkv"], a["hd"]) if cache is None else cache
+        kernels.qk_norm_rope_kv_write_q8(*head, *cache, 0)
+    else:
+        cache = list(torch.zeros(2, 1, 4, 16, a["nkv"], a["hd"], dtype=a["qkv"].dtype, device=DEV).unbind(0))
+        kernels.qk_norm_rope_kv_write(*head, *cache, 0)
+    return [q] + cache
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_rotation_tables_of_another_shape_are_refused(q8):
+    """The kernel reads cos and sin as rows of head_dim for as many positions as cos has rows."""
+    a = _write_args()
+    _run_write(a, q8)
+    c, s = a["cos"], a["sin"]
+    for bad in (dict(cos=c[0], sin=s[0]), dict(cos=c.view(-1), sin=s.view(-1)), dict(cos=c[:, :32].contiguous()),
+                dict(cos=c[:, :32].contiguous(), sin=s[:, :32].contiguous()), dict(sin=s[:16]), dict(cos=c[None]),
+                dict(sin=s.view(-1)), dict(cos=torch.cat([c, c], 1), sin=torch.cat([s, s], 1)), dict(sin=s.double())):
+        with pytest.raises(_lib.B2Error):
+            _run_write({**a, **bad}, q8)
+    _lib.check_device_status(DEV, "refusals")
