@@ -471,7 +471,7 @@ def _norm_rope_args(qkv, nq, nkv, hd, q_weight, k_weight, eps, rope_pos, store_p
     if len(angles) != 2 or angles[1] != hd or sin.shape != angles:
         raise _lib.B2Error(f"cos and sin must be [positions, {hd}], got {tuple(angles)} and {tuple(sin.shape)}")
     _check(q_out, "q_out", qkv.dtype, n * nq * hd, dev)
-    return (ptr(qkv), qkv.stride(0) if n > 1 else max(qkv.stride(0), qkv.shape[1]), n, nq, nkv, hd, ptr(q_weight),
+    return (ptr(qkv), _rows_stride(qkv, n, (nq + 2 * nkv) * hd), n, nq, nkv, hd, ptr(q_weight),
             ptr(k_weight), float(eps), ptr(rope_pos), ptr(store_pos), ptr(table_index), ptr(block_tables),
             block_tables.shape[0], block_tables.shape[1])
 
@@ -565,8 +565,9 @@ def _q8_attention_io(q, nq, hd, out):
     return out
 
 
-def _rows_stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _rows_stride(t: torch.Tensor, rows: int, width: int) -> int:
+    """Elements between rows; of a single row, whose stride is any number, its width."""
+    return t.stride(0) if rows > 1 else width
 
 
 def paged_attention_q8(q: torch.Tensor, nq: int, nkv: int, head_dim: int, k_cache: torch.Tensor,
@@ -584,10 +585,10 @@ def paged_attention_q8(q: torch.Tensor, nq: int, nkv: int, head_dim: int, k_cach
     nbytes = _lib.lib().b2_paged_attention_q8_workspace_bytes(n, nq, nkv, head_dim, dtype_code(q.dtype))
     # scratch of this call alone: another stream or graph may run at the same time
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _call("b2_paged_attention_q8", dev, ptr(q), _rows_stride(q), n, nq, nkv, head_dim, ptr(k_cache), ptr(v_cache),
-          ptr(k_scale), ptr(v_scale), code, layer, NB, bs, ptr(block_tables), block_tables.shape[0],
-          block_tables.shape[1], ptr(table_index), ptr(ctx_lens), 1 if compat_pad else 0, float(scale), ptr(out),
-          _rows_stride(out), dtype_code(q.dtype), ptr(ws), nbytes)
+    _call("b2_paged_attention_q8", dev, ptr(q), _rows_stride(q, n, nq * head_dim), n, nq, nkv, head_dim,
+          ptr(k_cache), ptr(v_cache), ptr(k_scale), ptr(v_scale), code, layer, NB, bs, ptr(block_tables),
+          block_tables.shape[0], block_tables.shape[1], ptr(table_index), ptr(ctx_lens), 1 if compat_pad else 0,
+          float(scale), ptr(out), _rows_stride(out, n, nq * head_dim), dtype_code(q.dtype), ptr(ws), nbytes)
     return out
 
 
@@ -606,8 +607,8 @@ def prefill_attention_q8(q: torch.Tensor, nq: int, nkv: int, head_dim: int, k_ca
         _check(seq_ctx0, "seq_ctx0", torch.int32, n_seqs, dev)
     nbytes = _lib.lib().b2_prefill_attention_q8_workspace_bytes(n, nq, nkv, head_dim, n_seqs, dtype_code(q.dtype))
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _call("b2_prefill_attention_q8", dev, ptr(q), _rows_stride(q), n, nq, nkv, head_dim, ptr(k_cache), ptr(v_cache),
-          ptr(k_scale), ptr(v_scale), code, layer, NB, bs, ptr(block_tables), block_tables.shape[0],
-          block_tables.shape[1], ptr(seq_start), ptr(seq_ctx0), n_seqs, float(scale), ptr(out), _rows_stride(out),
-          dtype_code(q.dtype), ptr(ws), nbytes)
+    _call("b2_prefill_attention_q8", dev, ptr(q), _rows_stride(q, n, nq * head_dim), n, nq, nkv, head_dim,
+          ptr(k_cache), ptr(v_cache), ptr(k_scale), ptr(v_scale), code, layer, NB, bs, ptr(block_tables),
+          block_tables.shape[0], block_tables.shape[1], ptr(seq_start), ptr(seq_ctx0), n_seqs, float(scale), ptr(out),
+          _rows_stride(out, n, nq * head_dim), dtype_code(q.dtype), ptr(ws), nbytes)
     return out

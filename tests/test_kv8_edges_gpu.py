@@ -283,3 +283,36 @@ def test_rotation_tables_of_another_shape_are_refused(q8):
         with pytest.raises(_lib.B2Error):
             _run_write({**a, **bad}, q8)
     _lib.check_device_status(DEV, "refusals")
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_a_single_row_may_have_any_stride(q8):
+    a = _write_args(n=1)
+    want = _run_write(a, q8)
+    width = a["qkv"].shape[1]
+    odd = torch.zeros(3, width + 3, dtype=torch.bfloat16, device=DEV)
+    row = torch.as_strided(odd, (1, width), (width + 3, 1))
+    wide = torch.as_strided(odd, (1, width + 3), (width + 3, 1))  # columns behind the heads, an odd number
+    for qkv in (row, wide):
+        qkv[:, :width] = a["qkv"]
+        assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+                   for x, y in zip(_run_write({**a, "qkv": qkv}, q8), want))
+    _lib.check_device_status(DEV, "write")
+
+
+def test_a_single_query_row_may_have_any_stride():
+    nq, nkv, hd, ctx = 4, 2, 64, 40
+    tab, NB = _tables_for([3], 1, 1)
+    cache, t = _stored("int8", NB, nkv, hd), torch.from_numpy(tab).to(DEV)
+    q = torch.randn(1, nq * hd, generator=gen(2)).to(DEV, torch.bfloat16)
+    want = _decode(q, nq, nkv, hd, cache, tab, [ctx], 0.1)
+    pre, _ = _prefill(q, nq, nkv, hd, cache, tab, [1], [ctx - 1], 0.1)
+    wide = torch.zeros(1, nq * hd + 5, dtype=torch.bfloat16, device=DEV)
+    wide[:, :nq * hd] = q
+    out = torch.full((3, nq * hd + 5), 7.0, dtype=torch.bfloat16, device=DEV)
+    kernels.paged_attention_q8(wide, nq, nkv, hd, *cache, 0, t, None, i32([ctx]), False, 0.1, out=out)
+    assert torch.equal(out[:1, :nq * hd], want) and (out[1:] == 7).all() and (out[0, nq * hd:] == 7).all()
+    out.fill_(7)
+    kernels.prefill_attention_q8(wide, nq, nkv, hd, *cache, 0, t, i32([0, 1]), 1, 0.1, seq_ctx0=i32([ctx - 1]), out=out)
+    assert torch.equal(out[:1, :nq * hd], pre) and (out[1:] == 7).all() and (out[0, nq * hd:] == 7).all()
+    _lib.check_device_status(DEV, "attention")
