@@ -27,3 +27,18 @@ def test_kernels_that_begin_early_do_not_load_through_the_read_only_path(source)
     text = open(os.path.join(os.path.dirname(_lib.LIB_PATH), "csrc", source)).read()
     for word in ("__ldg", "global.nc", "__restrict__"):
         assert word not in text, word
+
+
+@pytest.mark.parametrize("kv_dtype", ["int8", "fp8_e4m3"])
+def test_a_pool_that_no_kernel_reads_is_refused_with_its_model(kv_dtype):
+    from pythonintern_b200.config import KVCacheConfig, ModelConfig
+    from pythonintern_b200.model.kv_cache import KVCacheManager
+
+    def manager(heads, kv_heads, kind):
+        cfg = ModelConfig(hidden_dim=32 * heads, num_heads=heads, num_kv_heads=kv_heads, dtype="bfloat16")
+        return KVCacheManager(KVCacheConfig(16, 4, "meta", kv_dtype=kind), cfg, 1)
+
+    with pytest.raises(ValueError, match="16 q heads"):
+        manager(17, 1, kv_dtype)
+    assert manager(32, 2, kv_dtype).pool.quantised  # 16 to 1
+    assert not manager(17, 1, "model").pool.quantised
