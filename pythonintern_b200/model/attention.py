@@ -113,6 +113,8 @@ class DistributedAttention(nn.Module):
         self.v_proj = ColumnParallelLinear(H, config.num_kv_heads * hd, False, rank, world_size, dtype=dt, device=dev)
         self.out_proj = RowParallelLinear(config.num_heads * hd, H, False, rank, world_size, communicator,
                                           dtype=dt, device=dev)
+        if config.qk_norm and hd not in (32, 64, 128):
+            raise ValueError(f"qk_norm needs heads of 32, 64 or 128; got head_dim {hd}")
         # per-head norms, the same weights on every rank
         self.q_norm = RMSNorm(hd, eps=config.rms_norm_eps, device=dev) if config.qk_norm else None
         self.k_norm = RMSNorm(hd, eps=config.rms_norm_eps, device=dev) if config.qk_norm else None

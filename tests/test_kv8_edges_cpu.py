@@ -42,3 +42,18 @@ def test_a_pool_that_no_kernel_reads_is_refused_with_its_model(kv_dtype):
         manager(17, 1, kv_dtype)
     assert manager(32, 2, kv_dtype).pool.quantised  # 16 to 1
     assert not manager(17, 1, "model").pool.quantised
+
+
+def test_norms_of_heads_that_no_kernel_serves_are_refused_with_the_layer():
+    from pythonintern_b200.config import ModelConfig
+    from pythonintern_b200.model.attention import DistributedAttention
+
+    def layer(hd, qk_norm):
+        return DistributedAttention(ModelConfig(hidden_dim=4 * hd, num_heads=4, num_kv_heads=2, dtype="bfloat16",
+                                                max_seq_len=32, qk_norm=qk_norm), 0, device="cpu")
+
+    for hd in (16, 96):
+        with pytest.raises(ValueError, match="qk_norm"):
+            layer(hd, True)
+        assert layer(hd, False).q_norm is None
+    assert layer(64, True).q_norm.weight.shape == (64,)
