@@ -168,7 +168,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     p.seq_start = seq_start;
     if (params.seq_ctx0) p.seq_ctx0 = seq_ctx0;
   }
-  const int n_items = count_pairs(p, QT, lane) * p.nkv;
+  if (blockIdx.x == 0) {  // a seq_start that goes back or leaves the rows is reported, whatever it names
+    bool bad = false;
+    for (int i = threadIdx.x; i < p.n_seqs; i += kThreads)
+      bad |= p.seq_start[i] < 0 || p.seq_start[i + 1] > p.n_rows || p.seq_start[i + 1] < p.seq_start[i];
+    if (bad) raise_status(p.status, B2_DEV_RANGE);
+  }
+  const int pairs = count_pairs(p, QT, lane);
+  // sequences that fit the rows have at most (len / QT + 2) / 2 pairs each; more: nothing is computed
+  if (pairs < 0 || pairs > p.n_rows / QT / 2 + p.n_seqs + 1) return;
+  const int n_items = pairs * p.nkv;
   if ((int)blockIdx.x >= n_items) return;  // nothing allocated yet
 
   if (threadIdx.x == 0) {

@@ -316,3 +316,22 @@ def test_a_single_query_row_may_have_any_stride():
     kernels.prefill_attention_q8(wide, nq, nkv, hd, *cache, 0, t, i32([0, 1]), 1, 0.1, seq_ctx0=i32([ctx - 1]), out=out)
     assert torch.equal(out[:1, :nq * hd], pre) and (out[1:] == 7).all() and (out[0, nq * hd:] == 7).all()
     _lib.check_device_status(DEV, "attention")
+
+
+@pytest.mark.parametrize("nq,nkv,T", [(32, 16, 450), (4, 2, 20)])
+def test_a_seq_start_that_leaves_the_rows_or_goes_back_is_reported(nq, nkv, T):
+    """In the tcgen05 kernel (450 rows) and the other one; where it names more tokens than there are rows, nothing is
+    computed."""
+    hd = 128
+    tab, NB = _tables_for([T // 16 + 2] * 3, 1, 1)
+    cache, t = _stored("int8", NB, nkv, hd), torch.from_numpy(tab).to(DEV)
+    q = torch.randn(T, nq * hd, generator=gen(2)).to(DEV, torch.bfloat16)
+    half = T // 2
+    for start, nothing in (([0, 1 << 30, 1 << 30, 1 << 30], True), ([0, 2 ** 31 - 1, 0, T], False),
+                           ([0, T, half, T], False), ([0, half, half - 1, half], False), ([-5, half, half, T], False),
+                           ([0, half, T, T + 1], False)):
+        out = torch.full((T, nq * hd), 7.0, dtype=torch.bfloat16, device=DEV)
+        kernels.prefill_attention_q8(q, nq, nkv, hd, *cache, 0, t, i32(start), 3, 0.1, out=out)
+        with pytest.raises(IndexError):
+            _lib.check_device_status(DEV, "prefill")
+        assert torch.isfinite(out).all() and (not nothing or (out == 7).all())
