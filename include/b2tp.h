@@ -322,7 +322,8 @@ int b2_kv_read_q8(const void* k_cache, const void* v_cache, const float* k_scale
  * ctx_lens (seq_start, seq_ctx0), so there is no split count.  workspace: at least
  * *_workspace_bytes() bytes, in any state; calls that may overlap on the GPU need one each.
  * A row that sees no key gives zeros; rows behind the last sequence of a prefill are left as
- * they were.  A seq_start that goes back or leaves [0, n_rows] raises B2_DEV_RANGE, and no such sequence is computed.  Keys behind a row's context are never used, whatever their codes and scales. */
+ * they were.  A seq_start that goes back or leaves [0, n_rows] raises B2_DEV_RANGE, and no such sequence
+ * is computed.  Keys behind a row's context are never used, whatever their codes and scales. */
 size_t b2_paged_attention_q8_workspace_bytes(int n_rows, int nq, int nkv, int head_dim, int dtype);
 int b2_paged_attention_q8(const void* q, int64_t ld_q, int n_rows, int nq, int nkv, int head_dim, const void* k_cache,
                           const void* v_cache, const float* k_scale, const float* v_scale, int cache_dtype, int layer,

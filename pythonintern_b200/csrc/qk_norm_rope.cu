@@ -294,6 +294,7 @@ __device__ __forceinline__ void tile_block(const NormRopeParams& p, int64_t bloc
   const bool goes_on = mine > 0 && off > 0 && row_before == row && pos_before + 1 == at.pos;
   const unsigned on = __ballot_sync(0xffffffffu, there && goes_on);
   unsigned begins = __ballot_sync(0xffffffffu, there && lane < p.chunk && at.slot_ok && !goes_on);
+  const unsigned good = __ballot_sync(0xffffffffu, there && at.rope_ok);
   const bool norm = is_k && p.k_weight != nullptr;
   float2 wl[4], wh[4];
   if (norm) {
@@ -303,6 +304,7 @@ __device__ __forceinline__ void tile_block(const NormRopeParams& p, int64_t bloc
   for (; begins; begins &= begins - 1) {
     const int b = __ffs(begins) - 1, t = t0 + b;
     const int len = b == 31 ? 1 : __ffs(~(on >> (b + 1)));  // the run's tokens: 1 and those that go on
+    if (!(good >> b & ((1u << len) - 1))) continue;  // none to be stored: the tile stays as it is
     const int first = __shfl_sync(0xffffffffu, off, b);
     const int64_t blk = __shfl_sync(0xffffffffu, at.block, b);
     float2 lo[ITERS][4], hi[ITERS][4];

@@ -335,3 +335,44 @@ def test_a_seq_start_that_leaves_the_rows_or_goes_back_is_reported(nq, nkv, T):
         with pytest.raises(IndexError):
             _lib.check_device_status(DEV, "prefill")
         assert torch.isfinite(out).all() and (not nothing or (out == 7).all())
+
+
+# ------------------------------------------------------------------ positions in the cache and in the rotation tables
+def _tokens(lens, ctx0, positions, nq=4, nkv=2, hd=64):
+    a = _write_args(sum(lens), nq, nkv, hd, positions)
+    a["pos"] = torch.cat([torch.arange(c, c + n) for c, n in zip(ctx0, lens)]).to(DEV)
+    a["row"] = torch.arange(len(lens)).repeat_interleave(torch.tensor(lens)).to(DEV, torch.int32)
+    width = max(-(-(c + n) // 16) for c, n in zip(ctx0, lens))
+    a["tab"] = torch.randperm(width * len(lens), generator=gen(4)).to(DEV, torch.int32).view(len(lens), width)
+    return a
+
+
+def _write_into(a, q8, rows=slice(None)):
+    NB = a["tab"].numel()
+    if q8:
+        cache = _stored("int8", NB, a["nkv"], a["hd"], seed=3)
+    else:
+        cache = list(torch.full((2, 1, NB, 16, a["nkv"], a["hd"]), 3.0, dtype=torch.bfloat16, device=DEV).unbind(0))
+    q = torch.full((a["qkv"].shape[0], a["nq"] * a["hd"]), 9.0, dtype=torch.bfloat16, device=DEV)
+    some = {k: a[k][rows].contiguous() for k in ("qkv", "pos", "row")}
+    store = None if a["store"] is None else a["store"][rows].contiguous()
+    part = q[rows].contiguous()
+    fn = kernels.qk_norm_rope_kv_write_q8 if q8 else kernels.qk_norm_rope_kv_write
+    fn(some["qkv"], a["nq"], a["nkv"], a["hd"], None, None, 1e-5, some["pos"], store, some["row"], a["tab"], a["cos"],
+       a["sin"], part, *cache, 0)
+    q[rows] = part
+    return [q] + cache
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("positions", [20, 32, 33, 40])
+def test_tokens_past_the_rotation_tables_leave_no_trace(q8, positions):
+    """Their q rows, slots and blocks stay as they were, and all other tokens are written as without them."""
+    a = _tokens([5, 20, 3], [0, 25, 7], positions)
+    good = a["pos"] < positions
+    want = _write_into(a, q8, good)
+    _lib.check_device_status(DEV, "write")
+    got = _write_into(a, q8)
+    with pytest.raises(IndexError):
+        _lib.check_device_status(DEV, "write")
+    assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(got, want))
