@@ -365,6 +365,20 @@ def _write_into(a, q8, rows=slice(None)):
 
 
 @pytest.mark.parametrize("q8", [False, True])
+def test_tokens_are_rotated_by_one_position_and_stored_at_another(q8):
+    """store_pos gives the slots, rope_pos the angles: the same, bit for bit, as tables whose rows are put in the
+    order of the slots."""
+    a = _tokens([20, 15, 33, 1], [0, 25, 64, 48], 100)
+    order = torch.randperm(100, generator=gen(7)).to(DEV)
+    split = {**a, "pos": order[a["pos"]], "store": a["pos"]}
+    assert (split["pos"] != split["store"]).any()
+    joint = {**a, "cos": a["cos"][order].contiguous(), "sin": a["sin"][order].contiguous()}
+    assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+               for x, y in zip(_write_into(split, q8), _write_into(joint, q8)))
+    _lib.check_device_status(DEV, "write")
+
+
+@pytest.mark.parametrize("q8", [False, True])
 @pytest.mark.parametrize("positions", [20, 32, 33, 40])
 def test_tokens_past_the_rotation_tables_leave_no_trace(q8, positions):
     """Their q rows, slots and blocks stay as they were, and all other tokens are written as without them."""
@@ -376,3 +390,32 @@ def test_tokens_past_the_rotation_tables_leave_no_trace(q8, positions):
     with pytest.raises(IndexError):
         _lib.check_device_status(DEV, "write")
     assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(got, want))
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("what", ["row", "block", "position"])
+def test_tokens_without_a_slot_leave_the_others_right(q8, what):
+    """A sequence whose table row or block is not there, and tokens of no position behind the last one."""
+    a = _tokens([5, 20, 3, 4], [0, 12, 7, 16], 64)
+    good = torch.ones(32, dtype=torch.bool, device=DEV)
+    if what == "row":
+        a["row"][-4:] = 4
+        good[-4:] = False
+    elif what == "block":
+        a["tab"][1, 1] = 1 << 20  # positions 16..31 of the second sequence, 12..31
+        good[9:25] = False
+    else:
+        a["pos"][-4:] = -1
+        good[-4:] = False
+    want = _write_into(a, q8, good)
+    want_q = _write_into({**a, "tab": torch.arange(8, device=DEV, dtype=torch.int32).view(4, 2),
+                          "row": a["row"].clamp(max=3)}, q8)[0]
+    if what == "position":
+        with pytest.raises(IndexError):
+            _lib.check_device_status(DEV, "write")
+    _lib.check_device_status(DEV, "write")
+    got = _write_into(a, q8)
+    with pytest.raises(IndexError):
+        _lib.check_device_status(DEV, "write")
+    assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(got[1:], want[1:]))
+    assert torch.equal(got[0], want_q)  # a token without a slot still has its q, one without a position does not
