@@ -287,11 +287,12 @@ int b2_block_tables_truncate(int32_t* block_tables, int n_seqs, int table_stride
  *   scale = max|x| / 127 (B2_I8) or / 448 (B2_E4M3), 0 where that is below 2^-126;
  *   a run that begins inside a block keeps the block's scale if it is larger, else the codes
  *   in the slots before the run are rounded again: code * old_scale / scale;
- *   code = x / scale to nearest even, saturating.
+ *   code = x * (1 / scale) in float32 to nearest even, saturating.
  * A value that is not finite makes the tile's scale NaN until the block is begun anew and its run's
  * codes 0.  No NaN code is ever stored, and readers expect none within a sequence: one that is put there
- * by other means may reach rows that do not see it.  Slots behind the run keep their codes.  Two runs of
- * one call must not meet in one block. */
+ * by other means may reach rows that do not see it.  Slots behind the run keep their codes.  What a token
+ * did to a block's scale and history stays when its sequence is cut back before it.  Two runs of one call must
+ * not meet in one block; a position outside the tables in the middle of a run parts it in two. */
 int b2_qk_norm_rope_kv_write(const void* qkv, int64_t ld_qkv, int n_tokens, int nq, int nkv, int head_dim,
                              const float* q_weight, const float* k_weight, float eps, const int64_t* rope_pos,
                              const int64_t* store_pos, const int32_t* table_index, const int32_t* block_tables,

@@ -35,7 +35,8 @@
 //    float32 up to 2^-22 of an element.
 // Softmax statistics are float32: l = sum 2^(s - m), and P = 2^(s - m) vs 2^(m - m2) is rounded to
 // float16 (to two terms for float32 queries).  The second reference m2 follows the largest
-// s + log2(vs), so a scale that differs by orders of magnitude between blocks costs no precision.
+// s + log2(vs), so a scale that differs by orders of magnitude between blocks costs no precision; it stays
+// within 2^100 of m, however loud the keys of V tiles of zeros are.
 // References move only when a value would pass 2^15 and then to where it is 2^8, so the common
 // step needs no maximum across lanes, only one vote.
 #include "q8.cuh"
@@ -1108,7 +1109,7 @@ int check_q8_pointers(const char* name, const Q8AttnParams& p, int dtype) {
 // head, one per SM at a time, 22 ns per key; this file's kernel cuts all tiles of 32 columns evenly over
 // the SMs, 13 ns per key and tile of an SM.  Both are proportional to the context, which only the
 // device knows, so the rule compares tiles with rounds of items.  Both sides measured (us, here / tcgen05):
-//   heads 32/8, 1 sequence, 32 000 keys:    64 tokens  220 / 722,  128  395 / 723,  256  746 / 726
+//   heads 32/8, 1 sequence, 32 000 keys:    64 tokens  210 / 722,  128  375 / 723,  256  746 / 726
 //   heads 32/8, 8 sequences, 4 000 keys:    16 tokens   86 /  94,   32  137 /  76,  256  796 / 203
 //   heads  8/8, 64 sequences, 1 000 keys:   16 tokens   58 / 107,   64  165 / 110,  256  507 / 139
 //   heads  8/1, 64 sequences, 1 000 keys:    8 tokens   45 /  29,   16   65 /  26,   64  153 /  35

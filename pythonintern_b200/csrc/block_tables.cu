@@ -19,8 +19,8 @@
 // more tokens than the maps hold) raises its bit in *status and changes nothing.  A block id outside the pool, in
 // the ring or in a table, is found only when its block is moved: it is moved as -1, and reported.
 //
-// Bound by latency: one extend and one truncate of 128 sequences with 5 new tokens each take 11.2 us in a graph, 16 new
-// prompts of 1 024 tokens 8.6, 2 048 ragged sequences 18.6 (5.2 MB: 0.8 us of reading and writing); a chain of
+// Bound by latency: one extend and one truncate of 128 sequences with 5 new tokens each take 12.2 us in a graph, 16 new
+// prompts of 1 024 tokens 9.5, 2 048 ragged sequences 20.0 (5.2 MB: 0.8 us of reading and writing); a chain of
 // loads, scan, bisection, dependent loads and stores, and the ticket, twice.
 #include <algorithm>
 #include <mutex>
@@ -377,7 +377,7 @@ int b2_block_tables_truncate(int32_t* block_tables, int n_seqs, int table_stride
   p.state = free_state;
   p.status = status;
   // What comes back is known on the device alone: at most the whole pool, most often a block or two per
-  // sequence.  One thread per 8 sequences is enough for the latter, and the grid walks what there is.
+  // sequence.  The grid has room for 32 blocks of each at once and walks what there is.
   return b2::launch<false>(p, std::min<int64_t>(num_blocks, 32 * (int64_t)n_seqs), stream);
 }
 

@@ -689,12 +689,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 }  // namespace
 }  // namespace pftc
 
-// Launches the tensor-core prefill attention over the 8-bit cache (bf16 q, head_dim 128).
-// k_cache ... v_scale are those of the layer.  Returns B2_ENOTSUP, launching nothing, for shapes
-// it does not serve.
 // Heads to a kv head that the kernel is compiled for.
 bool prefill_q8_tc_serves(int rep) { return (rep >= 1 && rep <= 8) || rep == 12 || rep == 16; }
 
+// Launches the tensor-core prefill attention over the 8-bit cache (bf16 q, head_dim 128).
+// k_cache ... v_scale are those of the layer.  Returns B2_ENOTSUP, launching nothing, for shapes
+// it does not serve.
 int prefill_attention_q8_tc(const void* q, int64_t ld_q, int n_rows, int nq, int nkv, const uint8_t* k_cache,
                             const uint8_t* v_cache, const float* k_scale, const float* v_scale, int cache_dtype,
                             int num_blocks, const int32_t* tables, int table_stride, const int32_t* seq_start,

@@ -146,7 +146,7 @@ class KVCacheManager:
         self.block_tables: Dict[str, BlockTable] = {}
         num_local_kv_heads = max(1, model_config.num_kv_heads // world_size)
         device = config.device if config.device not in ("cpu", None) else "cuda"
-        group = model_config.num_heads // model_config.num_kv_heads
+        group = model_config.num_queries_per_kv
         if config.kv_dtype != "model" and group > 16:
             raise ValueError(f"a KV pool of {config.kv_dtype} serves up to 16 q heads to a kv head; the model has {group}")
         self.pool = PhysicalKVCachePool(
